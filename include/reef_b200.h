@@ -67,7 +67,8 @@ int reef_b200_check_device(void);
  * the last call:
  *   0x101..0x106  a bounded wait gave up (TMA stage full / empty,
  *                 accumulator full / empty, the MMA drain, a peer's flag);
- *   0x201         a decode or embedding position outside the cache / table;
+ *   0x201         a decode, draft or embedding position outside the cache /
+ *                 table;
  *   0x202         a token id outside the vocabulary;
  *   0x301         a float product or sum that is not finite (the engine
  *                 throws std::overflow_error there). */
@@ -130,6 +131,16 @@ int reef_b200_gemm_w8a8(size_t rows, size_t in, size_t out, const int8_t* x_q,
 int reef_b200_rmsnorm_quant(size_t rows, size_t width, float eps, const float* x,
                             const float* gain, int8_t* x_q, float* x_scale,
                             reef_b200_stream_t stream);
+
+/* The residual's addition and the pre-norm in one pass: h = x + residual (one
+ * rounded add per element), then reef_b200_rmsnorm_quant of h, the same bits
+ * as the two calls without h being read back.  x, residual, h [rows][width]
+ * fp32 (h may be x or residual), gain [width], x_q [rows][width] int8, x_scale
+ * [rows]; width a multiple of 32, at most 16384; x, residual, gain and h
+ * 16-byte aligned, x_q 4-byte (REEF_B200_ERR_ALIGNMENT). */
+int reef_b200_add_rmsnorm_quant(size_t rows, size_t width, float eps, const float* x,
+                                const float* residual, const float* gain, float* h, int8_t* x_q,
+                                float* x_scale, reef_b200_stream_t stream);
 
 /* Gate/up projection of a SwiGLU MLP with the activation in the GEMM
  * epilogue (no counterpart in reef, whose GPT-Neo MLP is GELU; the Llama
@@ -291,6 +302,30 @@ int reef_b200_matvec_rows_f32(size_t out, size_t in, const float* w, const float
  * uint32).  Ties give the lowest index; a NaN never wins unless it is x[0]
  * (the engine's scan then keeps 0).  n in [1, 2^32 - 1]. */
 int reef_b200_argmax_f32(size_t n, const float* x, uint32_t* index, reef_b200_stream_t stream);
+/* Token sampling (no counterpart in reef, which chooses greedily).  Per row of
+ * logits [rows][n] fp32, with temperature T and a uniform number u in [0, 1):
+ *   w_i = exp((x_i - max x) / T);
+ *   order: largest value first, equal values by index;
+ *   kept: the first top_k of the order; of those the shortest prefix whose
+ *     mass reaches top_p of theirs (rank r stays while the mass before it is
+ *     < top_p * their total; the first always stays); of those w_i >= min_p;
+ *   index: the first i, in index order, at which the running sum of the kept
+ *     w exceeds u times their total; prob: w_i over that total (may be NULL).
+ * temperature, top_p, min_p [rows] fp32, top_k [rows] int32 and u [rows] fp32
+ * on the device.  A NULL array turns that filter off (temperature: 1), and so
+ * do top_k <= 0 or >= n, top_p >= 1 and min_p <= 0 in its row; NaN counts as
+ * off, min_p above 1 as 1, u below 0 or NaN as 0 and u from 1 up as the last
+ * kept.  T not above 0 (NaN among it): the first largest logit, prob 1.  A NaN
+ * logit counts as -inf, and -inf is never chosen; with +inf in a row only its
+ * +infs weigh.  A row without any logit above -inf gives REEF_B200_NO_TOKEN
+ * and prob 0.  Sums are exact (weights rounded once to 2^-43), so the same
+ * call always gives the same token.  n <= 2^20, rows <= 2^24
+ * (REEF_B200_ERR_TOO_LARGE). */
+#define REEF_B200_NO_TOKEN 0xffffffffu
+int reef_b200_sample_f32(size_t rows, size_t n, const float* logits, const float* temperature,
+                         const int32_t* top_k, const float* top_p, const float* min_p,
+                         const float* u, uint32_t* index, float* prob,
+                         reef_b200_stream_t stream);
 /* embedding_f32 (kernels.hpp:81-84; the engine's lookup_token_embeddings +
  * add_position_embeddings, embedding.hpp:31-66) for `count` tokens:
  * y[t][c] = wte[ids[t]][c] + wpe[first_position + t][c], one rounded float
@@ -448,6 +483,63 @@ int reef_b200_decode_attn_i8(size_t batch, size_t heads_q, size_t heads_kv, size
                              const float* k_scale, const int8_t* v_cache, const float* v_scale,
                              void* workspace, size_t workspace_bytes, float* out,
                              reef_b200_stream_t stream);
+
+/* ---- drafted tokens over the int8 KV cache ------------------------------ */
+
+/* A pass that checks drafted tokens runs several new tokens of a sequence at
+ * once (reef decodes one at a time; no counterpart there).  Sequence b has
+ * lens[b] committed rows in the cache and draft_lens[b] (NULL: drafts) drafted
+ * tokens, whose keys and values stand at rows lens[b] + t.  They form a tree:
+ * parents[b][t] is the drafted token that t follows, an earlier one, or -1
+ * (any value that is not an earlier node counts as -1); NULL: a chain (t - 1).
+ * Node 0 is the root, the last token already chosen.  drafts <= 64
+ * (REEF_B200_ERR_TOO_LARGE).  All arrays are on the device, int32.
+ *
+ * reef_b200_tree_attn_i8: reef_b200_decode_attn_i8's head for every drafted
+ * token, each seeing the committed rows, itself and its ancestors.  q8 [batch]
+ * [drafts][heads_q][128] + q_scale [batch][drafts][heads_q]; caches, scales,
+ * max_len and alignment as there (any heads_q that is a multiple of heads_kv);
+ * out [batch][drafts][heads_q][128] fp32, rows past a sequence's drafts left as
+ * they are.  The output is accurate to fp32 (P is not rounded to 16 bits).  A
+ * sequence with lens[b] + draft_lens[b] > max_len, or a negative length,
+ * records 0x201 in the device error word and is left out.  Keys that a query
+ * does not see add nothing, whatever their scales hold.  batch <= 2048
+ * (REEF_B200_ERR_TOO_LARGE).  workspace: 16-byte aligned, at least
+ * reef_b200_tree_attn_workspace_bytes(); calls that may run at once need one
+ * each. */
+size_t reef_b200_tree_attn_workspace_bytes(size_t batch, size_t drafts, size_t heads_q,
+                                           size_t heads_kv, size_t max_len);
+int reef_b200_tree_attn_i8(size_t batch, size_t drafts, size_t heads_q, size_t heads_kv,
+                           size_t head_dim, size_t max_len, const int32_t* lens,
+                           const int32_t* draft_lens, const int32_t* parents, float sm_scale,
+                           const int8_t* q8, const float* q_scale, const int8_t* k_cache,
+                           const float* k_scale, const int8_t* v_cache, const float* v_scale,
+                           void* workspace, size_t workspace_bytes, float* out,
+                           reef_b200_stream_t stream);
+/* The accepted path of each tree: from cur = 0, the next cur is the lowest c >
+ * cur with parents[b][c] = cur and tokens[b][c] = chosen[b][cur] (tokens: the
+ * drafted ids; chosen[b][t]: the id the model chose after node t), until there
+ * is none.  path [batch][drafts]: the nodes passed, then -1; accepted [batch]:
+ * how many; next [batch]: chosen of the last one, the token that follows.  A
+ * sequence without drafts: accepted 0, next REEF_B200_NO_TOKEN. */
+int reef_b200_tree_accept(size_t batch, size_t drafts, const int32_t* draft_lens,
+                          const int32_t* parents, const uint32_t* tokens, const uint32_t* chosen,
+                          int32_t* path, int32_t* accepted, uint32_t* next,
+                          reef_b200_stream_t stream);
+/* The cache compacted to a path: row lens[b] + i := row lens[b] + path[b][i]
+ * for i < accepted[b], of K, V and their scales, in every KV head and layer
+ * (`layers` caches [batch][heads_kv][max_len][128] and scales [batch][heads_kv]
+ * [max_len] back to back); every source is read before any row is written, so
+ * a path may be in any order and name a row twice.  new_lens[b] = lens[b] +
+ * accepted[b] (not lens itself: REEF_B200_ERR_INVALID).  A path entry outside
+ * [0, drafts), a row outside the cache or a count outside [0, drafts] records
+ * 0x201 and leaves that sequence as it is (new_lens[b] = lens[b]).  Caches
+ * 16-byte aligned. */
+int reef_b200_kv_compact_i8(size_t layers, size_t batch, size_t heads_kv, size_t head_dim,
+                            size_t max_len, size_t drafts, const int32_t* lens,
+                            const int32_t* path, const int32_t* accepted, int8_t* k_cache,
+                            float* k_scale, int8_t* v_cache, float* v_scale, int32_t* new_lens,
+                            reef_b200_stream_t stream);
 
 /* ---- tensor parallelism (new: reef runs on one core) -------------------- */
 

@@ -83,6 +83,12 @@ SIGNATURES = {
     "reef_b200_decode_attn_workspace_bytes": ([_sz, _sz, _sz], _sz),
     "reef_b200_decode_attn_i8": ([_sz, _sz, _sz, _sz, _sz, _p, _sz, C.c_float] + [_p] * 7
                                  + [_sz, _p, _p], _i),
+    "reef_b200_sample_f32": ([_sz, _sz] + [_p] * 9, _i),
+    "reef_b200_add_rmsnorm_quant": ([_sz, _sz, C.c_float] + [_p] * 7, _i),
+    "reef_b200_tree_attn_workspace_bytes": ([_sz] * 5, _sz),
+    "reef_b200_tree_attn_i8": ([_sz] * 6 + [_p] * 3 + [C.c_float] + [_p] * 7 + [_sz, _p, _p], _i),
+    "reef_b200_tree_accept": ([_sz, _sz] + [_p] * 8, _i),
+    "reef_b200_kv_compact_i8": ([_sz] * 6 + [_p] * 9, _i),
     "reef_b200_comm_unique_id_bytes": ([], _sz),
     "reef_b200_comm_unique_id": ([_p, _sz], _i),
     "reef_b200_comm_init": ([_i, _i, _p, C.c_double, _p], _i),

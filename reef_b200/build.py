@@ -11,8 +11,8 @@ epilogues and the exact float kernels depend on IEEE rounding.  -fmad=false
 keeps nvcc from contracting multiply-adds where a result is defined bit for
 bit: reef's operators, the RMSNorm order and the RoPE / SwiGLU values that a
 fused epilogue must reproduce (flash_attn.cu holds the unfused RoPE packing
-the QKV epilogue matches bit for bit).  The decode head, checked within a
-tolerance (FMA_FREE_EXEMPT), keeps nvcc's contraction.
+the QKV epilogue matches bit for bit).  The decode and draft heads, checked
+within a tolerance (FMA_FREE_EXEMPT), keep nvcc's contraction.
 """
 from __future__ import annotations
 
@@ -36,7 +36,7 @@ COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC",
           f"-I{os.path.join(ROOT, 'include')}", f"-I{CSRC}"]
 # translation units whose float results are checked within a tolerance, not
 # bit for bit: nvcc may contract their multiply-adds
-FMA_FREE_EXEMPT = {"decode_attn.cu"}
+FMA_FREE_EXEMPT = {"decode_attn.cu", "tree_attn.cu"}
 
 
 def _nccl_dirs():

@@ -83,6 +83,19 @@ int reef_b200_argmax_f32(size_t n, const float* x, uint32_t* index, reef_b200_st
   return argmax_f32(static_cast<long long>(n), x, index, S(stream));
 }
 
+int reef_b200_sample_f32(size_t rows, size_t n, const float* logits, const float* temperature,
+                         const int32_t* top_k, const float* top_p, const float* min_p,
+                         const float* u, uint32_t* index, float* prob,
+                         reef_b200_stream_t stream) {
+  if (rows == 0) return REEF_B200_OK;
+  if (n == 0 || !logits || !u || !index) return REEF_B200_ERR_INVALID;
+  if (n > static_cast<size_t>(kMaxSampleLogits) || rows > (1u << 24))
+    return REEF_B200_ERR_TOO_LARGE;
+  if (int rc = check_device()) return rc;
+  return sample_f32(static_cast<long long>(rows), static_cast<int>(n), logits, temperature, top_k,
+                    top_p, min_p, u, index, prob, S(stream));
+}
+
 int reef_b200_embedding_f32(size_t width, size_t count, const uint32_t* ids,
                             size_t first_position, size_t vocab, size_t max_positions,
                             const float* wte, const float* wpe, float* y,
@@ -248,6 +261,23 @@ int reef_b200_rmsnorm_quant(size_t rows, size_t width, float eps, const float* x
   if (int rc = check_device()) return rc;
   return rmsnorm_quant(static_cast<long long>(rows), static_cast<int>(width), eps, x, gain, x_q,
                        x_scale, S(stream));
+}
+
+int reef_b200_add_rmsnorm_quant(size_t rows, size_t width, float eps, const float* x,
+                                const float* residual, const float* gain, float* h, int8_t* x_q,
+                                float* x_scale, reef_b200_stream_t stream) {
+  if (rows == 0) return REEF_B200_OK;
+  if (width == 0 || width > 16384 || rows > kMaxDim || !x || !residual || !gain || !h || !x_q ||
+      !x_scale)
+    return REEF_B200_ERR_INVALID;
+  if (width % 32 != 0 ||
+      (reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(residual) |
+       reinterpret_cast<uintptr_t>(gain) | reinterpret_cast<uintptr_t>(h)) % 16 != 0 ||
+      reinterpret_cast<uintptr_t>(x_q) % 4 != 0)
+    return REEF_B200_ERR_ALIGNMENT;
+  if (int rc = check_device()) return rc;
+  return add_rmsnorm_quant(static_cast<long long>(rows), static_cast<int>(width), eps, x, residual,
+                           gain, h, x_q, x_scale, S(stream));
 }
 
 int reef_b200_linear_w8a8_swiglu(size_t rows, size_t in, size_t ffn, const int8_t* x_q,
@@ -582,6 +612,105 @@ int reef_b200_gemm_w8a8_skinny(size_t rows, size_t in, size_t out, const int8_t*
     return REEF_B200_ERR_INVALID;
   return gemm_i8_skinny(static_cast<int>(rows), static_cast<int>(out), static_cast<int>(in), x_q,
                         w, kEpiF32W8A8, x_scale, w_scale, bias, nullptr, y, workspace, S(stream));
+}
+
+}  // extern "C"
+
+extern "C" {
+
+size_t reef_b200_tree_attn_workspace_bytes(size_t batch, size_t drafts, size_t heads_q,
+                                           size_t heads_kv, size_t max_len) {
+  if (batch == 0 || batch > static_cast<size_t>(kMaxTreeBatch) || drafts == 0 ||
+      drafts > static_cast<size_t>(kMaxDrafts) || heads_q == 0 || heads_q > 4096 ||
+      heads_kv == 0 || heads_q % heads_kv != 0 || batch * heads_kv > 65535 || max_len == 0 ||
+      max_len > (1u << 24))
+    return 0;
+  return tree_attn_workspace_bytes();
+}
+
+int reef_b200_tree_attn_i8(size_t batch, size_t drafts, size_t heads_q, size_t heads_kv,
+                           size_t head_dim, size_t max_len, const int32_t* lens,
+                           const int32_t* draft_lens, const int32_t* parents, float sm_scale,
+                           const int8_t* q8, const float* q_scale, const int8_t* k_cache,
+                           const float* k_scale, const int8_t* v_cache, const float* v_scale,
+                           void* workspace, size_t workspace_bytes, float* out,
+                           reef_b200_stream_t stream) {
+  if (batch == 0 || drafts == 0) return REEF_B200_OK;
+  if (head_dim != 128 || heads_q == 0 || heads_q > 4096 || heads_kv == 0 ||
+      heads_q % heads_kv != 0 || max_len == 0 || !lens || !q8 || !q_scale || !k_cache ||
+      !k_scale || !v_cache || !v_scale || !workspace || !out)
+    return REEF_B200_ERR_INVALID;
+  if (drafts > static_cast<size_t>(kMaxDrafts) || batch > static_cast<size_t>(kMaxTreeBatch) ||
+      batch * heads_kv > 65535 || max_len > (1u << 24))
+    return REEF_B200_ERR_TOO_LARGE;
+  // TMA and the bulk copies want 16-byte bases and whole 16-byte groups of
+  // scales; q is read as words, the workspace and out as 16-byte vectors
+  if (max_len % 4 != 0 ||
+      (reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) |
+       reinterpret_cast<uintptr_t>(k_scale) | reinterpret_cast<uintptr_t>(v_scale) |
+       reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(out)) % 16 != 0 ||
+      reinterpret_cast<uintptr_t>(q8) % 16 != 0)
+    return REEF_B200_ERR_ALIGNMENT;
+  if (int rc = check_device()) return rc;
+  if (workspace_bytes <
+      reef_b200_tree_attn_workspace_bytes(batch, drafts, heads_q, heads_kv, max_len))
+    return REEF_B200_ERR_INVALID;
+  TreeProblem p{};
+  p.batch = static_cast<int>(batch);
+  p.drafts = static_cast<int>(drafts);
+  p.heads_q = static_cast<int>(heads_q);
+  p.heads_kv = static_cast<int>(heads_kv);
+  p.max_len = static_cast<int>(max_len);
+  p.sm_scale = sm_scale;
+  p.q8 = q8;
+  p.q_scale = q_scale;
+  p.k_cache = k_cache;
+  p.k_scale = k_scale;
+  p.v_cache = v_cache;
+  p.v_scale = v_scale;
+  p.lens = lens;
+  p.draft_lens = draft_lens;
+  p.parents = parents;
+  p.workspace = workspace;
+  p.out = out;
+  PdlScope pdl;  // as reef_b200_decode_attn_i8
+  return tree_attn_i8(p, S(stream));
+}
+
+int reef_b200_tree_accept(size_t batch, size_t drafts, const int32_t* draft_lens,
+                          const int32_t* parents, const uint32_t* tokens, const uint32_t* chosen,
+                          int32_t* path, int32_t* accepted, uint32_t* next,
+                          reef_b200_stream_t stream) {
+  if (batch == 0) return REEF_B200_OK;
+  if (drafts == 0 || !tokens || !chosen || !path || !accepted || !next)
+    return REEF_B200_ERR_INVALID;
+  if (drafts > static_cast<size_t>(kMaxDrafts) || batch > (1u << 24))
+    return REEF_B200_ERR_TOO_LARGE;
+  if (int rc = check_device()) return rc;
+  return tree_accept(static_cast<int>(batch), static_cast<int>(drafts), draft_lens, parents,
+                     reinterpret_cast<const int*>(tokens), reinterpret_cast<const int*>(chosen),
+                     path, accepted, reinterpret_cast<int*>(next), S(stream));
+}
+
+int reef_b200_kv_compact_i8(size_t layers, size_t batch, size_t heads_kv, size_t head_dim,
+                            size_t max_len, size_t drafts, const int32_t* lens,
+                            const int32_t* path, const int32_t* accepted, int8_t* k_cache,
+                            float* k_scale, int8_t* v_cache, float* v_scale, int32_t* new_lens,
+                            reef_b200_stream_t stream) {
+  if (layers == 0 || batch == 0) return REEF_B200_OK;
+  if (heads_kv == 0 || head_dim != 128 || max_len == 0 || drafts == 0 || !lens || !path ||
+      !accepted || !k_cache || !k_scale || !v_cache || !v_scale || !new_lens || new_lens == lens)
+    return REEF_B200_ERR_INVALID;
+  if (drafts > static_cast<size_t>(kMaxDrafts) || layers > (1u << 16) || batch > (1u << 20) ||
+      heads_kv > 4096 || max_len > (1u << 24) || layers * batch * heads_kv > kMaxDim)
+    return REEF_B200_ERR_TOO_LARGE;
+  if ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) % 16 != 0)
+    return REEF_B200_ERR_ALIGNMENT;
+  if (int rc = check_device()) return rc;
+  return kv_compact_i8(static_cast<long long>(layers), static_cast<int>(batch),
+                       static_cast<int>(heads_kv), static_cast<int>(max_len),
+                       static_cast<int>(drafts), lens, path, accepted, k_cache, k_scale, v_cache,
+                       v_scale, new_lens, S(stream));
 }
 
 }  // extern "C"

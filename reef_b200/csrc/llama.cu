@@ -8,6 +8,7 @@
 // GEMM inputs follow reef's rule exactly.
 //
 //   rmsnorm_quant   y = x * (1 / sqrt(mean(x^2) + eps)) * gain  -> int8 + scale
+//   add_rmsnorm_quant h = x + residual, then rmsnorm_quant of h
 //   swiglu_partials y = silu(gate) * up = gate / (1 + e^-gate) * up on the decode
 //                   gate/up GEMM's split-K partials -> int8 + scale
 // One CTA per row; the row stays in registers between the reduction and the
@@ -299,6 +300,78 @@ __global__ void __launch_bounds__(kChunks * 32)
   }
 }
 
+// The residual's addition and the pre-norm in one pass: h = x + residual (one
+// rounded add, written for the next residual), then rmsnorm_quant_kernel's
+// exact steps on it (the same thread layout and summation order), so x_q / xs
+// hold the bits rmsnorm_quant gives on h.  The row stays in registers, so x and
+// residual are read once and h is never read back; h may be x or residual:
+// a thread reads its elements before it writes them, and nobody else reads
+// them.
+template <int P>
+__global__ void __launch_bounds__(kChunks * 32)
+    add_rmsnorm_quant_kernel(int width, float eps, const float* x, const float* residual,
+                             const float* __restrict__ gain, float* h_out,
+                             int8_t* __restrict__ xq, float* __restrict__ xs) {
+  __shared__ float csum[kChunks];
+  __shared__ float cmax[kChunks];
+  const long long row = blockIdx.x;
+  const int c = threadIdx.x >> 5, l = threadIdx.x & 31;
+  const int n4 = width / (4 * kChunks);  // float4 per chunk
+  const long long base = row * width + static_cast<long long>(c) * n4 * 4;  // elements
+  const float4* x4 = reinterpret_cast<const float4*>(x + base);
+  const float4* r4 = reinterpret_cast<const float4*>(residual + base);
+  float4* h4 = reinterpret_cast<float4*>(h_out + base);
+  float4 a[4][P], b[4][P];
+#pragma unroll
+  for (int w = 0; w < 4; ++w)
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      const int idx = l + 32 * w + kChunkThreads * k;
+      if (idx < n4) {
+        a[w][k] = x4[idx];
+        b[w][k] = r4[idx];
+      }
+    }
+#pragma unroll
+  for (int w = 0; w < 4; ++w)
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      const int idx = l + 32 * w + kChunkThreads * k;
+      if (idx < n4) {
+        const float4 p = a[w][k], q = b[w][k];
+        a[w][k] = make_float4(__fadd_rn(p.x, q.x), __fadd_rn(p.y, q.y), __fadd_rn(p.z, q.z),
+                              __fadd_rn(p.w, q.w));
+        h4[idx] = a[w][k];
+      }
+    }
+  const float4* gr = reinterpret_cast<const float4*>(gain) + c * n4;
+  float m = 0.0f;
+  const float cs = chunk_sum_of<P, true>([&](int w, int k, int) { return a[w][k]; }, gr, n4, l,
+                                         b, m);
+  m = warp_max(m);
+  if (l == 0) {
+    csum[c] = cs;
+    cmax[c] = m;
+  }
+  __syncthreads();
+  const float r = 1.0f / sqrtf(chunk_tree(csum) / static_cast<float>(width) + eps);
+  float mm = cmax[0];
+#pragma unroll
+  for (int j = 1; j < kChunks; ++j) mm = fmaxf(mm, cmax[j]);
+  const float mx = mm * r;
+  const float scale = mx > 0.0f ? __fdiv_rn(mx, 127.0f) : 1.0f;
+  if (threadIdx.x == 0) xs[row] = scale;
+  char4* out = reinterpret_cast<char4*>(xq + row * static_cast<long long>(width)) + c * n4;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      const int idx = l + 32 * w + kChunkThreads * k;
+      if (idx < n4) out[idx] = q8x4(scale4(b[w][k], r), scale);
+    }
+  }
+}
+
 // TP>1, pass 1: this rank's chunk sums and max|x * gain| over its columns.
 // x [rows][width_local], width_local = (chunks_local / 8) * width; stats
 // [rows][chunks_local + 1].  One CTA of chunks_local warps per row.
@@ -481,6 +554,19 @@ int reduce_rmsnorm_quant(long long rows, int width, int splits, const int32_t* p
   if (P <= 1) return launch_k(reduce_rmsnorm_quant_kernel<1>, grid, T, 0, stream, width, splits, part, x_scale, w_scale, residual, h, eps, gain, x_q, q_scale);
   if (P <= 2) return launch_k(reduce_rmsnorm_quant_kernel<2>, grid, T, 0, stream, width, splits, part, x_scale, w_scale, residual, h, eps, gain, x_q, q_scale);
   if (P <= 4) return launch_k(reduce_rmsnorm_quant_kernel<4>, grid, T, 0, stream, width, splits, part, x_scale, w_scale, residual, h, eps, gain, x_q, q_scale);
+  return kErrInvalid;
+}
+
+int add_rmsnorm_quant(long long rows, int width, float eps, const float* x, const float* residual,
+                      const float* gain, float* h, int8_t* x_q, float* x_scale,
+                      cudaStream_t stream) {
+  if (rows == 0) return kOk;
+  if (width <= 0 || width % (4 * kChunks) != 0) return kErrInvalid;
+  const dim3 grid(static_cast<unsigned>(rows)), T(kChunks * 32);
+  const int P = per_thread(width);
+  if (P <= 1) return launch_k(add_rmsnorm_quant_kernel<1>, grid, T, 0, stream, width, eps, x, residual, gain, h, x_q, x_scale);
+  if (P <= 2) return launch_k(add_rmsnorm_quant_kernel<2>, grid, T, 0, stream, width, eps, x, residual, gain, h, x_q, x_scale);
+  if (P <= 4) return launch_k(add_rmsnorm_quant_kernel<4>, grid, T, 0, stream, width, eps, x, residual, gain, h, x_q, x_scale);
   return kErrInvalid;
 }
 

@@ -257,6 +257,24 @@ int matvec_rows_f32(long long out, long long in, const float* w, const float* x,
                     cudaStream_t stream);
 int argmax_f32(long long n, const float* x, uint32_t* index, cudaStream_t stream);
 
+// sample.cu -- token sampling (null parameter arrays: that filter is off;
+// temperature 1); prob may be null.  n <= kMaxSampleLogits.
+constexpr long long kMaxSampleLogits = 1 << 20;
+int sample_f32(long long rows, int n, const float* logits, const float* temperature,
+               const int* top_k, const float* top_p, const float* min_p, const float* u,
+               uint32_t* index, float* prob, cudaStream_t stream);
+
+// spec.cu -- after a pass over drafted tokens: the accepted path of each
+// sequence's tree, and the cache compacted to it (drafts <= kMaxDrafts)
+constexpr int kMaxDrafts = 64;
+int tree_accept(int batch, int drafts, const int* draft_lens, const int* parents,
+                const int* tokens, const int* chosen, int* path, int* accepted, int* next,
+                cudaStream_t stream);
+int kv_compact_i8(long long layers, int batch, int heads_kv, int max_len, int drafts,
+                  const int* lens, const int* path, const int* accepted, int8_t* k_cache,
+                  float* k_scale, int8_t* v_cache, float* v_scale, int* new_lens,
+                  cudaStream_t stream);
+
 // gptneo.cu -- reef's float layernorm, bit for bit (one row per CTA)
 int layernorm_exact(long long rows, int width, float eps, const float* x, const float* gain,
                     const float* shift, float* y, cudaStream_t stream);
@@ -310,6 +328,11 @@ int w8a8_epilogue_i32(long long rows, long long out, const int32_t* acc,
 // llama.cu -- fused RMSNorm / SwiGLU + per-token quantisation
 int rmsnorm_quant(long long rows, int width, float eps, const float* x, const float* gain,
                   int8_t* x_q, float* x_scale, cudaStream_t stream);
+// h = x + residual, then rmsnorm_quant on h, in one pass (the same bits as the
+// two); h may be x or residual.  16-byte alignment.
+int add_rmsnorm_quant(long long rows, int width, float eps, const float* x, const float* residual,
+                      const float* gain, float* h, int8_t* x_q, float* x_scale,
+                      cudaStream_t stream);
 // skinny_reduce (kEpiF32W8A8 + residual) into h, then rmsnorm_quant on h, in
 // one pass (one CTA per row): the same h, x_q and scales as the two kernels.
 // part [splits][rows][width] int32; x_q [rows][width]; 16-byte alignment.
@@ -408,5 +431,25 @@ int decode_rope_append_partials(int batch, int heads_q, int heads_kv, int max_le
                                 int8_t* q8, float* q_scale, int8_t* k_cache, float* k_scale,
                                 int8_t* v_cache, float* v_scale, int* lens, cudaStream_t stream);
 int decode_attn_i8(const DecodeProblem& p, cudaStream_t stream);
+
+// tree_attn.cu -- int8 attention of drafted tokens over the same cache
+constexpr int kMaxTreeBatch = 2048;
+struct TreeProblem {
+  int batch, drafts, heads_q, heads_kv, max_len;
+  float sm_scale;
+  const int8_t* q8;       // [B][T][Hq][128]
+  const float* q_scale;   // [B][T][Hq]
+  const int8_t* k_cache;  // [B][Hkv][max_len][128]
+  const float* k_scale;   // [B][Hkv][max_len]
+  const int8_t* v_cache;
+  const float* v_scale;
+  const int* lens;        // [B] committed keys; the drafts' rows follow them
+  const int* draft_lens;  // [B] or null (all T)
+  const int* parents;     // [B][T] or null (a chain)
+  void* workspace;        // tree_attn_workspace_bytes()
+  float* out;             // [B][T][Hq][128]
+};
+size_t tree_attn_workspace_bytes();
+int tree_attn_i8(const TreeProblem& p, cudaStream_t stream);
 
 }  // namespace reef

@@ -28,6 +28,30 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return t.data_ptr()
 
 
+def _take(t: torch.Tensor | None, name: str, dtype, shape, device) -> int | None:
+    """The address of an argument that must be a contiguous CUDA tensor of
+    this type and shape on this device (None passes as NULL)."""
+    if t is None:
+        return None
+    if t.dtype is not dtype and (not isinstance(dtype, tuple) or t.dtype not in dtype):
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    return _ptr(t)
+
+
+def _call_on(device: torch.device, name: str, *args) -> None:
+    """An entry point on `device` and its current stream (the last argument),
+    whichever device is current."""
+    if device.index == torch.cuda.current_device():
+        _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+
+
 def kpad(n: int) -> int:
     return (n + 15) // 16 * 16
 
@@ -67,6 +91,28 @@ def argmax_f32(x: torch.Tensor) -> torch.Tensor:
     idx = torch.empty((1,), dtype=torch.int32, device=x.device)
     _lib.call("reef_b200_argmax_f32", x.numel(), _ptr(x), _ptr(idx), _stream())
     return idx
+
+
+def sample_f32(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor | None = None,
+               top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None,
+               min_p: torch.Tensor | None = None):
+    """One token per row of logits [rows][n] fp32 from the uniform numbers u
+    [rows]: softmax at `temperature` (not above 0: greedy), cut by top_k, then
+    top_p, then min_p, drawn in index order.  The parameters are per row
+    (fp32 [rows]; top_k int32) or None (off).  Returns (index [rows] int32
+    holding uint32 ids, prob [rows] fp32 under the cut distribution); a row
+    without a logit above -inf gives -1 (REEF_B200_NO_TOKEN) and 0."""
+    rows, n = logits.shape
+    dev = logits.device
+    f32, one = torch.float32, (rows,)
+    args = (_take(logits, "logits", f32, (rows, n), dev),
+            _take(temperature, "temperature", f32, one, dev),
+            _take(top_k, "top_k", torch.int32, one, dev), _take(top_p, "top_p", f32, one, dev),
+            _take(min_p, "min_p", f32, one, dev), _take(u, "u", f32, one, dev))
+    index = torch.empty(one, dtype=torch.int32, device=dev)
+    prob = torch.empty(one, dtype=f32, device=dev)
+    _call_on(dev, "reef_b200_sample_f32", rows, n, *args, index.data_ptr(), prob.data_ptr())
+    return index, prob
 
 
 def pack_weight_i8(wt: torch.Tensor) -> torch.Tensor:
@@ -218,3 +264,103 @@ def gemm_w8a8_skinny(x_q, x_scale, w, w_scale, bias=None, in_features: int | Non
     _lib.call("reef_b200_gemm_w8a8_skinny", rows, k, n, _ptr(x_q), _ptr(x_scale), _ptr(w),
               _ptr(w_scale), _ptr(bias), _ptr(ws), ws.numel(), _ptr(y), _stream())
     return y
+
+
+def add_rmsnorm_quant(x: torch.Tensor, residual: torch.Tensor, gain: torch.Tensor,
+                      eps: float = 1e-5, h: torch.Tensor | None = None):
+    """h = x + residual, then the Llama pre-norm of h in int8: returns (h
+    [rows][width] fp32, x_q [rows][width] int8, x_scale [rows]); h may be given,
+    x or residual among them.  The bits of add_f32 and rmsnorm_quant."""
+    rows, width = x.shape
+    dev, f32 = x.device, torch.float32
+    h = torch.empty_like(x) if h is None else h
+    args = (_take(x, "x", f32, (rows, width), dev),
+            _take(residual, "residual", f32, (rows, width), dev),
+            _take(gain, "gain", f32, (width,), dev), _take(h, "h", f32, (rows, width), dev))
+    x_q = torch.empty((rows, width), dtype=torch.int8, device=dev)
+    xs = torch.empty((rows,), dtype=f32, device=dev)
+    _call_on(dev, "reef_b200_add_rmsnorm_quant", rows, width, eps, *args, x_q.data_ptr(),
+             xs.data_ptr())
+    return h, x_q, xs
+
+
+# ---- drafted tokens over the int8 KV cache ---------------------------------------
+
+_IDS = (torch.int32, torch.uint32)
+
+
+def tree_attn_i8(q8: torch.Tensor, q_scale: torch.Tensor, k_cache: torch.Tensor,
+                 k_scale: torch.Tensor, v_cache: torch.Tensor, v_scale: torch.Tensor,
+                 lens: torch.Tensor, parents: torch.Tensor | None = None,
+                 draft_lens: torch.Tensor | None = None, sm_scale: float | None = None,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of drafted tokens over the int8 KV cache.  q8 [batch][drafts]
+    [heads_q][128] int8 + q_scale; caches [batch][heads_kv][max_len][128] int8
+    + scales [batch][heads_kv][max_len]; lens [batch] int32 committed rows, the
+    drafted tokens' own rows right behind them.  Token t of a sequence sees the
+    committed rows, itself and its ancestors under parents [batch][drafts] (None:
+    a chain).  Returns out [batch][drafts][heads_q][128] fp32; rows past
+    draft_lens are left as they are (zeros in an out made here)."""
+    b, t, hq, d = q8.shape
+    _, hkv, max_len, _ = k_cache.shape
+    dev, f32, i8, i32 = q8.device, torch.float32, torch.int8, torch.int32
+    if out is None:
+        make = torch.empty if draft_lens is None else torch.zeros
+        out = make((b, t, hq, d), dtype=f32, device=dev)
+    cache, rows = (b, hkv, max_len, d), (b, hkv, max_len)
+    before = (_take(lens, "lens", i32, (b,), dev),
+              _take(draft_lens, "draft_lens", i32, (b,), dev),
+              _take(parents, "parents", i32, (b, t), dev))
+    after = (_take(q8, "q8", i8, (b, t, hq, d), dev),
+             _take(q_scale, "q_scale", f32, (b, t, hq), dev),
+             _take(k_cache, "k_cache", i8, cache, dev), _take(k_scale, "k_scale", f32, rows, dev),
+             _take(v_cache, "v_cache", i8, cache, dev), _take(v_scale, "v_scale", f32, rows, dev))
+    o = _take(out, "out", f32, (b, t, hq, d), dev)
+    nbytes = _lib.lib().reef_b200_tree_attn_workspace_bytes(b, t, hq, hkv, max_len)
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+    _call_on(dev, "reef_b200_tree_attn_i8", b, t, hq, hkv, d, max_len, *before,
+             d ** -0.5 if sm_scale is None else sm_scale, *after, ws.data_ptr(), ws.numel(), o)
+    return out
+
+
+def tree_accept(tokens: torch.Tensor, chosen: torch.Tensor, parents: torch.Tensor | None = None,
+                draft_lens: torch.Tensor | None = None):
+    """The path of each tree that the model's own choices follow: tokens /
+    chosen [batch][drafts] (the drafted ids; the id chosen after each node), node
+    0 the root.  Returns (path [batch][drafts] int32, -1 behind it, accepted
+    [batch] int32, next [batch], the id that follows the path, in chosen's
+    type)."""
+    b, t = tokens.shape
+    dev, i32 = tokens.device, torch.int32
+    args = (_take(draft_lens, "draft_lens", i32, (b,), dev),
+            _take(parents, "parents", i32, (b, t), dev),
+            _take(tokens, "tokens", _IDS, (b, t), dev), _take(chosen, "chosen", _IDS, (b, t), dev))
+    path = torch.empty((b, t), dtype=i32, device=dev)
+    accepted = torch.empty((b,), dtype=i32, device=dev)
+    following = torch.empty((b,), dtype=chosen.dtype, device=dev)
+    _call_on(dev, "reef_b200_tree_accept", b, t, *args, path.data_ptr(), accepted.data_ptr(),
+             following.data_ptr())
+    return path, accepted, following
+
+
+def kv_compact_i8(k_cache: torch.Tensor, k_scale: torch.Tensor, v_cache: torch.Tensor,
+                  v_scale: torch.Tensor, lens: torch.Tensor, path: torch.Tensor,
+                  accepted: torch.Tensor) -> torch.Tensor:
+    """Moves the accepted drafted rows (tree_accept's path) right behind the
+    committed ones, in place: row lens + i becomes row lens + path[i].  Caches
+    [batch][heads_kv][max_len][128], or [layers][batch]... for every layer's at
+    once.  Returns the new lens (lens + accepted)."""
+    n = 1 if k_cache.dim() == 4 else k_cache.shape[0]
+    b, hkv, max_len, d = k_cache.shape[-4:]
+    t = path.shape[1]
+    dev, f32, i8, i32 = k_cache.device, torch.float32, torch.int8, torch.int32
+    cache = (b, hkv, max_len, d) if k_cache.dim() == 4 else (n, b, hkv, max_len, d)
+    args = (_take(lens, "lens", i32, (b,), dev), _take(path, "path", i32, (b, t), dev),
+            _take(accepted, "accepted", i32, (b,), dev), _take(k_cache, "k_cache", i8, cache, dev),
+            _take(k_scale, "k_scale", f32, cache[:-1], dev),
+            _take(v_cache, "v_cache", i8, cache, dev),
+            _take(v_scale, "v_scale", f32, cache[:-1], dev))
+    new_lens = torch.empty((b,), dtype=i32, device=dev)
+    _call_on(dev, "reef_b200_kv_compact_i8", n, b, hkv, d, max_len, t, *args,
+             new_lens.data_ptr())
+    return new_lens

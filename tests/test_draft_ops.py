@@ -1,0 +1,123 @@
+"""Refusals of the sampling, drafted-token and residual-norm entry points: they
+come back before any CUDA call (no GPU needed)."""
+import ctypes as C
+
+import pytest
+import torch
+
+from reef_b200 import _lib
+from reef_b200 import kernels as K
+
+INVALID, ALIGNMENT, TOO_LARGE = 1, 2, 7
+
+
+@pytest.fixture(scope="module")
+def L():
+    return _lib.lib()
+
+
+P, Q = C.c_void_p(4096), C.c_void_p(8192)  # never dereferenced
+
+
+def test_sample_refusals(L):
+    f = L.reef_b200_sample_f32
+    assert f(0, 0, *[None] * 9) == 0  # no rows: a no-op
+    assert f(1, 0, P, None, None, None, None, P, P, None, None) == INVALID
+    for bad in range(3):
+        a = [P, P, P]
+        a[bad] = None
+        assert f(1, 8, a[0], None, None, None, None, a[1], a[2], None, None) == INVALID
+    assert f(1, (1 << 20) + 1, P, None, None, None, None, P, P, None, None) == TOO_LARGE
+    assert f((1 << 24) + 1, 8, P, None, None, None, None, P, P, None, None) == TOO_LARGE
+
+
+def test_add_rmsnorm_refusals(L):
+    f = L.reef_b200_add_rmsnorm_quant
+    assert f(0, 0, 1e-5, *[None] * 7) == 0
+    assert f(1, 0, 1e-5, *[P] * 6, None) == INVALID
+    assert f(1, 16416, 1e-5, *[P] * 6, None) == INVALID
+    assert f(1, 48, 1e-5, *[P] * 6, None) == ALIGNMENT
+    for i in range(6):
+        a = [P] * 6
+        a[i] = None
+        assert f(1, 64, 1e-5, *a, None) == INVALID
+    for i in range(5):  # x, residual, gain, h: 16 bytes; x_q: 4
+        a = [P] * 6
+        a[i] = C.c_void_p(4096 + (8 if i < 4 else 2))
+        assert f(1, 64, 1e-5, *a, None) == ALIGNMENT
+
+
+def tree(L, b=1, t=2, hq=4, hkv=2, d=128, n=64, lens=P, ws=P, out=P, q=P, k=P, ks=P, v=P, vs=P,
+         nbytes=1 << 40):
+    return L.reef_b200_tree_attn_i8(b, t, hq, hkv, d, n, lens, None, None, 1.0, q, P, k, ks, v, vs,
+                                    ws, nbytes, out, None)
+
+
+def test_tree_attn_refusals(L):
+    assert tree(L, b=0) == 0 and tree(L, t=0) == 0
+    for bad in (dict(hq=0), dict(hkv=0), dict(hq=5), dict(d=64), dict(n=0), dict(hq=8192),
+                dict(lens=None), dict(ws=None), dict(out=None), dict(q=None), dict(k=None),
+                dict(ks=None), dict(v=None), dict(vs=None)):
+        assert tree(L, **bad) == INVALID, bad
+    for bad in (dict(t=65), dict(b=2049), dict(b=2048, hq=64, hkv=64), dict(n=(1 << 24) + 4)):
+        assert tree(L, **bad) == TOO_LARGE, bad
+    off = C.c_void_p(4096 + 4)
+    for bad in (dict(n=62), dict(k=off), dict(v=off), dict(ks=off), dict(vs=off), dict(ws=off),
+                dict(out=off), dict(q=off)):
+        assert tree(L, **bad) == ALIGNMENT, bad
+    need = L.reef_b200_tree_attn_workspace_bytes
+    for bad in ((0, 1, 1, 1, 4), (2049, 1, 1, 1, 4), (1, 0, 1, 1, 4), (1, 65, 1, 1, 4),
+                (1, 1, 0, 1, 4), (1, 1, 3, 2, 4), (1, 1, 1, 0, 4), (1, 1, 1, 1, 0)):
+        assert need(*bad) == 0
+
+
+def test_accept_refusals(L):
+    f = L.reef_b200_tree_accept
+    assert f(0, 0, *[None] * 8) == 0
+    assert f(1, 0, None, None, *[P] * 5, None) == INVALID
+    for i in range(5):
+        a = [P] * 5
+        a[i] = None
+        assert f(1, 4, None, None, *a, None) == INVALID
+    assert f(1, 65, None, None, *[P] * 5, None) == TOO_LARGE
+
+
+def compact(L, layers=1, b=1, hkv=2, d=128, n=64, t=4, a=None, new=Q):
+    return L.reef_b200_kv_compact_i8(layers, b, hkv, d, n, t, *(a or [P] * 7), new, None)
+
+
+def test_compact_refusals(L):
+    assert compact(L, layers=0) == 0 and compact(L, b=0) == 0
+    for bad in (dict(hkv=0), dict(d=64), dict(n=0), dict(t=0), dict(new=None), dict(new=P)):
+        assert compact(L, **bad) == INVALID, bad
+    for i in range(7):
+        a = [P] * 7
+        a[i] = None
+        assert compact(L, a=a) == INVALID
+    for bad in (dict(t=65), dict(layers=65537), dict(n=(1 << 24) + 1),
+                dict(layers=65536, b=1 << 20)):
+        assert compact(L, **bad) == TOO_LARGE, bad
+    for i in (3, 5):
+        a = [P] * 7
+        a[i] = C.c_void_p(4096 + 8)
+        assert compact(L, a=a) == ALIGNMENT
+
+
+def test_wrappers_refuse_tensors_before_any_call():
+    f, i = torch.zeros, torch.int32
+    with pytest.raises(ValueError, match="CUDA"):
+        K.sample_f32(f(2, 5), f(2))
+    with pytest.raises(TypeError, match="logits"):
+        K.sample_f32(f(2, 5, dtype=torch.bfloat16), f(2))
+    with pytest.raises(ValueError, match="CUDA"):
+        K.add_rmsnorm_quant(f(2, 32), f(2, 32), f(32))
+    with pytest.raises(TypeError, match="lens"):
+        K.kv_compact_i8(f(1, 1, 4, 128, dtype=torch.int8), f(1, 1, 4),
+                        f(1, 1, 4, 128, dtype=torch.int8), f(1, 1, 4), f(1), f(1, 2, dtype=i),
+                        f(1, dtype=i))
+    with pytest.raises(ValueError, match="CUDA"):
+        K.tree_accept(f(1, 2, dtype=i), f(1, 2, dtype=i))
+    with pytest.raises(TypeError, match="lens"):
+        K.tree_attn_i8(f(1, 2, 4, 128, dtype=torch.int8), f(1, 2, 4),
+                       f(1, 2, 8, 128, dtype=torch.int8), f(1, 2, 8),
+                       f(1, 2, 8, 128, dtype=torch.int8), f(1, 2, 8), f(1))

@@ -1,0 +1,236 @@
+"""Attention of drafted tokens over the int8 KV cache against a plain
+implementation in 64 bits on the dequantised inputs.
+
+Tolerance, per output element, relative to W = sum p |v| / sum p (what the
+element's terms add up to without cancelling): P goes into the product as two
+bf16 terms, each rounding off by half a step (2^-9 of what is left): 2^-18
+together; exp2 is off by 2 ulp and a score s (log2 units) by four fp32 roundings,
+2^-22 and 2^-22 max|s| of p, in the numerator and in the denominator; every
+fp32 add of the products may lose 2^-23, over n / 64 adds in a warp (two terms
+per 16 of every 128 keys) and a few dozen where warps and CTAs are joined.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from reef_b200 import _lib
+from reef_b200 import kernels as K
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _no_device_errors(cuda_lib):
+    yield
+    K.check_device_error()
+
+
+def rows8(gen, shape, std):
+    x = torch.randn(shape + (128,), generator=gen, device="cuda") * std
+    sc = x.abs().amax(-1) / 127.0
+    return torch.round(x / sc[..., None]).clamp(-127, 127).to(torch.int8), sc
+
+
+def trees(seed, b, t):
+    r = np.random.RandomState(seed)
+    p = np.floor(r.random_sample((b, t)) * np.arange(t)).astype(np.int32)
+    p[:, 0] = -1
+    if t > 3:
+        p[0, 2] = -1  # a second root
+    return p
+
+
+def make(b, t, hq, hkv, max_len, seed, std=1.5):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q8, qs = rows8(g, (b, t, hq), std)
+    k8, ks = rows8(g, (b, hkv, max_len), std)
+    v8, vs = rows8(g, (b, hkv, max_len), 1.0)
+    return dict(q8=q8, q_scale=qs, k_cache=k8, k_scale=ks, v_cache=v8, v_scale=vs)
+
+
+def check(x, lens, parents, draft_lens, out, sm):
+    """Every live row of `out` against 64 bits; rows behind stay -7."""
+    q8, ks, vs = x["q8"], x["k_scale"], x["v_scale"]
+    b, t, hq, _ = q8.shape
+    hkv = ks.shape[1]
+    for i in range(b):
+        n, d = int(lens[i]), t if draft_lens is None else int(draft_lens[i])
+        assert torch.all(out[i, max(d, 0):] == -7.0)
+        if d <= 0:
+            continue
+        sees = torch.zeros((d, n + d), dtype=torch.bool)
+        sees[:, :n] = True
+        for r in range(d):
+            j = r
+            while j >= 0:
+                sees[r, n + j] = True
+                up = j - 1 if parents is None else int(parents[i][j])
+                j = up if up < j else -1
+        sees = sees.cuda()
+        for h in range(hq):
+            kh = h // (hq // hkv)
+            q = q8[i, :d, h].double() * x["q_scale"][i, :d, h, None].double()
+            k = x["k_cache"][i, kh, : n + d].double() * ks[i, kh, : n + d, None].double()
+            v = x["v_cache"][i, kh, : n + d].double() * vs[i, kh, : n + d, None].double()
+            s = torch.where(sees, q @ k.T * sm, -math.inf)
+            p = torch.softmax(s, -1)
+            v = torch.nan_to_num(v) if not torch.isfinite(v).all() else v
+            want, weight = p @ v, p @ v.abs()
+            smax = float(s[sees].abs().max()) * math.log2(math.e)
+            rel = 2.0**-18 + 2 * (1 + smax) * 2.0**-22 + ((n + d) / 64 + 32) * 2.0**-23
+            assert bool(((out[i, :d, h].double() - want).abs() <= rel * weight + 1e-30).all()), \
+                (i, h, float(((out[i, :d, h].double() - want).abs() / weight).max()), rel)
+
+
+def run(x, lens, parents=None, draft_lens=None, sm=None, **kw):
+    b, t, hq, _ = x["q8"].shape
+    dev = lambda a: None if a is None else torch.tensor(np.asarray(a, np.int32), device="cuda")
+    out = torch.full((b, t, hq, 128), -7.0, device="cuda")
+    got = K.tree_attn_i8(**x, lens=dev(lens), parents=dev(parents), draft_lens=dev(draft_lens),
+                         sm_scale=sm, out=out, **kw)
+    assert got is out
+    torch.cuda.synchronize()
+    return out
+
+
+CASES = [
+    # batch, drafts, heads_q, heads_kv, max_len, lens, draft_lens, tree
+    (1, 1, 1, 1, 4, [0], None, False),               # one token, nothing committed
+    (1, 1, 4, 4, 132, [131], None, False),           # the last row of the cache
+    (2, 4, 8, 2, 300, [0, 296], None, True),         # empty and full
+    (3, 7, 4, 1, 520, [127, 128, 250], None, True),  # drafts across a tile's border
+    (3, 5, 6, 2, 260, [121, 5, 255], [5, 0, 1], True),   # three heads a group; no drafts
+    (1, 64, 2, 1, 1024, [901], None, True),          # the widest tree
+    (1, 64, 8, 8, 192, [128], None, False),          # a chain of 64
+    (5, 8, 8, 1, 2048, [2040, 1, 1000, 129, 0], [8, 3, 8, 1, 8], True),
+    (2, 3, 16, 1, 4096, [4000, 77], None, True),     # 48 rows, several row tiles
+    (1, 2, 40, 2, 640, [600], None, False),          # 40 rows of one KV head
+    (300, 2, 2, 1, 256, [(37 * i) % 254 for i in range(300)], None, False),  # more than CTAs
+    (40, 16, 8, 2, 512, [(61 * i) % 497 for i in range(40)], [i % 17 for i in range(40)], True),
+]
+
+
+@pytest.mark.parametrize("b,t,hq,hkv,max_len,lens,draft_lens,tree", CASES)
+def test_against_64_bits(b, t, hq, hkv, max_len, lens, draft_lens, tree):
+    x = make(b, t, hq, hkv, max_len, seed=b + t + hq + max_len)
+    parents = trees(7 * b + t, b, t) if tree else None
+    sm = 1.0 / math.sqrt(128)
+    check(x, lens, parents, draft_lens, run(x, lens, parents, draft_lens, sm), sm)
+
+
+@pytest.mark.parametrize("std,sm", [(0.01, 1.0), (6.0, 0.3), (1.5, 0.0)])
+def test_flat_and_peaked_scores(std, sm):
+    x = make(2, 6, 8, 2, 400, seed=11, std=std)
+    check(x, [390, 17], None, None, run(x, [390, 17], None, None, sm), sm)
+
+
+def test_scales_far_apart():
+    """V scales of 2^-60 to 2^60 in one sequence: P times the scale keeps its range."""
+    x = make(1, 4, 4, 1, 256, seed=3)
+    e = torch.arange(256, device="cuda").float() % 121 - 60
+    x["v_scale"] = torch.exp2(e)[None, None].contiguous()
+    check(x, [250], None, None, run(x, [250], None, None, 0.01), 0.01)
+
+
+@pytest.mark.parametrize("junk", [math.nan, math.inf, -math.inf, 3.4e38])
+def test_rows_nobody_sees_add_nothing(junk):
+    """Scales behind the drafts, and of a sibling's row, that are not numbers."""
+    x = make(2, 4, 8, 1, 260, seed=5)
+    parents = [[-1, 0, 0, 1], [-1, 0, 1, 2]]  # nodes 1 and 2 of sequence 0 are siblings
+    lens = [126, 200]
+    want = run(x, lens, parents, None, 0.1)
+    for c in ("k_scale", "v_scale"):
+        x[c][0, :, 130:] = junk
+        x[c][1, :, 204:] = junk
+    got = run(x, lens, parents, None, 0.1)
+    assert torch.equal(got, want)
+    for c in ("k_scale", "v_scale"):
+        x[c][0, :, 128] = junk  # node 2: seen by itself alone
+    got = run(x, lens, parents, None, 0.1)
+    assert torch.equal(got[0, [0, 1, 3]], want[0, [0, 1, 3]]) and torch.equal(got[1], want[1])
+
+
+def test_parents_that_are_no_earlier_node_count_as_roots():
+    x = make(1, 5, 2, 1, 128, seed=9)
+    assert torch.equal(run(x, [100], [[-1, 1, 7, -5, 2]]), run(x, [100], [[-1, -1, -1, -1, 2]]))
+
+
+def test_a_chain_is_the_default_and_a_single_token_is_decode():
+    x = make(3, 6, 8, 2, 512, seed=21)
+    lens = [500, 3, 128]
+    chain = run(x, lens)
+    assert torch.equal(chain, run(x, lens, [[-1, 0, 1, 2, 3, 4]] * 3))
+    # the existing single-token head on the row that token 5 stands in
+    ws = torch.empty(_lib.lib().reef_b200_decode_attn_workspace_bytes(3, 8, 512),
+                     dtype=torch.uint8, device="cuda")
+    n = torch.tensor([v + 6 for v in lens], dtype=torch.int32, device="cuda")
+    q8, qs = x["q8"][:, 5].contiguous(), x["q_scale"][:, 5].contiguous()
+    out = torch.empty((3, 8, 128), device="cuda")
+    _lib.call("reef_b200_decode_attn_i8", 3, 8, 2, 128, 512, n.data_ptr(), 0, 128**-0.5,
+              q8.data_ptr(), qs.data_ptr(), x["k_cache"].data_ptr(), x["k_scale"].data_ptr(),
+              x["v_cache"].data_ptr(), x["v_scale"].data_ptr(), ws.data_ptr(), ws.numel(),
+              out.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    assert float((chain[:, 5] - out).abs().max()) < 1e-2  # that head's own tolerance
+
+
+def test_same_call_same_bits():
+    x = make(9, 8, 16, 2, 1500, seed=2)
+    lens, par = [(331 * i) % 1490 for i in range(9)], trees(4, 9, 8)
+    first = run(x, lens, par)
+    for _ in range(3):
+        assert torch.equal(run(x, lens, par), first)
+
+
+def test_positions_outside_the_cache_are_reported_and_left_out():
+    x = make(3, 4, 2, 1, 64, seed=1)
+    out = run(x, [60, 61, -1])
+    assert torch.all(out[1:] == -7.0)
+    check({k: v[:1] for k, v in x.items()}, [60], None, None, out[:1], 128**-0.5)
+    with pytest.raises(_lib.ReefError, match="0x201"):
+        K.check_device_error()
+
+
+def test_on_another_stream_and_in_a_graph():
+    x = make(2, 8, 8, 1, 700, seed=31)
+    lens = torch.tensor([690, 333], dtype=torch.int32, device="cuda")
+    want = K.tree_attn_i8(**x, lens=lens)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = K.tree_attn_i8(**x, lens=lens)
+    side.synchronize()
+    assert torch.equal(got, want)
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(K.tree_attn_i8(**x, lens=lens))
+        graphs.append(g)
+    lens.fill_(12)
+    x["q8"].neg_()
+    for g in graphs + graphs:
+        g.replay()
+    torch.cuda.synchronize()
+    want = K.tree_attn_i8(**x, lens=lens)
+    assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+
+
+def test_a_row_of_scales_past_two_to_the_31_bytes():
+    """Offsets of K rows pass 32 bits: the last of 140 sequences x 4 heads x 32768 rows."""
+    b, hkv, max_len = 140, 4, 32768
+    x = make(b, 2, 4, hkv, 4, seed=8)
+    k = torch.zeros((b, hkv, max_len, 128), dtype=torch.int8, device="cuda")
+    assert k.numel() > 1 << 31
+    sc = torch.zeros((b, hkv, max_len), device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(6)
+    full = dict(q8=x["q8"], q_scale=x["q_scale"], k_cache=k, k_scale=sc, v_cache=k.clone(),
+                v_scale=sc.clone())
+    for c, std in (("k", 1.5), ("v", 1.0)):
+        full[c + "_cache"][-1, :, -500:], full[c + "_scale"][-1, :, -500:] = rows8(g, (hkv, 500), std)
+    lens = [0] * (b - 1) + [max_len - 2]
+    draft_lens = [0] * (b - 1) + [2]
+    out = run(full, lens, None, draft_lens)
+    last = {n: v[-1:] for n, v in full.items()}
+    check(last, lens[-1:], None, None, out[-1:], 128**-0.5)
