@@ -15,17 +15,30 @@
 //
 // Exactness.  A draw lands next to a border between two tokens often enough
 // (a vocabulary has 1e5 borders) that sums in float would choose wrongly for
-// one row in a few dozen.  So w is computed in double and held as a 64-bit
-// integer, round(w * 2^43): sums of up to 2^20 of them are exact, hence the
-// same in any order, and nothing depends on the schedule.  The rounding moves a
-// border by 2^-44 * sqrt(n), about 2e-11 of the largest weight.
+// one row in a few dozen.  So w is held as a 64-bit integer, w * 2^43 rounded:
+// sums of up to 2^20 of them are exact, hence the same in any order, and nothing
+// depends on the schedule.  Weights from 2^-20 up ("heavy") are computed in
+// double; of the others 23 bits are all that is left, and float with the
+// constants in two terms gives those.  Together a border moves by about 2^-44 *
+// sqrt(n), 2e-11 of the largest weight.
 //
-// A cluster of C CTAs owns a row: each keeps its slice of the logits in shared
-// memory, so the row is read from HBM once however many passes follow.  The
-// kept set is always "key > cut, or key = cut and index <= cut_index" of the
-// order-preserving 32-bit key of x, so top-k and top-p are radix selections
-// (11 + 11 + 10 bits) over counts or masses, histograms summed over the cluster
-// through distributed shared memory.
+// Passes.  A cluster of C CTAs owns a row: each keeps its slice of the logits in
+// shared memory, so the row is read from HBM once however many passes follow.
+// The first finds the maximum.  The next sums the light weights (a dozen float
+// instructions each) and lists the heavy ones in index order, to be weighed
+// many lanes at a time and to be all that later passes go over: what top-p keeps
+// last weighs more than (1 - top_p) * total / n (the excluded ones are at
+// most n and weigh less), so the list reaches down to half of that.  top-k lists
+// what lies above a bound instead: the k-th largest of the maxima of groups of
+// eight logits, from a histogram that the first pass makes on the way.  A
+// list short enough goes to one CTA, which ends the row alone.
+// The kept set is always "x > value, or x = value and index <= index": a
+// histogram over the listed range (counts or masses, 1024 equal steps, summed
+// over the cluster through distributed shared memory) gives the step in which
+// the last kept one lies, and the few elements of that step are compared with
+// each other.  Where steps do not help (all values alike, infinities, a list
+// that does not fit) a radix selection over the order-preserving 32-bit key
+// takes its place.
 #include "common.cuh"
 #include "ops.h"
 
@@ -42,11 +55,15 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBins = 2048;
+constexpr int kBins = 1024;
 constexpr int kMaxCluster = 8;
-constexpr double kOne = 8796093022208.0;  // 2^43, the weight 1
+constexpr int kSlice = 16384;   // logits per CTA: two CTAs fit on an SM
+constexpr int kList = 1016;     // of a warp's run (1024 at that slice) that are listed
+constexpr int kGather = 1024;   // of a row that one CTA takes over
+constexpr int kNear = 256;      // elements of one step, over the cluster
+constexpr int kMaxResident = 168 * 1024;      // bytes of logits a CTA keeps
+constexpr double kOne = 8796093022208.0;      // 2^43, the weight 1
 constexpr uint32_t kKeyNegInf = 0x007fffffu;  // key_of(-inf)
-constexpr int kMaxResident = 184 * 1024;      // bytes of logits a CTA keeps
 
 typedef unsigned long long u64;
 
@@ -64,24 +81,45 @@ struct SampleArgs {
   float* prob;
 };
 
-struct Shared {
-  uint32_t lo[kBins], hi[kBins];  // this CTA's histogram (hi: masses only)
-  u64 sum[kBins];                 // the cluster's
-  u64 slot[2][kMaxCluster];       // one value of every CTA
-  u64 warp[kWarps];
-  u64 pick[2];                    // a result of one thread for all
-  u64 found;                      // a result of one CTA for all
+struct alignas(16) Shared {
+  union {
+    uint32_t hist[2 * kBins];  // this CTA's histogram: masses as low and high words, or counts
+    struct {                   // or the elements of one step, a part for each CTA
+      u64 w[kNear];
+      float x[kNear];
+      int index[kNear];
+    } near;
+  };
+  union {
+    u64 sum[kBins];            // the cluster's histogram
+    uint32_t count[2 * kBins];
+    struct {                   // or the row's list, gathered in CTA 0
+      float x[kGather];
+      int index[kGather];
+    } all;
+  };
+  uint16_t list[kWarps][kList];  // elements of a warp's run, in index order
+  int listed[kWarps];
+  int near_n[kMaxCluster];
+  u64 slot[2][2][kMaxCluster];   // two values of every CTA
+  double exp2_of[64];            // 2^(j / 64)
+  u64 warp[kWarps], part[kWarps];
+  u64 pick[2];                   // a result of one thread for all
+  u64 found;                     // a result of one CTA for all
 };
 
 // Order-preserving key: x < y exactly when key_of(x) < key_of(y); -0 equals
 // +0, NaN is taken as -inf.
 __device__ __forceinline__ uint32_t key_of(float x) {
-  if (isnan(x)) return kKeyNegInf;
-  const uint32_t b = __float_as_uint(x + 0.0f);
+  const uint32_t b = __float_as_uint(fmaxf(x, -INFINITY) + 0.0f);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
+}
+// the least value whose key starts with these bits
+__device__ __forceinline__ float floor_of(uint32_t key) {
+  return key <= kKeyNegInf ? -INFINITY : value_of(key);
 }
 
 template <typename T>
@@ -90,107 +128,320 @@ __device__ __forceinline__ T warp_sum(T v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+// inclusive prefix sum over the lanes
+__device__ __forceinline__ u64 warp_prefix(u64 v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 t = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += t;
+  }
+  return v;
+}
 
 struct Row {
   const float* x;   // this CTA's slice, global
   const float* sm;  // its resident part
   int resident, count;
   int first;        // index of its first element in the row
-  uint32_t max_key;
-  double top, rcp_t;
-  __device__ __forceinline__ uint32_t key(int i) const {
-    return key_of(i < resident ? sm[i] : __ldg(x + i));
+  float top;        // the row's maximum
+  bool plain;       // magnitudes at which light() holds
+  float heavy;      // values from here up weigh 2^-20 or (barely) less
+  float least;      // values below weigh nothing
+  double c, rcp_t;  // log2(e) / T, 1 / T
+  float c_hi, c_lo, k_hi, k_lo;  // c, and top * c - 43, in two terms
+  const double* exp2_of;
+  __device__ __forceinline__ float at(int i) const { return i < resident ? sm[i] : __ldg(x + i); }
+  // exp((x - top) / T), 1 for the maximum itself, 0 for -inf and NaN
+  __device__ __forceinline__ double weight(float v) const {
+    if (v == top) return 1.0;
+    if (!(v > -INFINITY) || top == INFINITY) return 0.0;
+    return exp((static_cast<double>(v) - static_cast<double>(top)) * rcp_t);
   }
-  // exp((x - max) / T), 1 for the maximum itself
-  __device__ __forceinline__ double weight(uint32_t k) const {
-    if (k == max_key) return 1.0;
-    if (k == kKeyNegInf) return 0.0;
-    return exp((static_cast<double>(value_of(k)) - top) * rcp_t);
+  // weight * 2^43 of a value below `heavy`: under 2^23.  log2 of it is v * c -
+  // (top * c - 43), one fma that rounds once, plus what the second terms add
+  // (2^-10 at most), taken to first order.
+  __device__ __forceinline__ uint32_t light(float v) const {
+    v = fmaxf(v, least);  // (-inf and NaN too)
+    const float e = __fmaf_rn(v, c_lo, -k_lo);
+    float w;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(__fmaf_rn(v, c_hi, -k_hi)));
+    w *= __fmaf_rn(e, 0.69314718f, 1.0f);
+    return __float_as_uint(w + 8388608.0f) & 0x7fffffu;  // the integer next to it
   }
-  __device__ __forceinline__ u64 fixed(uint32_t k) const {
-    return __double2ull_rn(weight(k) * kOne);
+  // weight * 2^43
+  __device__ __forceinline__ u64 fixed(float v) const {
+    if (!plain) return __double2ull_rn(weight(v) * kOne);
+    if (!(v >= heavy)) return light(v);
+    // 2^t = 2^(n / 64) * 2^r, |r| <= 1/128: a table, and the series of e^(r ln 2)
+    // to the fifth power (2^-53 of it is left out)
+    const double t = (static_cast<double>(v) - static_cast<double>(top)) * c;
+    const double kShift = 105553116266496.0;  // 1.5 * 2^46: a sum's last bit is 1/64
+    const double m = t + kShift;
+    const int n = __double2loint(m);
+    const double r = t - (m - kShift);
+    double q = __fma_rn(r, 0x1.5d87fe78a6730p-10, 0x1.3b2ab6fba4e77p-7);
+    q = __fma_rn(q, r, 0x1.c6b08d704a0bfp-5);
+    q = __fma_rn(q, r, 0x1.ebfbdff82c58ep-3);
+    q = __fma_rn(q, r, 0x1.62e42fefa39efp-1);
+    const double s = exp2_of[n & 63];
+    const double w = __fma_rn(q * r, s, s);  // in [2^-1, 2), times 2^(n >> 6)
+    const double up = __hiloint2double(__double2hiint(w) + (((n >> 6) + 43) << 20),
+                                       __double2loint(w));
+    // the integer next to it, from the low bits of a sum with 2^52
+    return static_cast<u64>(__double_as_longlong(up + 4503599627370496.0)) & 0xfffffffffffffull;
+  }
+  // a value that weighs a little less than 2^log2w
+  __device__ __forceinline__ float below_top(double log2w) const {
+    const double d = log2w / c;
+    return static_cast<float>(top + d - 1e-6 * (fabs(d) + fabsf(top)));
   }
 };
 
-// the elements that stay: key > cut, or key = cut and index <= cut_index
+// the elements that stay: x > value, or x = value and index <= index
 struct Cut {
-  uint32_t key;
+  float value;
   int index;
-  __device__ __forceinline__ bool keeps(uint32_t k, int i) const {
-    return k > key || (k == key && i <= index);
+  __device__ __forceinline__ bool keeps(float v, int i) const {
+    return v > value || (v == value && i <= index);
   }
 };
+
+// How a pass goes over the row: every element of the slice; the elements
+// listed; or, in the one CTA that took the row over, the gathered list.
+enum Mode : int { kAll, kListed, kGathered };
 
 struct Ctx {
   cg::cluster_group cluster;
   Shared* s;
   int rank, ranks, tid, warp, lane, flip;
-  // Warp w's part of the slice: a contiguous run, so that the warps' sums are
-  // prefix sums in index order.
-  __device__ __forceinline__ void run_of(const Row& r, int& i0, int& i1) const {
-    const int per = (r.count + kWarps - 1) / kWarps;
-    i0 = min(r.count, warp * per);
-    i1 = min(r.count, i0 + per);
+  Mode mode;
+  int gathered;
+  __device__ __forceinline__ void sync() const {
+    if (ranks == 1) __syncthreads();
+    else cluster.sync();
   }
-  // Every CTA's value to every CTA: v of CTA c in slot(c) after it.
-  __device__ __forceinline__ const u64* exchange(u64 v) {
+  __device__ __forceinline__ Shared* of(int k) const {
+    return ranks == 1 ? s : cluster.map_shared_rank(s, k);
+  }
+  // Warp w's part of the slice (or gathered list): a contiguous run, so that
+  // the warps' sums are prefix sums in index order.
+  __device__ __forceinline__ int run_length(int count) const {
+    return ((count + kWarps - 1) / kWarps + 3) & ~3;
+  }
+  __device__ __forceinline__ void run_of(int count, int& i0, int& i1) const {
+    const int per = run_length(count);
+    i0 = min(count, warp * per);
+    i1 = min(count, i0 + per);
+  }
+  // four neighbours of the slice, -inf from i1 on
+  __device__ __forceinline__ float4 four(const Row& r, int i, int i1) const {
+    if (i + 3 < min(i1, r.resident)) return *reinterpret_cast<const float4*>(r.sm + i);
+    return make_float4(i < i1 ? r.at(i) : -INFINITY, i + 1 < i1 ? r.at(i + 1) : -INFINITY,
+                       i + 2 < i1 ? r.at(i + 2) : -INFINITY, i + 3 < i1 ? r.at(i + 3) : -INFINITY);
+  }
+  // f(x, index) for the elements of the warp's run
+  template <typename F>
+  __device__ __forceinline__ void each(const Row& r, F f) const {
+    int i0, i1;
+    if (mode == kAll) {
+      run_of(r.count, i0, i1);
+      for (int i = i0 + lane; i < i1; i += 32) f(r.at(i), r.first + i);
+    } else if (mode == kListed) {
+      for (int j = lane; j < s->listed[warp]; j += 32) {
+        const int i = s->list[warp][j];
+        f(r.at(i), r.first + i);
+      }
+    } else {
+      run_of(gathered, i0, i1);
+      for (int j = i0 + lane; j < i1; j += 32) f(s->all.x[j], s->all.index[j]);
+    }
+  }
+  // Two values of every CTA to every CTA: of CTA k in [0][k] and [1][k] after it.
+  __device__ __forceinline__ u64 (*exchange(u64 v, u64 w = 0))[kMaxCluster] {
     flip ^= 1;
-    if (tid < ranks) cluster.map_shared_rank(s, tid)->slot[flip][rank] = v;
-    cluster.sync();
+    if (tid < ranks) {
+      Shared* o = of(tid);
+      o->slot[flip][0][rank] = v;
+      o->slot[flip][1][rank] = w;
+    }
+    sync();
     return s->slot[flip];
   }
 };
 
-// Sum of f(key, index) over the row's elements; s->warp holds this CTA's per
-// warp, slot its cluster's per CTA.
-template <typename F>
-__device__ __forceinline__ u64 row_sum(Ctx& c, const Row& r, F f, const u64** slot) {
-  int i0, i1;
-  c.run_of(r, i0, i1);
-  u64 v = 0;
-  for (int i = i0 + c.lane; i < i1; i += 32) v += f(r.key(i), r.first + i);
+// this CTA's sum of the warps' values, in s->warp after it
+__device__ __forceinline__ u64 block_sum(const Ctx& c, u64 v) {
   v = warp_sum(v);
   if (c.lane == 0) c.s->warp[c.warp] = v;
   __syncthreads();
   u64 mine = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) mine += c.s->warp[w];
-  *slot = c.exchange(mine);
+  return mine;
+}
+
+// Sum of f(x, index) over the row's elements; s->warp holds this CTA's per
+// warp, slot its cluster's per CTA.
+template <typename F>
+__device__ __forceinline__ u64 row_sum(Ctx& c, const Row& r, F f, const u64** slot) {
+  u64 v = 0;
+  c.each(r, [&](float x, int i) { v += f(x, i); });
+  *slot = c.exchange(block_sum(c, v))[0];
   u64 all = 0;
   for (int k = 0; k < c.ranks; ++k) all += (*slot)[k];
   return all;
 }
 
+// Lists the elements from `least` up (above -inf, and in `weigh` not above
+// r.heavy), and counts them; with `weigh` also sums all weights, per warp and
+// CTA as row_sum does.  Whether every warp's list fits.
+template <bool kWeigh>
+__device__ __noinline__ bool build(Ctx& ctx, const Row& row, float least, u64* mass,
+                                   const u64** slot, int* count) {
+  const Ctx c = ctx;
+  const Row r = row;
+  Shared* s = c.s;
+  uint16_t* list = s->list[c.warp];
+  int i0, i1, n = 0;
+  uint32_t light = 0;  // 256 elements per lane at most, each under 2^23
+  c.run_of(r.count, i0, i1);
+  const unsigned below = (1u << c.lane) - 1;
+  for (int i = i0; i < i1; i += 128) {
+    const int j = i + 4 * c.lane;
+    const float4 v4 = c.four(r, j, i1);
+    const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+    unsigned ballot[4];
+    bool in[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      in[e] = v[e] >= least;
+      ballot[e] = __ballot_sync(0xffffffffu, in[e]);
+      if (kWeigh) {
+        const uint32_t w = r.light(v[e]);
+        light += in[e] ? 0u : w;
+      }
+    }
+    if ((ballot[0] | ballot[1] | ballot[2] | ballot[3]) == 0) continue;
+    int at = n;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) at += __popc(ballot[e] & below);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (in[e]) {
+        if (at < kList) list[at] = static_cast<uint16_t>(j + e);
+        ++at;
+      }
+      n += __popc(ballot[e]);
+    }
+  }
+  u64 sum = light;
+  if (c.lane == 0) s->listed[c.warp] = n;
+  __syncwarp();
+  if (kWeigh)
+    for (int j = c.lane; j < min(n, kList); j += 32) sum += r.fixed(r.at(list[j]));
+  const u64 all = block_sum(c, sum);
+  int total = 0;
+  bool fits = r.count <= 65536;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    total += s->listed[w];
+    fits = fits && s->listed[w] <= kList;
+  }
+  u64(*got)[kMaxCluster] = ctx.exchange(all, fits ? static_cast<u64>(total) : ~0ull);
+  *slot = got[0];
+  *mass = 0;
+  *count = 0;
+  for (int k = 0; k < c.ranks; ++k) {
+    *mass += got[0][k];
+    fits = fits && got[1][k] != ~0ull;
+    *count += static_cast<int>(got[1][k]);
+  }
+  return fits;
+}
+
+// After build: the row goes on with the list alone, in CTA 0 if it is short
+// (false in the others: they are done), else in every CTA.
+__device__ __noinline__ bool gather(Ctx& c, const Row& r, int count) {
+  Shared* s = c.s;
+  if (c.ranks == 1 || count > kGather) {
+    c.mode = kListed;
+    return true;
+  }
+  int at = 0;
+  for (int k = 0; k < c.rank; ++k) at += static_cast<int>(s->slot[c.flip][1][k]);
+  for (int w = 0; w < c.warp; ++w) at += s->listed[w];
+  Shared* o = c.of(0);
+  for (int j = c.lane; j < s->listed[c.warp]; j += 32) {
+    const int i = s->list[c.warp][j];
+    o->all.x[at + j] = r.at(i);
+    o->all.index[at + j] = r.first + i;
+  }
+  c.sync();
+  c.mode = kGathered;
+  c.gathered = count;
+  c.ranks = 1;
+  return c.rank == 0;
+}
+
 // After row_sum(f): the first element, in index order, at which the running
 // sum exceeds `target` (< the total).  True in the one lane that found it.
+// The CTA that has it goes over its warp's run again with all warps.
 template <typename F>
 __device__ __forceinline__ bool locate(Ctx& c, const Row& r, F f, const u64* slot, u64 target,
-                                       int* at, uint32_t* at_key) {
+                                       int* at, float* at_x) {
   for (int k = 0; k < c.rank; ++k) {
     if (target < slot[k]) return false;  // an earlier CTA has it
     target -= slot[k];
   }
   if (target >= slot[c.rank]) return false;
-  for (int w = 0; w < c.warp; ++w) {
-    if (target < c.s->warp[w]) return false;
-    target -= c.s->warp[w];
+  int w = 0;
+  for (; w < kWarps - 1 && target >= c.s->warp[w]; ++w) target -= c.s->warp[w];
+  int i0 = 0, i1 = c.s->listed[w];
+  if (c.mode != kListed) {
+    const int count = c.mode == kAll ? r.count : c.gathered;
+    const int per = c.run_length(count);
+    i0 = min(count, w * per);
+    i1 = min(count, i0 + per);
   }
-  if (target >= c.s->warp[c.warp]) return false;
-  int i0, i1;
-  c.run_of(r, i0, i1);
-  for (int i = i0; i < i1; i += 32) {
-    const uint32_t k = i + c.lane < i1 ? r.key(i + c.lane) : 0u;
-    const u64 v = i + c.lane < i1 ? f(k, r.first + i + c.lane) : 0ull;
-    u64 run = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const u64 t = __shfl_up_sync(0xffffffffu, run, o);
-      if (c.lane >= o) run += t;
+  const int per = (i1 - i0 + kWarps - 1) / kWarps;
+  auto element = [&](int j, float* x, int* index) {
+    if (c.mode == kGathered) {
+      *x = c.s->all.x[j];
+      *index = c.s->all.index[j];
+    } else {
+      const int i = c.mode == kListed ? c.s->list[w][j] : j;
+      *x = r.at(i);
+      *index = r.first + i;
     }
+  };
+  i1 = min(i1, i0 + (c.warp + 1) * per);
+  i0 = min(i1, i0 + c.warp * per);
+  float x = 0.0f;
+  int index = 0;
+  u64 v = 0;
+  for (int j = i0 + c.lane; j < i1; j += 32) {
+    element(j, &x, &index);
+    v += f(x, index);
+  }
+  v = warp_sum(v);
+  if (c.lane == 0) c.s->part[c.warp] = v;
+  __syncthreads();
+  for (int k = 0; k < c.warp; ++k) {
+    if (target < c.s->part[k]) return false;
+    target -= c.s->part[k];
+  }
+  if (target >= c.s->part[c.warp]) return false;
+  for (int i = i0; i < i1; i += 32) {
+    u64 run = 0;
+    if (i + c.lane < i1) {
+      element(i + c.lane, &x, &index);
+      run = f(x, index);
+    }
+    run = warp_prefix(run, c.lane);
     const unsigned past = __ballot_sync(0xffffffffu, run > target);
     if (past != 0) {
-      *at = r.first + i + c.lane;
-      *at_key = k;
+      *at = index;
+      *at_x = x;
       return c.lane == __ffs(static_cast<int>(past)) - 1;
     }
     target -= __shfl_sync(0xffffffffu, run, 31);
@@ -198,67 +449,27 @@ __device__ __forceinline__ bool locate(Ctx& c, const Row& r, F f, const u64* slo
   return false;
 }
 
-// One level of a selection: of the elements that `cut` keeps and whose key
-// agrees with `prefix` above bit shift + bits, the histogram of the next `bits`
-// bits; finds, from the largest bin down, the bin at which the running sum
-// reaches `target` (1 <= target <= the total).  Returns the bin, and in
-// *before the sum of the bins above it.
-template <bool kMass>
-__device__ __forceinline__ uint32_t select_level(Ctx& c, const Row& r, const Cut& cut,
-                                                 uint32_t prefix, int shift, int bits, u64 target,
-                                                 u64* before) {
+// Thread t's share of a histogram is its bins [bins - (t + 1) * m, bins - t *
+// m); of(b) is the sum in bin b.  Finds, from the largest bin down, the bin at
+// which the running sum reaches `target` (>= 1), and the sum of the bins above
+// it; false if it never does.
+template <typename Of>
+__device__ __forceinline__ bool scan_bins(const Ctx& c, int bins, u64 target, Of of, int* bin,
+                                          u64* before) {
   Shared* s = c.s;
-  const int bins = 1 << bits;
-  for (int i = c.tid; i < bins; i += kThreads) {
-    s->lo[i] = 0;
-    if (kMass) s->hi[i] = 0;
-  }
-  __syncthreads();
-  const int above = shift + bits;
-  for (int i = c.tid; i < r.count; i += kThreads) {
-    const uint32_t k = r.key(i);
-    if (above < 32 && (k >> above) != (prefix >> above)) continue;
-    if (!cut.keeps(k, r.first + i)) continue;
-    const uint32_t bin = (k >> shift) & (bins - 1);
-    if (kMass) {  // a 64-bit add of two 32-bit ones: the carry goes on, the order is free
-      const u64 v = r.fixed(k);
-      const uint32_t vl = static_cast<uint32_t>(v), vh = static_cast<uint32_t>(v >> 32);
-      uint32_t carry = 0;
-      if (vl != 0) carry = atomicAdd(&s->lo[bin], vl) > ~vl;
-      if (vh + carry != 0) atomicAdd(&s->hi[bin], vh + carry);
-    } else {
-      atomicAdd(&s->lo[bin], 1u);
-    }
-  }
-  c.cluster.sync();  // every CTA's histogram is done
-  const int per = bins / c.ranks;
-  for (int i = c.rank * per + c.tid; i < (c.rank + 1) * per; i += kThreads) {
-    u64 v = 0;
-    for (int k = 0; k < c.ranks; ++k) {
-      const Shared* o = c.cluster.map_shared_rank(s, k);
-      v += o->lo[i] + (kMass ? static_cast<u64>(o->hi[i]) << 32 : 0ull);
-    }
-    for (int k = 0; k < c.ranks; ++k) c.cluster.map_shared_rank(s, k)->sum[i] = v;
-  }
-  c.cluster.sync();  // every CTA has the cluster's
-  // thread t's bins, from the largest down: [bins - (t + 1) * m, bins - t * m)
-  const int m = bins / kThreads;  // 2 or 4
+  const int m = bins / kThreads;
   u64 own = 0;
-  for (int j = 0; j < m; ++j) own += s->sum[bins - 1 - (c.tid * m + j)];
-  u64 run = own;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const u64 t = __shfl_up_sync(0xffffffffu, run, o);
-    if (c.lane >= o) run += t;
-  }
+  for (int j = 0; j < m; ++j) own += of(bins - 1 - (c.tid * m + j));
+  u64 run = warp_prefix(own, c.lane);
   if (c.lane == 31) s->warp[c.warp] = run;
+  if (c.tid == 0) s->pick[0] = ~0ull;
   __syncthreads();
   run -= own;
   for (int w = 0; w < c.warp; ++w) run += s->warp[w];
   if (run < target && target <= run + own) {
     for (int j = 0; j < m; ++j) {
       const int b = bins - 1 - (c.tid * m + j);
-      const u64 v = s->sum[b];
+      const u64 v = of(b);
       if (target <= run + v) {
         s->pick[0] = static_cast<u64>(b);
         s->pick[1] = run;
@@ -269,49 +480,169 @@ __device__ __forceinline__ uint32_t select_level(Ctx& c, const Row& r, const Cut
   }
   __syncthreads();
   *before = s->pick[1];
-  return static_cast<uint32_t>(s->pick[0]);
+  *bin = static_cast<int>(s->pick[0]);
+  return s->pick[0] != ~0ull;
 }
 
-// The shortest prefix of the kept order whose sum (count or mass) reaches
-// `target` (1 <= target <= the kept total), as a tighter cut.
+// One histogram of the cluster: bin_of(x, index) is an element's bin, or -1.
+// As scan_bins; every CTA gets the same answer.
+template <bool kMass, typename BinOf>
+__device__ __forceinline__ bool histogram(const Ctx& c, const Row& r, BinOf bin_of, u64 target,
+                                          int* bin, u64* before) {
+  Shared* s = c.s;
+  for (int i = c.tid; i < (kMass ? 2 : 1) * kBins; i += kThreads) s->hist[i] = 0;
+  __syncthreads();
+  c.each(r, [&](float x, int i) {
+    const int b = bin_of(x, i);
+    if (b < 0) return;
+    if (kMass) {  // a 64-bit add of two 32-bit ones: the carry goes on, the order is free
+      const u64 v = r.fixed(x);
+      const uint32_t vl = static_cast<uint32_t>(v), vh = static_cast<uint32_t>(v >> 32);
+      uint32_t carry = 0;
+      if (vl != 0) carry = atomicAdd(&s->hist[b], vl) > ~vl;
+      if (vh + carry != 0) atomicAdd(&s->hist[kBins + b], vh + carry);
+    } else {
+      atomicAdd(&s->hist[b], 1u);
+    }
+  });
+  c.sync();  // every CTA's histogram is done
+  auto local = [&](const Shared* o, int b) -> u64 {
+    return o->hist[b] + (kMass ? static_cast<u64>(o->hist[kBins + b]) << 32 : 0ull);
+  };
+  if (c.ranks == 1)
+    return scan_bins(c, kBins, target, [&](int b) { return local(s, b); }, bin, before);
+  const int per = kBins / c.ranks;
+  for (int i = c.rank * per + c.tid; i < (c.rank + 1) * per; i += kThreads) {
+    u64 v = 0;
+    for (int k = 0; k < c.ranks; ++k) v += local(c.of(k), i);
+    for (int k = 0; k < c.ranks; ++k) c.of(k)->sum[i] = v;
+  }
+  c.sync();  // every CTA has the cluster's
+  return scan_bins(c, kBins, target, [&](int b) { return s->sum[b]; }, bin, before);
+}
+
+// Of the elements that `cut` keeps from `least` up (finite), the shortest
+// prefix of the order whose sum (count or mass) reaches `target` (>= 1), as a
+// tighter cut.  False, with the cut as it was, where equal steps do not part
+// them.
 template <bool kMass>
-__device__ __forceinline__ Cut select(Ctx& c, const Row& r, Cut cut, u64 target) {
-  u64 before = 0;
-  uint32_t key = select_level<kMass>(c, r, cut, 0, 21, 11, target, &before) << 21;
+__device__ __noinline__ bool select_steps(const Ctx& ctx, const Row& row, Cut* cut_io, float least,
+                                          u64 target) {
+  const Ctx c = ctx;
+  const Row r = row;
+  const Cut cut = *cut_io;
+  Shared* s = c.s;
+  const float scale = (kBins - 0.25f) / (r.top - least);
+  if (!(scale > 0.0f && scale < 1e30f)) return false;
+  auto bin_of = [&](float x, int i) {  // rounding is monotone: so are the steps
+    if (!(x >= least) || !cut.keeps(x, i)) return -1;
+    return min(kBins - 1, static_cast<int>((x - least) * scale));
+  };
+  if (c.tid == 0) s->near_n[c.rank] = 0;
+  int bin;
+  u64 before;
+  if (!histogram<kMass>(c, r, bin_of, target, &bin, &before)) return false;
   target -= before;
-  key |= select_level<kMass>(c, r, cut, key, 10, 11, target, &before) << 10;
-  target -= before;
-  key |= select_level<kMass>(c, r, cut, key, 0, 10, target, &before);
-  target -= before;
-  // of the elements equal to key, the first `ties` stay
+  // the elements of that step to every CTA, each into its own part
+  const int room = kNear / c.ranks;
+  c.each(r, [&](float x, int i) {
+    if (bin_of(x, i) != bin) return;
+    const int at = atomicAdd(&s->near_n[c.rank], 1);
+    if (at >= room) return;
+    for (int k = 0; k < c.ranks; ++k) {
+      Shared* o = c.of(k);
+      o->near.x[c.rank * room + at] = x;
+      o->near.index[c.rank * room + at] = i;
+    }
+  });
+  __syncthreads();
+  if (c.tid < c.ranks && c.tid != c.rank) c.of(c.tid)->near_n[c.rank] = s->near_n[c.rank];
+  c.sync();
+  bool fits = true;
+  for (int k = 0; k < c.ranks; ++k) fits = fits && s->near_n[k] <= room;
+  if (!fits) return false;
+  const bool mine = c.tid < kNear && c.tid % room < s->near_n[min(c.tid / room, c.ranks - 1)];
+  float x = 0.0f;
+  int index = 0;
+  u64 w = 0;
+  if (mine) {
+    x = s->near.x[c.tid];
+    index = s->near.index[c.tid];
+    w = kMass ? r.fixed(x) : 1ull;
+    s->near.w[c.tid] = w;
+  }
+  __syncthreads();
+  if (mine) {
+    u64 run = 0;  // what comes before it in the order
+    for (int k = 0; k < c.ranks; ++k)
+      for (int j = k * room; j < k * room + s->near_n[k]; ++j)
+        if (s->near.x[j] > x || (s->near.x[j] == x && s->near.index[j] < index)) run += s->near.w[j];
+    if (run < target && target <= run + w)
+      s->found = (static_cast<u64>(__float_as_uint(x)) << 32) | static_cast<uint32_t>(index);
+  }
+  __syncthreads();
+  *cut_io = Cut{__uint_as_float(static_cast<uint32_t>(s->found >> 32)),
+                static_cast<int>(static_cast<uint32_t>(s->found))};
+  return true;
+}
+
+// select_steps by radix, for any values: ten bits of the key at a time (the
+// last ten overlap), then the first so many of the elements equal to it.
+template <bool kMass>
+__device__ __noinline__ void select_radix(Ctx& c, const Row& r, Cut* cut_io, float least,
+                                          u64 target) {
+  const Cut cut = *cut_io;
+  uint32_t key = 0;
+#pragma unroll 1
+  for (int above = 32; above > 0; above = above > 10 ? above - 10 : 0) {
+    const int shift = above > 10 ? above - 10 : 0;
+    auto bin_of = [&](float x, int i) {
+      x = fmaxf(x, -INFINITY);  // NaN
+      if (!(x >= least) || !cut.keeps(x, i)) return -1;
+      const uint32_t k = key_of(x);
+      if (above < 32 && (k >> above) != (key >> above)) return -1;
+      return static_cast<int>((k >> shift) & (kBins - 1));
+    };
+    int bin;
+    u64 before;
+    histogram<kMass>(c, r, bin_of, target, &bin, &before);
+    target -= before;
+    key = (key & ~((kBins - 1u) << shift)) | (static_cast<uint32_t>(bin & (kBins - 1)) << shift);
+  }
+  const float value = value_of(key);
   u64 ties = target;
   if (kMass) {
-    const u64 w = r.fixed(key);
+    const u64 w = r.fixed(value);
     ties = w > 0 ? (target + w - 1) / w : 1;
   }
   const u64* slot;
-  auto tie = [&](uint32_t k, int i) -> u64 { return k == key && cut.keeps(k, i) ? 1ull : 0ull; };
+  auto tie = [&](float x, int i) -> u64 {
+    x = fmaxf(x, -INFINITY);
+    return x == value && cut.keeps(x, i) ? 1ull : 0ull;
+  };
   row_sum(c, r, tie, &slot);
   int at;
-  uint32_t at_key;
-  if (locate(c, r, tie, slot, ties - 1, &at, &at_key))
-    for (int k = 0; k < c.ranks; ++k)
-      c.cluster.map_shared_rank(c.s, k)->found = static_cast<u64>(at);
-  c.cluster.sync();
-  return Cut{key, static_cast<int>(c.s->found)};
+  float at_x;
+  if (locate(c, r, tie, slot, ties - 1, &at, &at_x))
+    for (int k = 0; k < c.ranks; ++k) c.of(k)->found = static_cast<u64>(at);
+  c.sync();
+  *cut_io = Cut{value, static_cast<int>(c.s->found)};
 }
 
-__global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
   extern __shared__ __align__(16) uint8_t raw[];
   Ctx c{cg::this_cluster()};
-  c.s = reinterpret_cast<Shared*>(raw);
+  Shared* s = reinterpret_cast<Shared*>(raw);
   float* sm = reinterpret_cast<float*>(raw + sizeof(Shared));
+  c.s = s;
   c.rank = static_cast<int>(c.cluster.block_rank());
   c.ranks = static_cast<int>(c.cluster.num_blocks());
   c.tid = threadIdx.x;
   c.warp = c.tid >> 5;
   c.lane = c.tid & 31;
   c.flip = 0;
+  c.mode = kAll;
+  c.gathered = 0;
   const long long row = blockIdx.x / c.ranks;
   Row r;
   r.first = min(a.n, c.rank * a.slice);
@@ -319,80 +650,168 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
   r.x = a.logits + row * a.n + r.first;
   r.sm = sm;
   r.resident = min(r.count, a.resident);
-  r.max_key = 0;
-
-  // ---- the row's maximum and the first index that has it
-  u64 best = 0;  // key << 32 | ~index: the largest is the first largest logit
-  for (int i = c.tid; i < r.count; i += kThreads) {
-    const float x = __ldg(r.x + i);
-    if (i < r.resident) sm[i] = x;
-    const u64 v = (static_cast<u64>(key_of(x)) << 32) | ~static_cast<uint32_t>(r.first + i);
-    best = v > best ? v : best;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const u64 v = __shfl_xor_sync(0xffffffffu, best, o);
-    best = v > best ? v : best;
-  }
-  if (c.lane == 0) c.s->warp[c.warp] = best;
-  c.cluster.sync();  // (also: every CTA of the cluster has started)
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) best = c.s->warp[w] > best ? c.s->warp[w] : best;
-  const u64* slot = c.exchange(best);
-  for (int k = 0; k < c.ranks; ++k) best = slot[k] > best ? slot[k] : best;
-  r.max_key = static_cast<uint32_t>(best >> 32);
-  const uint32_t first_max = ~static_cast<uint32_t>(best);
-
   const float t = a.temperature != nullptr ? a.temperature[row] : 1.0f;
-  const bool none = r.max_key == kKeyNegInf;
-  // every CTA of the cluster takes the same branch (row-wide values only)
-  if (none || !(t > 0.0f)) {
-    if (c.rank == 0 && c.tid == 0) {
-      a.index[row] = none ? 0xffffffffu : first_max;
-      if (a.prob != nullptr) a.prob[row] = none ? 0.0f : 1.0f;
-    }
-    c.cluster.sync();  // no CTA leaves while another may write its slots
-    return;
-  }
-  r.top = static_cast<double>(value_of(r.max_key));
-  r.rcp_t = 1.0 / static_cast<double>(t);
-
-  // ---- the kept set
-  Cut cut{0u, 0x7fffffff};
-  const int k = a.top_k != nullptr ? a.top_k[row] : 0;
   const float p = a.top_p != nullptr ? a.top_p[row] : 1.0f;
   const float mp = a.min_p != nullptr ? a.min_p[row] : 0.0f;
-  if (k > 0 && k < a.n) cut = select<false>(c, r, cut, static_cast<u64>(k));
-  if (p < 1.0f) {
-    auto kept = [&](uint32_t key, int i) { return cut.keeps(key, i) ? r.fixed(key) : 0ull; };
-    const u64 all = row_sum(c, r, kept, &slot);
-    const double want = ceil(static_cast<double>(p) * static_cast<double>(all));
-    u64 target = want > 1.0 ? static_cast<u64>(want) : 1ull;
-    target = target < all ? target : all;
-    cut = select<true>(c, r, cut, target);
+  int k = a.top_k != nullptr ? a.top_k[row] : 0;
+  if (k >= a.n || !(t > 0.0f)) k = 0;
+
+  // (every CTA of the cluster takes the same branches: row-wide values only)
+  if (k > 0) {
+    for (int i = c.tid; i < 2 * kBins; i += kThreads) s->hist[i] = 0;
+    __syncthreads();
   }
+  // the others have started when the wait below ends: nothing is written to them before
+  if (c.ranks > 1) cg::this_cluster().barrier_arrive();
+
+  // ---- the slice into shared memory, the row's maximum, and for top-k the
+  // histogram of the maxima of eight logits
+  float top = -INFINITY;  // (fmaxf passes NaN over)
+  for (int i = c.tid; i < r.count; i += 8 * kThreads) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      v[j] = i + j * kThreads < r.count ? __ldg(r.x + i + j * kThreads) : -INFINITY;
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (i + j * kThreads < r.resident) sm[i + j * kThreads] = v[j];
+      m = fmaxf(m, v[j]);
+    }
+    if (k > 0) atomicAdd(&s->hist[key_of(m) >> 21], 1u);
+    top = fmaxf(top, m);
+  }
+  if (c.tid < 64 && t > 0.0f) s->exp2_of[c.tid] = exp2(c.tid / 64.0);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (c.lane == 0) s->warp[c.warp] = key_of(top);
+  __syncthreads();
+  u64 best = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) best = s->warp[w] > best ? s->warp[w] : best;
+  if (c.ranks > 1) cg::this_cluster().barrier_wait();
+  const u64* slot = c.exchange(best)[0];
+  for (int j = 0; j < c.ranks; ++j) best = slot[j] > best ? slot[j] : best;
+  top = value_of(static_cast<uint32_t>(best));
+  r.top = top;
+
+  if (top == -INFINITY) {
+    if (c.rank == 0 && c.tid == 0) {
+      a.index[row] = 0xffffffffu;
+      if (a.prob != nullptr) a.prob[row] = 0.0f;
+    }
+    return;  // (nobody reads or writes another CTA after the exchange)
+  }
+  int at;
+  float at_x;
+  if (!(t > 0.0f)) {  // greedy: the first that equals the maximum
+    auto first = [&](float x, int) -> u64 { return x == top ? 1ull : 0ull; };
+    row_sum(c, r, first, &slot);
+    if (locate(c, r, first, slot, 0, &at, &at_x)) {
+      a.index[row] = static_cast<uint32_t>(at);
+      if (a.prob != nullptr) a.prob[row] = 1.0f;
+    }
+    return;
+  }
+  r.rcp_t = 1.0 / static_cast<double>(t);
+  r.c = 1.4426950408889634 * r.rcp_t;
+  r.c_hi = static_cast<float>(r.c);
+  r.c_lo = static_cast<float>(r.c - static_cast<double>(r.c_hi));
+  const double shift = static_cast<double>(top) * r.c - 43.0;
+  r.k_hi = static_cast<float>(shift);
+  r.k_lo = static_cast<float>(shift - static_cast<double>(r.k_hi));
+  r.plain = fabs(shift) < 8192.0 && fabsf(top) < 1e30f && t < 1e30f && t > 1e-30f;
+  r.heavy = r.below_top(-20.0);
+  r.least = r.below_top(-60.0);
+  r.exp2_of = s->exp2_of;
+
+  // ---- the kept set
+  Cut cut{-INFINITY, 0x7fffffff};
+  u64 mass = 0;
+  int count = 0;
+  if (k > 0) {
+    // the histogram of the groups' maxima, summed over the cluster
+    u64 before;
+    int bin;
+    bool ok;
+    if (c.ranks == 1) {
+      ok = scan_bins(c, 2 * kBins, k, [&](int b) -> u64 { return s->hist[b]; }, &bin, &before);
+    } else {
+      const int per = 2 * kBins / c.ranks;
+      for (int i = c.rank * per + c.tid; i < (c.rank + 1) * per; i += kThreads) {
+        uint32_t v = 0;
+        for (int j = 0; j < c.ranks; ++j) v += c.of(j)->hist[i];
+        for (int j = 0; j < c.ranks; ++j) c.of(j)->count[i] = v;
+      }
+      c.sync();
+      ok = scan_bins(c, 2 * kBins, k, [&](int b) -> u64 { return s->count[b]; }, &bin, &before);
+    }
+    // k groups have their maximum, so k logits lie, from here up
+    const float least = ok ? floor_of(static_cast<uint32_t>(bin) << 21) : -INFINITY;
+    ok = least > -INFINITY && build<false>(c, r, least, &mass, &slot, &count);
+    if (ok && !gather(c, r, count)) return;
+    if (!ok || !select_steps<false>(c, r, &cut, least, static_cast<u64>(k)))
+      select_radix<false>(c, r, &cut, least, static_cast<u64>(k));
+  }
+  if (p < 1.0f) {
+    bool listed = false;
+    auto kept = [&](float x, int i) { return cut.keeps(x, i) ? r.fixed(x) : 0ull; };
+    if (k == 0 && r.plain) {
+      // the total is 1 at least; half of the bound, for the roundings on the way
+      const double l2 = log2(0.5 * (1.0 - static_cast<double>(fmaxf(p, 0.0f))) / a.n);
+      listed = build<true>(c, r, r.below_top(fmin(l2, -20.0)), &mass, &slot, &count);
+      if (listed && !gather(c, r, count)) return;
+    }
+    if (!listed) mass = row_sum(c, r, kept, &slot);
+    const double want = ceil(static_cast<double>(p) * static_cast<double>(mass));
+    const u64 target = want > 1.0 ? static_cast<u64>(want) : 1ull;
+    if (target < mass) {
+      float least = cut.value;
+      if (r.plain)
+        least = fmaxf(least,
+                      r.below_top(log2(0.5 * static_cast<double>(mass - target) / (a.n * kOne))));
+      if (c.mode == kAll || !(least > -INFINITY) || !select_steps<true>(c, r, &cut, least, target))
+        select_radix<true>(c, r, &cut, least, target);
+    }
+  }
+  // min-p in float but next to the border, in double there
   const double least = mp > 0.0f ? fmin(static_cast<double>(mp), 1.0) : 0.0;
-  auto kept = [&](uint32_t key, int i) -> u64 {
-    if (!cut.keeps(key, i)) return 0ull;
-    const double w = r.weight(key);
-    return w >= least ? __double2ull_rn(w * kOne) : 0ull;
+  float sure = INFINITY, out = -INFINITY;  // x from `sure` up stays, below `out` not
+  if (least > 0.0 && r.plain) {
+    const double x = static_cast<double>(top) + log(least) * static_cast<double>(t);
+    const double slack = 1e-6 * (fabs(x) + fabs(static_cast<double>(top)) + 1e-6);
+    sure = static_cast<float>(x + slack);
+    out = static_cast<float>(x - slack);
+  }
+  auto kept = [&](float x, int i) -> u64 {
+    if (!cut.keeps(x, i)) return 0ull;
+    if (least > 0.0 && !(x >= sure)) {
+      if (x < out || !(r.weight(x) >= least)) return 0ull;
+    }
+    return r.fixed(x);
   };
 
   // ---- the draw
-  const u64 all = row_sum(c, r, kept, &slot);
+  u64 all = 0;
+  bool summed = false;
+  if (c.mode == kAll && r.plain && k == 0 && !(p < 1.0f)) {
+    if (least > 0.0) {  // what min-p may keep is listed
+      if (build<false>(c, r, out, &mass, &slot, &count) && !gather(c, r, count)) return;
+    } else {  // every element counts: s->warp and slot hold their sums
+      summed = build<true>(c, r, r.heavy, &all, &slot, &count);
+    }
+  }
+  if (!summed) all = row_sum(c, r, kept, &slot);
   const float u = a.u[row];
   u64 target = u > 0.0f ? static_cast<u64>(fmin(static_cast<double>(u), 1.0) *
                                            static_cast<double>(all))
                         : 0ull;
   target = target < all ? target : all - 1;
-  int at;
-  uint32_t at_key;
-  if (locate(c, r, kept, slot, target, &at, &at_key)) {
+  if (locate(c, r, kept, slot, target, &at, &at_x)) {
     a.index[row] = static_cast<uint32_t>(at);
     if (a.prob != nullptr)
-      a.prob[row] = static_cast<float>(r.weight(at_key) * kOne / static_cast<double>(all));
+      a.prob[row] = static_cast<float>(r.weight(at_x) * kOne / static_cast<double>(all));
   }
-  c.cluster.sync();
 }
 
 }  // namespace
@@ -400,14 +819,14 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
 int sample_f32(long long rows, int n, const float* logits, const float* temperature,
                const int* top_k, const float* top_p, const float* min_p, const float* u,
                uint32_t* index, float* prob, cudaStream_t stream) {
-  // Enough CTAs per row that its slices fit on chip, and more while the GPU
-  // has SMs to spare and a slice stays above 4096 logits.
+  // Slices of 16384 logits (two CTAs to an SM), and smaller ones while the GPU
+  // has SMs to spare.
   int c = 1;
   const long long fit = kMaxResident / 4;
-  while (c < kMaxCluster && (n > c * fit || (rows * c * 2 <= num_sms() && n > c * 8192))) c *= 2;
+  while (c < kMaxCluster && (n > c * kSlice || (rows * c * 2 <= num_sms() && n > c * 4096))) c *= 2;
   SampleArgs a{};
   a.n = n;
-  a.slice = (n + c - 1) / c;
+  a.slice = ((n + c - 1) / c + 3) & ~3;
   a.resident = static_cast<int>(std::min<long long>(a.slice, fit));
   a.logits = logits;
   a.temperature = temperature;
