@@ -20,17 +20,31 @@
 // one that several share leaves a partial (max, sum, O) in each, at most two per
 // CTA, which a second kernel joins in the order of the keys.
 //
-// Within a CTA: K and V tiles by TMA through a 3-stage ring; warp w owns keys
-// [16w, 16w + 16) of every tile with its own running maximum, S^T = K . q^T by
-// int8 mma, O^T = V^T . P^T by bf16 mma.  The output is fp32 and meant to be:
-// V's codes are exact in bf16, and P times the key's V scale goes in as two
-// bf16 terms, head and remainder (16 bits of it together, a relative error
-// of 2^-17 at most, where a single f16 P leaves 2^-12), with fp32 sums.
+// The output is fp32 and meant to be.  V's codes are exact in f16; P takes the
+// key's V scale in, P' = 2^(s - m + log2 v_scale + 11) <= 2^15 with m the
+// running maximum of s + log2 v_scale, and goes into the product as two f16
+// terms, head and remainder (22 bits together, where one f16 leaves 11), with
+// fp32 sums; the softmax sum takes P' / v_scale.  Two kernels:
+//
+// Up to 16 query rows, tree_mma_kernel: bound by the cache's bytes.  K and V
+// tiles by TMA through a 3-stage ring; warp w owns keys [16w, 16w + 16) of every
+// tile with its own running maximum, S^T = K . q^T by int8 mma.sync, O^T = V^T .
+// P^T by f16 mma.sync (the rows are the n = 8 side, so few are padding).
+//
+// More rows, tree_tc_kernel: tcgen05 with a tile of 128 query rows, bound by
+// the exponentials and conversions of the softmax warps and the tensor pipe (S in
+// int8, P'.V twice in f16).  The CTA's key tiles go alternately to two lanes,
+// each with a score tile S_x and an accumulator O_x in TMEM and a softmax
+// warpgroup, one thread per query row; P' overwrites S_x (head in its first 64
+// columns, remainder in the last) and the product reads it there.  Another
+// warpgroup turns V's codes into f16, [key][dim] as they stand: the product
+// takes B with the dims contiguous.  The two lanes are joined at the segment's
+// end.
 #include "attn_mma.cuh"
 #include "common.cuh"
 #include "ops.h"
 
-#include <cuda_bf16.h>
+#include <cuda_fp16.h>
 
 #include <algorithm>
 
@@ -44,10 +58,13 @@ constexpr int kTileKeys = 128;  // keys per unit
 constexpr int kStages = 3;
 constexpr int kMaxBatch = kMaxTreeBatch;  // a CTA holds every sequence's length
 constexpr int kPartRow = 132;     // floats per row of a partial: m, l, 2 unused, O[128]
-constexpr int kMaxTileRows = 32;  // query rows per segment
+constexpr int kMaxTileRows = 16;  // query rows per segment (tree_mma_kernel)
+constexpr int kTcRows = 128;      // the same (tree_tc_kernel)
 constexpr int kMaxCtasPerSm = 2;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLazy = 4.0f;  // log2 of the largest P before its maximum is raised
+constexpr float kLazy = 4.0f;   // the maximum is raised when a score passes it by more (log2)
+constexpr float kLift = 11.0f;  // log2 of P' at the maximum
+constexpr float kNoScale = 0x1p-100f;  // a V scale below counts as 0
 
 struct TreeArgs {
   int batch, drafts, heads_q, heads_kv, max_len;
@@ -75,7 +92,7 @@ struct TreeArgs {
 struct TL {  // shared memory layout (bytes from a 1024-aligned base)
   static constexpr int kKV = 2 * kTileKeys * 128;  // K then V, int8 [128][128] SW128
   static constexpr int kScales = kStages * kKV;    // per stage ks[128], vs[128]
-  static constexpr int kWarpM = kScales + kStages * 1024;  // m[8][32], then l[8][32]
+  static constexpr int kWarpM = kScales + kStages * 1024;  // m[8][16], then l[8][16]
   static constexpr int kAnc = kWarpM + 2 * kTWarps * kMaxTileRows * 4;  // u64[64]
   static constexpr int kPar = kAnc + kMaxDrafts * 8;                    // int[64]
   static constexpr int kPre = kPar + kMaxDrafts * 4;                    // int[batch + 1]
@@ -87,38 +104,53 @@ static_assert(TL::kBars % 8 == 0 && TL::kAnc % 8 == 0, "aligned");
 static_assert(TL::kBytes <= 232448 / 2 - 1024, "two CTAs per SM");
 static_assert(kTWarps * 8 * 128 * 4 <= TL::kKV, "eight rows merge inside a stage");
 
-// two f32 -> bf16 pair, the first in the low half
-__device__ __forceinline__ uint32_t bf2(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+// two f32 -> f16 pair, the first in the low half
+__device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-__device__ __forceinline__ float bf_lo(uint32_t v) { return __uint_as_float(v << 16); }
-__device__ __forceinline__ float bf_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
+// what the pair leaves of them, as another pair
+__device__ __forceinline__ uint32_t rest_of(float lo, float hi, uint32_t pair) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pair));
+  return half2_of(lo - f.x, hi - f.y);
+}
 
-// D (16x8 f32) += A (16x16 bf16, row) x B (16x8 bf16, col)
-__device__ __forceinline__ void mma_bf16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                               uint32_t b1) {
+// D (16x8 f32) += A (16x16 f16, row) x B (16x8 f16, col)
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                        uint32_t b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, "
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
       "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// A word of an ldmatrix .trans over int8 pairs: bytes (k, d), (k, d + 1),
-// (k + 1, d), (k + 1, d + 1).  Out: the bf16 pairs {(k, d), (k + 1, d)} and
-// {(k, d + 1), (k + 1, d + 1)}, exact: under the exponent byte 0x43 the low
-// seven bits of a code read 128 + (code & 127), its sign bit alone 128 or
-// 256, and their difference is the code.
-__device__ __forceinline__ uint32_t bf16_codes(uint32_t x) {
-  const uint32_t p = x & 0xff7fff7fu, n = x & 0xff80ff80u;
-  const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&p),
-                                   *reinterpret_cast<const __nv_bfloat162*>(&n));
+// Two int8 codes with their sign bits flipped, each under the exponent byte
+// 0x64, i.e. the f16 values code + 1152 -> the codes, exactly
+__device__ __forceinline__ uint32_t unbias(uint32_t x) {
+  const uint32_t bias = 0x64806480u;  // 1152
+  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&x),
+                            *reinterpret_cast<const __half2*>(&bias));
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+// A word of an ldmatrix .trans over int8 pairs: bytes (k, d), (k, d + 1),
+// (k + 1, d), (k + 1, d + 1).  Out: the f16 pairs {(k, d), (k + 1, d)} and
+// {(k, d + 1), (k + 1, d + 1)}.
 __device__ __forceinline__ void split_codes(uint32_t w, uint32_t& even, uint32_t& odd) {
-  even = bf16_codes(__byte_perm(w, 0x43434343u, 0x4240));
-  odd = bf16_codes(__byte_perm(w, 0x43434343u, 0x4341));
+  const uint32_t u = w ^ 0x80808080u;
+  even = unbias(__byte_perm(u, 0x64646464u, 0x4240));
+  odd = unbias(__byte_perm(u, 0x64646464u, 0x4341));
+}
+
+// log2 and reciprocal of a V scale (2^-22 off at most); of one that counts as
+// 0, of kNoScale instead (its codes are taken as zeros)
+__device__ __forceinline__ float scale_log2(float vs) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaxf(vs, kNoScale)));
+  return vs == vs ? y : vs;
+}
+__device__ __forceinline__ float scale_rcp(float vs) {
+  return __frcp_rn(fmaxf(vs, kNoScale));
 }
 
 // d of sequence b, 0 when it has none or its rows do not fit in the cache
@@ -128,11 +160,12 @@ __device__ __forceinline__ int drafts_of(const TreeArgs& a, int b, int len, bool
   return *bad || d < 0 ? 0 : d;
 }
 
-// pre[b] = 128-key tiles of the sequences before b (all threads; B <= 2048:
-// eight sequences per thread); returns after a barrier
+// pre[b] = 128-key tiles of the sequences before b (all threads of the block);
+// returns after a barrier
+template <int kThreads>
 __device__ __forceinline__ void count_tiles(const TreeArgs& a, int* pre, int* scratch) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  constexpr int kPer = kMaxBatch / kTThreads;
+  constexpr int kPer = kMaxBatch / kThreads;
   const int b0 = tid * kPer;
   int t[kPer], sum = 0;
 #pragma unroll
@@ -198,7 +231,7 @@ __device__ __forceinline__ void next_unit(const int* pre, int batch, int per_seq
 
 // NT: query rows of a segment / 8
 template <int NT>
-__global__ void __launch_bounds__(kTThreads, NT > 2 ? 1 : 2)
+__global__ void __launch_bounds__(kTThreads, 2)
     tree_mma_kernel(const __grid_constant__ CUtensorMap kmap,
                     const __grid_constant__ CUtensorMap vmap, TreeArgs a) {
   constexpr int kRows = 8 * NT;
@@ -207,8 +240,8 @@ __global__ void __launch_bounds__(kTThreads, NT > 2 ? 1 : 2)
                                            ~static_cast<uintptr_t>(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + TL::kBars);
   uint64_t* empty = full + kStages;
-  float* warp_m = reinterpret_cast<float*>(sm + TL::kWarpM);  // [8][32]
-  float* warp_l = warp_m + kTWarps * kMaxTileRows;            // [8][32]
+  float* warp_m = reinterpret_cast<float*>(sm + TL::kWarpM);  // [8][16]
+  float* warp_l = warp_m + kTWarps * kMaxTileRows;            // [8][16]
   unsigned long long* anc = reinterpret_cast<unsigned long long*>(sm + TL::kAnc);
   int* par = reinterpret_cast<int*>(sm + TL::kPar);
   int* pre = reinterpret_cast<int*>(sm + TL::kPre);
@@ -228,7 +261,7 @@ __global__ void __launch_bounds__(kTThreads, NT > 2 ? 1 : 2)
   }
   pdl_wait();
   pdl_trigger();  // the joining kernel waits for this grid's completion
-  count_tiles(a, pre, par);  // (its barriers also publish the mbarriers)
+  count_tiles<kTThreads>(a, pre, par);  // (its barriers also publish the mbarriers)
 
   const int per_seq = a.heads_kv * a.qtiles;
   const long long units = static_cast<long long>(pre[a.batch]) * per_seq;
@@ -361,13 +394,15 @@ __global__ void __launch_bounds__(kTThreads, NT > 2 ? 1 : 2)
       const float ks_lo = ksc[wk + g], ks_hi = ksc[wk + g + 8];
       const float vs_lo = n_lo < d ? ksc[kTileKeys + wk + g] : 0.0f;
       const float vs_hi = n_hi < d ? ksc[kTileKeys + wk + g + 8] : 0.0f;
+      const float lv_lo = scale_log2(vs_lo), lv_hi = scale_log2(vs_hi);
+      const float rv_lo = scale_rcp(vs_lo), rv_hi = scale_rcp(vs_hi);
       float sc[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        sc[nt][0] = small_i2f(c[nt][0]) * qsc[nt][0] * ks_lo;
-        sc[nt][1] = small_i2f(c[nt][1]) * qsc[nt][1] * ks_lo;
-        sc[nt][2] = small_i2f(c[nt][2]) * qsc[nt][0] * ks_hi;
-        sc[nt][3] = small_i2f(c[nt][3]) * qsc[nt][1] * ks_hi;
+        sc[nt][0] = fmaf(small_i2f(c[nt][0]) * qsc[nt][0], ks_lo, lv_lo);
+        sc[nt][1] = fmaf(small_i2f(c[nt][1]) * qsc[nt][1], ks_lo, lv_lo);
+        sc[nt][2] = fmaf(small_i2f(c[nt][2]) * qsc[nt][0], ks_hi, lv_hi);
+        sc[nt][3] = fmaf(small_i2f(c[nt][3]) * qsc[nt][1], ks_hi, lv_hi);
         if (edge) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
@@ -406,27 +441,29 @@ __global__ void __launch_bounds__(kTThreads, NT > 2 ? 1 : 2)
             }
           }
       }
-      // ---- P = 2^(s - m) (summed unscaled), times the key's V scale, as a
-      // bf16 head and remainder, transposed into the B operand
+      // ---- P', its sum without the V scale, and its two f16 terms, transposed
+      // into the B operand
       uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float r0 = m[nt][0] == -INFINITY ? 0.0f : m[nt][0];
-        const float r1 = m[nt][1] == -INFINITY ? 0.0f : m[nt][1];
+        const float r0 = (m[nt][0] == -INFINITY ? 0.0f : m[nt][0]) - kLift;
+        const float r1 = (m[nt][1] == -INFINITY ? 0.0f : m[nt][1]) - kLift;
         float p0 = fast_exp2(sc[nt][0] - r0), p1 = fast_exp2(sc[nt][1] - r1);
         float p2 = fast_exp2(sc[nt][2] - r0), p3 = fast_exp2(sc[nt][3] - r1);
-        l[nt][0] += p0 + p2;
-        l[nt][1] += p1 + p3;
-        // 0 * a scale that is not finite stays 0: a masked key adds nothing
-        p0 = p0 == 0.0f ? 0.0f : p0 * vs_lo;
-        p1 = p1 == 0.0f ? 0.0f : p1 * vs_lo;
-        p2 = p2 == 0.0f ? 0.0f : p2 * vs_hi;
-        p3 = p3 == 0.0f ? 0.0f : p3 * vs_hi;
-        const uint32_t h0 = bf2(p0, p1), h1 = bf2(p2, p3);
+        if (edge) {  // what is masked adds nothing, whatever its scales
+          l[nt][0] += (p0 == 0.0f ? 0.0f : p0 * rv_lo) + (p2 == 0.0f ? 0.0f : p2 * rv_hi);
+          l[nt][1] += (p1 == 0.0f ? 0.0f : p1 * rv_lo) + (p3 == 0.0f ? 0.0f : p3 * rv_hi);
+        } else {
+          l[nt][0] = fmaf(p2, rv_hi, fmaf(p0, rv_lo, l[nt][0]));
+          l[nt][1] = fmaf(p3, rv_hi, fmaf(p1, rv_lo, l[nt][1]));
+        }
+        if (vs_lo < kNoScale) p0 = p1 = 0.0f;
+        if (vs_hi < kNoScale) p2 = p3 = 0.0f;
+        const uint32_t h0 = half2_of(p0, p1), h1 = half2_of(p2, p3);
         ph[nt][0] = movmatrix_t(h0);
         ph[nt][1] = movmatrix_t(h1);
-        pl[nt][0] = movmatrix_t(bf2(p0 - bf_lo(h0), p1 - bf_hi(h0)));
-        pl[nt][1] = movmatrix_t(bf2(p2 - bf_lo(h1), p3 - bf_hi(h1)));
+        pl[nt][0] = movmatrix_t(rest_of(p0, p1, h0));
+        pl[nt][1] = movmatrix_t(rest_of(p2, p3, h1));
       }
       // ---- O^T += V^T . P^T; ldmatrix .trans matrices (keys wk + [0, 8),
       // chunk 2cc), (keys wk + [8, 16), chunk 2cc), then 2cc + 1
@@ -442,10 +479,10 @@ __global__ void __launch_bounds__(kTThreads, NT > 2 ? 1 : 2)
         split_codes(r[3], vc[2], vc[3]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          mma_bf16_16816(o[2 * cc][nt], va, ph[nt][0], ph[nt][1]);
-          mma_bf16_16816(o[2 * cc + 1][nt], vc, ph[nt][0], ph[nt][1]);
-          mma_bf16_16816(o[2 * cc][nt], va, pl[nt][0], pl[nt][1]);
-          mma_bf16_16816(o[2 * cc + 1][nt], vc, pl[nt][0], pl[nt][1]);
+          mma_f16(o[2 * cc][nt], va, ph[nt][0], ph[nt][1]);
+          mma_f16(o[2 * cc + 1][nt], vc, ph[nt][0], ph[nt][1]);
+          mma_f16(o[2 * cc][nt], va, pl[nt][0], pl[nt][1]);
+          mma_f16(o[2 * cc + 1][nt], vc, pl[nt][0], pl[nt][1]);
         }
       }
     }
@@ -549,6 +586,480 @@ __global__ void __launch_bounds__(kTThreads, NT > 2 ? 1 : 2)
   }
 }
 
+// ---- more rows: tcgen05 -----------------------------------------------------------
+
+constexpr int kCThreads = 512;  // control, converter and two softmax warpgroups
+constexpr int kKStages = 4;     // K tiles in flight (int8, 16 KiB)
+constexpr int kVStages = 3;     // V tiles in flight (the same)
+// Registers: 128 a thread at launch; the control warpgroup drops to 56 and the
+// converters to 72, the softmax warpgroups rise to 192 (a row's 128 scores).
+constexpr uint32_t kRegsControl = 56, kRegsConvert = 72, kRegsSoftmax = 192;
+static_assert(kRegsControl + kRegsConvert + 2 * kRegsSoftmax <= 4 * (65536 / kCThreads),
+              "register split exceeds the launch allocation");
+
+struct CL {  // shared memory layout (bytes from a 1024-aligned base)
+  static constexpr int kQ = 0;                            // int8 [128][128] SW128
+  static constexpr int kK = 16384;                        // kKStages x 16 KiB
+  static constexpr int kV = kK + kKStages * 16384;        // kVStages x 16 KiB
+  static constexpr int kVf = kV + kVStages * 16384;       // 2 x f16 [2 dim halves][128 keys][64] SW128
+  static constexpr int kScales = kVf + 2 * 32768;         // [8 warps][ks, log2 vs, 1 / vs][128]
+  static constexpr int kML = kScales + 8 * 3 * 128 * 4;   // [2 lanes][128] (m, l)
+  static constexpr int kPar = kML + 2 * 128 * 8;          // int[64]
+  static constexpr int kPre = kPar + kMaxDrafts * 4;      // int[batch + 1]
+  static constexpr int kBars = kPre + (kMaxBatch + 4) * 4;
+  static constexpr int kNumBars = 9 + 2 * kKStages + 2 * kVStages + 4;
+  static constexpr int kTmemSlot = kBars + kNumBars * 8;
+  static constexpr int kBytes = kTmemSlot + 16 + 1024;
+};
+static_assert(CL::kBytes <= 232448, "one CTA per SM");
+static_assert(CL::kBars % 8 == 0, "aligned");
+
+// B operand with N contiguous (128-byte swizzle): 64 values of N to a 128-byte
+// row of one k, rows of 8 k 1024 bytes together and those back to back (stride
+// byte offset), the next 64 of N 16384 bytes on (leading byte offset).
+__device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(16384u >> 4) << 16;
+  d |= static_cast<uint64_t>(1024u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(2u) << 61;
+  return d;
+}
+
+// A CTA's tiles of one segment.
+struct Piece {
+  Place at;  // its first tile
+  int n;     // tiles
+};
+__device__ __forceinline__ Piece piece_at(const Place& at, int left) {
+  return Piece{at, min(at.tiles - at.tile, left)};
+}
+__device__ __forceinline__ void next_piece(const int* pre, int batch, int per_seq, Place& at,
+                                           int n, int& left) {
+  left -= n;
+  at.tile += n - 1;
+  next_unit(pre, batch, per_seq, at);
+}
+
+__global__ void __launch_bounds__(kCThreads, 1)
+    tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
+                   const __grid_constant__ CUtensorMap vmap, TreeArgs a) {
+  extern __shared__ uint8_t sm_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) &
+                                           ~static_cast<uintptr_t>(1023));
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(sm + CL::kBars);  // the segment's Q is in
+  uint64_t* o_free = q_full + 1;    // its accumulators have been read
+  uint64_t* drain = q_full + 2;
+  uint64_t* s_full = q_full + 3;    // [2] S_x and every product before it done
+  uint64_t* p_full = q_full + 5;    // [2] P' is in S_x
+  uint64_t* o_done = q_full + 7;    // [2] the lane's last product done
+  uint64_t* k_full = q_full + 9;
+  uint64_t* k_empty = k_full + kKStages;
+  uint64_t* v_full = k_empty + kKStages;
+  uint64_t* v_empty = v_full + kVStages;
+  uint64_t* f_full = v_empty + kVStages;  // [2] f16 V
+  uint64_t* f_empty = f_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + CL::kTmemSlot);
+  int* par = reinterpret_cast<int*>(sm + CL::kPar);
+  int* pre = reinterpret_cast<int*>(sm + CL::kPre);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cta = blockIdx.x;
+  int* err = a.err;
+  if (tid == 0) {
+    prefetch_tensormap(&kmap);
+    prefetch_tensormap(&vmap);
+    mbar_init(q_full, 256);
+    mbar_init(o_free, 256);
+    mbar_init(drain, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&o_done[i], 1);
+      mbar_init(&f_full[i], 4);
+      mbar_init(&f_empty[i], 1);
+    }
+    for (int i = 0; i < kKStages; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < kVStages; ++i) {
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 4);
+    }
+    fence_barrier_init();
+  }
+  pdl_wait();
+  pdl_trigger();
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  count_tiles<kCThreads>(a, pre, par);
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // columns: S_0 [0, 128), S_1 [128, 256), O_0 [256, 384), O_1 [384, 512)
+  const uint32_t tS = tmem, tO = tmem + 256;
+
+  const int per_seq = a.heads_kv * a.qtiles;
+  const long long units = static_cast<long long>(pre[a.batch]) * per_seq;
+  const long long u0 = units * cta / a.ctas, u1 = units * (cta + 1) / a.ctas;
+  const int nunits = static_cast<int>(u1 - u0);
+  Place at{};
+  int left = nunits;
+  if (nunits > 0) at = place_of(pre, a.batch, per_seq, u0);
+  const int first_seg = at.b * per_seq + at.hq;
+  const bool first_cut = at.tile > 0;
+  if (nunits == 0 && tid == 0) a.meta[cta] = make_int4(-1, 0, -1, 0);
+
+  if (warp < 4) {
+    setmaxnreg_dec<kRegsControl>();
+    if (warp == 0 && lane < 2) {
+      // ---------------- TMA: lane 0 the K ring, lane 1 the V ring ----------------
+      const int stages = lane == 0 ? kKStages : kVStages;
+      uint64_t* full = lane == 0 ? k_full : v_full;
+      uint64_t* empty = lane == 0 ? k_empty : v_empty;
+      const CUtensorMap* map = lane == 0 ? &kmap : &vmap;
+      uint8_t* ring = sm + (lane == 0 ? CL::kK : CL::kV);
+      int issued = 0;
+      for (; issued < nunits; ++issued) {
+        const int s = issued % stages;
+        if (!mbar_wait(&empty[s], ((issued / stages) & 1) ^ 1u, err, kDevTimeoutEmpty)) break;
+        mbar_arrive_expect_tx(&full[s], 16384);
+        tma_load_3d(ring + s * 16384, map, &full[s], 0, at.tile * kTileKeys,
+                    at.b * a.heads_kv + at.hq / a.qtiles);
+        next_unit(pre, a.batch, per_seq, at);
+      }
+      // copies in flight land before exit
+      for (int j = issued > stages ? issued - stages : 0; j < issued; ++j)
+        mbar_wait(&full[j % stages], (j / stages) & 1, err, kDevTimeoutDrain);
+    } else if (warp == 1 && lane == 0 && nunits > 0) {
+      // ---------------- MMA ----------------
+      constexpr uint32_t kIdescS = idesc_i8(128, 128);
+      constexpr uint32_t kIdescO = idesc_f16(128, 128, true);
+      const uint32_t sq = smem_u32(sm + CL::kQ);
+      int kc = 0, fc = 0, pc[2] = {0, 0};
+      bool ok = true;
+      auto issue_s = [&](int x) {  // the next K tile against Q into S_x
+        const int s = kc % kKStages;
+        if (!mbar_wait(&k_full[s], (kc / kKStages) & 1, err, kDevTimeoutFull)) return false;
+        tc_fence_after();
+        const uint32_t sk = smem_u32(sm + CL::kK + s * 16384);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          mma_i8(tS + x * 128, smem_desc_k_sw128(sq + kk * 32), smem_desc_k_sw128(sk + kk * 32),
+                 kIdescS, kk > 0 ? 1u : 0u);
+        mma_commit(&s_full[x]);
+        mma_commit(&k_empty[s]);
+        ++kc;
+        return true;
+      };
+      for (int piece = 0; left > 0 && ok; ++piece) {
+        const Piece w = piece_at(at, left);
+        ok = mbar_wait(q_full, piece & 1, err, kDevTimeoutFull);
+        if (ok) ok = issue_s(0);
+        if (ok && w.n > 1) ok = issue_s(1);
+        for (int j = 0; j < w.n && ok; ++j) {
+          const int x = j & 1, f = fc & 1;
+          ok = mbar_wait(&p_full[x], pc[x]++ & 1, err, kDevTimeoutFull) &&
+               mbar_wait(&f_full[f], (fc >> 1) & 1, err, kDevTimeoutFull) &&
+               (j > 0 || piece == 0 || mbar_wait(o_free, (piece - 1) & 1, err, kDevTimeoutAccEmpty));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t sv = smem_u32(sm + CL::kVf + f * 32768);
+#pragma unroll
+          for (int kk = 0; kk < 16; ++kk)  // 16 keys a step: 8 columns of the heads, then the rests
+            mma_f16_tmem_a(tO + x * 128, tS + x * 128 + kk * 8,
+                           smem_desc_mn_sw128(sv + (kk & 7) * 2048), kIdescO,
+                           (j > 1 || kk > 0) ? 1u : 0u);
+          mma_commit(&f_empty[f]);
+          ++fc;
+          if (j + 2 < w.n) ok = issue_s(x);
+          else mma_commit(&o_done[x]);
+        }
+        next_piece(pre, a.batch, per_seq, at, w.n, left);
+      }
+      mma_commit(drain);
+      mbar_wait(drain, 0, err, kDevTimeoutDrain);
+    }
+  } else if (warp < 8) {
+    setmaxnreg_dec<kRegsConvert>();
+    // ---------------- V's codes to f16: thread t takes key t of every tile ----------------
+    const int t = tid - 128;
+    bool ok = true;
+    for (int j = 0; j < nunits; ++j) {
+      const int s = j % kVStages, f = j & 1;
+      const int key = at.tile * kTileKeys + t;
+      const float vs = key < a.max_len
+                           ? __ldg(a.v_scale + (static_cast<long long>(at.b) * a.heads_kv +
+                                                at.hq / a.qtiles) * a.max_len + key)
+                           : 0.0f;
+      if (ok) ok = mbar_wait(&v_full[s], (j / kVStages) & 1, err, kDevTimeoutFull);
+      uint4 v[8];
+      const uint8_t* row = sm + CL::kV + s * 16384 + t * 128;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) v[c] = *reinterpret_cast<const uint4*>(row + ((c ^ (t & 7)) << 4));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&v_empty[s]);
+      if (ok) ok = mbar_wait(&f_empty[f], ((j >> 1) & 1) ^ 1u, err, kDevTimeoutEmpty);
+      uint8_t* out = sm + CL::kVf + f * 32768 + t * 128;
+      const bool zero = vs < kNoScale;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {  // 16 dims: two 16-byte pieces of f16
+        const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+        uint32_t h[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t u = zero ? 0x80808080u : w[e] ^ 0x80808080u;
+          h[2 * e] = unbias(__byte_perm(u, 0x64646464u, 0x4140));
+          h[2 * e + 1] = unbias(__byte_perm(u, 0x64646464u, 0x4342));
+        }
+        uint8_t* o = out + (c >> 2) * 16384;
+        const int p = (c & 3) * 2;
+        *reinterpret_cast<uint4*>(o + ((p ^ (t & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(o + (((p + 1) ^ (t & 7)) << 4)) =
+            make_uint4(h[4], h[5], h[6], h[7]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&f_full[f]);
+      next_unit(pre, a.batch, per_seq, at);
+    }
+  } else {
+    setmaxnreg_inc<kRegsSoftmax>();
+    // ---------------- softmax of lane x; thread t owns query row t of the tile ----------------
+    const int x = (warp - 8) >> 2;
+    const int t = (warp & 3) * 32 + lane;  // == TMEM lane
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tSx = tS + x * 128 + lane_off;
+    float* scw = reinterpret_cast<float*>(sm + CL::kScales) + (warp - 8) * 384;
+    float2* ml = reinterpret_cast<float2*>(sm + CL::kML);  // [2][128]
+    const float base = a.sm_scale * kLog2e;
+    int sphase = 0, ophase = 0;
+    bool ok = true;
+    while (left > 0) {
+      const Piece w = piece_at(at, left);
+      const int b = w.at.b, hkv = w.at.hq / a.qtiles;
+      const int seg = b * per_seq + w.at.hq;
+      const int len = a.lens[b];
+      bool bad;
+      const int d = drafts_of(a, b, len, &bad);
+      const int r = (w.at.hq % a.qtiles) * kTcRows + t;  // query row of the KV head
+      const bool live = r < d * a.group;
+      const int node = r / a.group;
+      const long long qrow = (static_cast<long long>(b) * a.drafts + node) * a.heads_q +
+                             hkv * a.group + (r - node * a.group);
+      {  // this group's half of the row of Q
+        uint8_t* q = sm + CL::kQ + t * 128;
+#pragma unroll
+        for (int c = 4 * x; c < 4 * x + 4; ++c) {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (live) v = __ldg(reinterpret_cast<const uint4*>(a.q8 + qrow * 128) + c);
+          *reinterpret_cast<uint4*>(q + ((c ^ (t & 7)) << 4)) = v;
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(q_full);
+      }
+      if (a.parents != nullptr && tid - 256 < d)
+        par[tid - 256] = a.parents[static_cast<long long>(b) * a.drafts + tid - 256];
+      named_barrier(1, 256);
+      unsigned long long bits = 0;  // the drafted tokens that this row sees
+      if (live) {
+        if (a.parents == nullptr) {
+          bits = (2ull << node) - 1;
+        } else {
+          for (int i = node; i >= 0;) {  // strictly downwards: it ends
+            bits |= 1ull << i;
+            const int p = par[i];
+            i = p < i ? p : -1;
+          }
+        }
+      }
+      const float amul = live ? a.q_scale[qrow] * base : 0.0f;
+      // a warp without a live row only keeps the barriers going
+      const bool idle = !__any_sync(0xffffffffu, live);
+      const long long srow =
+          (static_cast<long long>(b) * a.heads_kv + hkv) * a.max_len;
+      const float4* ks4 = reinterpret_cast<const float4*>(a.k_scale + srow);
+      const float4* vs4 = reinterpret_cast<const float4*>(a.v_scale + srow);
+      auto scales = [&](int i, float4& k, float4& v) {  // this lane's four keys of tile i
+        const int key = (w.at.tile + i) * kTileKeys + 4 * lane;
+        k = v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < w.n && key < a.max_len) {
+          k = __ldg(ks4 + (key >> 2));
+          v = __ldg(vs4 + (key >> 2));
+        }
+      };
+      float4 nk, nv;
+      scales(x, nk, nv);
+      float m = -INFINITY, l = 0.0f;
+      for (int i = x; i < w.n; i += 2) {
+        __syncwarp();  // the warp is done with the last tile's scales
+        reinterpret_cast<float4*>(scw)[lane] = nk;
+        reinterpret_cast<float4*>(scw + 128)[lane] = make_float4(
+            scale_log2(nv.x), scale_log2(nv.y), scale_log2(nv.z), scale_log2(nv.w));
+        reinterpret_cast<float4*>(scw + 256)[lane] =
+            make_float4(scale_rcp(nv.x), scale_rcp(nv.y), scale_rcp(nv.z), scale_rcp(nv.w));
+        __syncwarp();
+        scales(i + 2, nk, nv);
+        if (ok) ok = mbar_wait(&s_full[x], sphase & 1, err, kDevTimeoutAccFull);
+        ++sphase;
+        ok = __all_sync(0xffffffffu, ok);  // reconverge before warp-collective tcgen05.ld
+        if (idle) {
+          mbar_arrive(&p_full[x]);
+          continue;
+        }
+        tc_fence_after();
+        uint32_t s[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          tmem_ld_32x32b_x32(tSx + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
+        tmem_ld_wait();
+        // scores in log2 units, with the key's V scale
+        const float4* k4 = reinterpret_cast<const float4*>(scw);
+        const float4* lv4 = reinterpret_cast<const float4*>(scw + 128);
+        const float4* rv4 = reinterpret_cast<const float4*>(scw + 256);
+        float mt = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 128; e += 4) {
+          const float4 k = k4[e >> 2], lv = lv4[e >> 2];
+          const float f0 = fmaf(small_i2f(static_cast<int>(s[e])) * amul, k.x, lv.x);
+          const float f1 = fmaf(small_i2f(static_cast<int>(s[e + 1])) * amul, k.y, lv.y);
+          const float f2 = fmaf(small_i2f(static_cast<int>(s[e + 2])) * amul, k.z, lv.z);
+          const float f3 = fmaf(small_i2f(static_cast<int>(s[e + 3])) * amul, k.w, lv.w);
+          s[e] = __float_as_uint(f0);
+          s[e + 1] = __float_as_uint(f1);
+          s[e + 2] = __float_as_uint(f2);
+          s[e + 3] = __float_as_uint(f3);
+        }
+        const int over = (w.at.tile + i) * kTileKeys - len;  // key e is drafted token over + e
+        const bool edge = over + kTileKeys > 0;
+        if (edge) {
+#pragma unroll
+          for (int e = 0; e < 128; ++e) {
+            const int n = over + e;
+            if (n >= 0 && (n >= kMaxDrafts || ((bits >> n) & 1ull) == 0))
+              s[e] = 0xff800000u;  // -inf
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 128; ++e) mt = fmaxf(mt, __uint_as_float(s[e]));
+        // The rescale is warp-collective, so the warp decides: when any row
+        // passes its maximum, every row moves to its own new one.
+        const bool first = i == x;
+        float alpha = 1.0f;
+        bool rescale = false;
+        if (__any_sync(0xffffffffu, mt > m + kLazy)) {
+          const float m_new = fmaxf(m, mt);
+          alpha = m == -INFINITY ? 0.0f : fast_exp2(m - m_new);
+          m = m_new;
+          rescale = !first;
+        }
+        const float nm = kLift - (m == -INFINITY ? 0.0f : m);
+        float ls = 0.0f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // 64 keys: 32 columns of heads, 32 of rests
+          uint32_t hi[32], lo[32];
+#pragma unroll
+          for (int e = 0; e < 64; e += 4) {
+            const float4 rv = rv4[h * 16 + (e >> 2)];
+            const float p0 = fast_exp2(__uint_as_float(s[h * 64 + e]) + nm);
+            const float p1 = fast_exp2(__uint_as_float(s[h * 64 + e + 1]) + nm);
+            const float p2 = fast_exp2(__uint_as_float(s[h * 64 + e + 2]) + nm);
+            const float p3 = fast_exp2(__uint_as_float(s[h * 64 + e + 3]) + nm);
+            if (edge) {  // what is masked adds nothing, whatever its scales
+              ls += (p0 == 0.0f ? 0.0f : p0 * rv.x) + (p1 == 0.0f ? 0.0f : p1 * rv.y) +
+                    (p2 == 0.0f ? 0.0f : p2 * rv.z) + (p3 == 0.0f ? 0.0f : p3 * rv.w);
+            } else {
+              ls = fmaf(p3, rv.w, fmaf(p2, rv.z, fmaf(p1, rv.y, fmaf(p0, rv.x, ls))));
+            }
+            hi[e >> 1] = half2_of(p0, p1);
+            hi[(e >> 1) + 1] = half2_of(p2, p3);
+            lo[e >> 1] = rest_of(p0, p1, hi[e >> 1]);
+            lo[(e >> 1) + 1] = rest_of(p2, p3, hi[(e >> 1) + 1]);
+          }
+          tmem_st_32x32b_x32(tSx + h * 32, hi);
+          tmem_st_32x32b_x32(tSx + 64 + h * 32, lo);
+        }
+        l = fmaf(l, alpha, ls);
+        if (rescale) {  // S_x(i) complete: so is every product on O_x before it
+          const uint32_t tOx = tO + x * 128 + lane_off;
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(tOx + c * 32, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st_32x32b_x32(tOx + c * 32, o);
+          }
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&p_full[x]);
+      }
+      // ---- the segment's end in this CTA: join the two lanes, half of the dims
+      // each
+      if (w.n > x) {
+        if (ok) ok = mbar_wait(&o_done[x], ophase & 1, err, kDevTimeoutAccFull);
+        ++ophase;
+      }
+      ml[x * 128 + t] = make_float2(m, l);
+      named_barrier(1, 256);  // both lanes' products are done, m and l in
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+      const float2 a0 = ml[t], a1 = ml[128 + t];
+      const float mx = fmaxf(a0.x, a1.x);
+      const float w0 = a0.x == -INFINITY ? 0.0f : exp2f(a0.x - mx);
+      const float w1 = a1.x == -INFINITY ? 0.0f : exp2f(a1.x - mx);
+      const float ls = a0.y * w0 + a1.y * w1;
+      const bool ends = w.at.tile + w.n == w.at.tiles;
+      const bool cut_before = seg == first_seg && first_cut;
+      const bool whole = ends && !cut_before;
+      float* prow = a.part + ((static_cast<long long>(cta) * 2 + (cut_before ? 0 : 1)) * kTcRows +
+                              t) * kPartRow;
+      float* dst = whole ? a.out + qrow * 128 : prow + 4;
+      const float scale = whole ? 1.0f / ls : 1.0f;
+      if (!idle) {
+#pragma unroll 1
+        for (int c = 2 * x; c < 2 * x + 2; ++c) {
+          uint32_t o0[32], o1[32];
+          tmem_ld_32x32b_x32(tO + lane_off + c * 32, o0);
+          if (w.n > 1) tmem_ld_32x32b_x32(tO + 128 + lane_off + c * 32, o1);
+          tmem_ld_wait();
+          if (live) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              float v[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                v[k] = w0 == 0.0f ? 0.0f : __uint_as_float(o0[e + k]) * w0;
+                if (w.n > 1 && w1 != 0.0f) v[k] = fmaf(__uint_as_float(o1[e + k]), w1, v[k]);
+                v[k] *= scale;
+              }
+              *reinterpret_cast<float4*>(dst + c * 32 + e) = make_float4(v[0], v[1], v[2], v[3]);
+            }
+          }
+        }
+      }
+      if (!whole && x == 0) {
+        prow[0] = mx;
+        prow[1] = ls;
+      }
+      tc_fence_before();
+      mbar_arrive(o_free);
+      if (left == w.n && tid == 256)
+        a.meta[cta] = make_int4(first_seg, first_cut ? 1 : 0, seg, ends ? 0 : 1);
+      next_piece(pre, a.batch, per_seq, at, w.n, left);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
 // Joins the partials of the segments that several CTAs share.  Block (c, i):
 // the segment that CTA c leaves unfinished after beginning it, query rows
 // [8i, 8i + 8) of it, one warp each (a lane holds four dims); the partials are
@@ -594,40 +1105,43 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a, int tile_row
       make_float4(o.x / l, o.y / l, o.z / l, o.w / l);
 }
 
-template <int NT>
-int launch_tree(const CUtensorMap& km, const CUtensorMap& vm, TreeArgs& a, cudaStream_t st) {
-  static int per_sm[64] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return kErrCuda;
-  if (per_sm[dev] == 0) {
-    int n = 0;
-    if (cudaFuncSetAttribute(tree_mma_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             TL::kBytes) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, tree_mma_kernel<NT>, kTThreads,
-                                                      TL::kBytes) != cudaSuccess ||
-        n <= 0)
-      return kErrCuda;
-    per_sm[dev] = std::min(n, kMaxCtasPerSm);
-  }
-  a.qtiles = (a.rows + 8 * NT - 1) / (8 * NT);
-  // one wave, and no more CTAs than the cache has room for units
+// One kernel over one wave of CTAs, then the join.
+int launch_tree(void (*kernel)(CUtensorMap, CUtensorMap, TreeArgs), int threads, int smem,
+                int per_sm, int tile_rows, const CUtensorMap& km, const CUtensorMap& vm,
+                TreeArgs& a, cudaStream_t st) {
+  a.qtiles = (a.rows + tile_rows - 1) / tile_rows;
+  // no more CTAs than the cache has room for units
   const long long most = static_cast<long long>(a.batch) * a.heads_kv * a.qtiles *
                          ((a.max_len + kTileKeys - 1) / kTileKeys);
-  a.ctas = static_cast<int>(std::min<long long>(static_cast<long long>(per_sm[dev]) * num_sms(),
-                                                most));
-  if (int rc = launch_k(tree_mma_kernel<NT>, dim3(static_cast<unsigned>(a.ctas)), dim3(kTThreads),
-                        TL::kBytes, st, km, vm, a))
+  a.ctas = static_cast<int>(std::min<long long>(static_cast<long long>(per_sm) * num_sms(), most));
+  if (int rc = launch_k(kernel, dim3(static_cast<unsigned>(a.ctas)), dim3(threads), smem, st, km,
+                        vm, a))
     return rc;
   PdlScope pdl;
-  return launch_k(tree_join_kernel, dim3(static_cast<unsigned>(a.ctas), NT), dim3(256), 0, st,
-                  a, 8 * NT);
+  return launch_k(tree_join_kernel, dim3(static_cast<unsigned>(a.ctas), tile_rows / 8), dim3(256),
+                  0, st, a, tile_rows);
+}
+
+// The kernels' shared memory, asked for once per device.
+bool opt_in() {
+  static bool done[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return false;
+  if (!done[dev]) {
+    const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    done[dev] = cudaFuncSetAttribute(tree_mma_kernel<1>, attr, TL::kBytes) == cudaSuccess &&
+                cudaFuncSetAttribute(tree_mma_kernel<2>, attr, TL::kBytes) == cudaSuccess &&
+                cudaFuncSetAttribute(tree_tc_kernel, attr, CL::kBytes) == cudaSuccess;
+  }
+  return done[dev];
 }
 
 }  // namespace
 
 size_t tree_attn_workspace_bytes() {
   const size_t ctas = static_cast<size_t>(kMaxCtasPerSm) * num_sms();
-  return ctas * 2 * kMaxTileRows * kPartRow * sizeof(float) + ctas * sizeof(int4);
+  const size_t rows = std::max<size_t>(ctas * kMaxTileRows, num_sms() * kTcRows);
+  return rows * 2 * kPartRow * sizeof(float) + ctas * sizeof(int4);
 }
 
 int tree_attn_i8(const TreeProblem& p, cudaStream_t st) {
@@ -661,9 +1175,12 @@ int tree_attn_i8(const TreeProblem& p, cudaStream_t st) {
     return rc;
   if (int rc = make_tma_3d_i8(&vm, p.v_cache, p.max_len, 128, 128, pairs, seg, 128, kTileKeys))
     return rc;
-  if (a.rows <= 8) return launch_tree<1>(km, vm, a, st);
-  if (a.rows <= 16) return launch_tree<2>(km, vm, a, st);
-  return launch_tree<4>(km, vm, a, st);
+  if (!opt_in()) return kErrCuda;
+  if (a.rows <= 8)
+    return launch_tree(tree_mma_kernel<1>, kTThreads, TL::kBytes, 2, 8, km, vm, a, st);
+  if (a.rows <= 16)
+    return launch_tree(tree_mma_kernel<2>, kTThreads, TL::kBytes, 2, 16, km, vm, a, st);
+  return launch_tree(tree_tc_kernel, kCThreads, CL::kBytes, 1, kTcRows, km, vm, a, st);
 }
 
 }  // namespace reef

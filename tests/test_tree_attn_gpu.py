@@ -2,12 +2,18 @@
 implementation in 64 bits on the dequantised inputs.
 
 Tolerance, per output element, relative to W = sum p |v| / sum p (what the
-element's terms add up to without cancelling): P goes into the product as two
-bf16 terms, each rounding off by half a step (2^-9 of what is left): 2^-18
-together; exp2 is off by 2 ulp and a score s (log2 units) by four fp32 roundings,
-2^-22 and 2^-22 max|s| of p, in the numerator and in the denominator; every
-fp32 add of the products may lose 2^-23, over n / 64 adds in a warp (two terms
-per 16 of every 128 keys) and a few dozen where warps and CTAs are joined.
+element's terms add up to without cancelling).  P, with the key's V scale and
+lifted to 2^11 at the largest or more, goes into the product as two f16 terms, each
+rounding off by half a step, 2^-12 of what is left (2^-24 together), or by half
+of the smallest number, 2^-25, where that is more: whatever W is, an element
+may be off by 2^-36 of the row's largest p * v_scale for each unit of the keys'
+codes, 2^-36 max(p v_scale) sum |code| in all (it is what is left where the keys
+that count have a code of 0 there).  exp2 is
+off by 2 ulp (2^-22), log2 of a V scale by 2^-22 and a score s (log2 units,
+that log2 in it) by four fp32 roundings, 2^-22 max|s| of p, in the numerator and in
+the denominator; every fp32 add of the products may lose 2^-23, over n / 64 adds
+(two terms per 16 of every 128 keys in a warp, or per 16 of every 256 in a lane)
+and a few dozen where warps, lanes and CTAs are joined.
 """
 import math
 
@@ -79,9 +85,12 @@ def check(x, lens, parents, draft_lens, out, sm):
             v = torch.nan_to_num(v) if not torch.isfinite(v).all() else v
             want, weight = p @ v, p @ v.abs()
             smax = float(s[sees].abs().max()) * math.log2(math.e)
-            rel = 2.0**-18 + 2 * (1 + smax) * 2.0**-22 + ((n + d) / 64 + 32) * 2.0**-23
-            assert bool(((out[i, :d, h].double() - want).abs() <= rel * weight + 1e-30).all()), \
-                (i, h, float(((out[i, :d, h].double() - want).abs() / weight).max()), rel)
+            smax += float(torch.log2(vs[i, kh, : n + d]).abs().max())
+            rel = 2.0**-24 + 2 * (2 + smax) * 2.0**-22 + ((n + d) / 64 + 32) * 2.0**-23
+            codes = x["v_cache"][i, kh, : n + d].double().abs().sum(0)
+            small = 2.0**-36 * (p * vs[i, kh, : n + d].double()).amax(1, keepdim=True) * codes
+            off = (out[i, :d, h].double() - want).abs()
+            assert bool((off <= rel * weight + small).all()), (i, h, float((off / weight).max()), rel)
 
 
 def run(x, lens, parents=None, draft_lens=None, sm=None, **kw):
@@ -107,6 +116,9 @@ CASES = [
     (5, 8, 8, 1, 2048, [2040, 1, 1000, 129, 0], [8, 3, 8, 1, 8], True),
     (2, 3, 16, 1, 4096, [4000, 77], None, True),     # 48 rows, several row tiles
     (1, 2, 40, 2, 640, [600], None, False),          # 40 rows of one KV head
+    (2, 48, 32, 4, 1500, [1400, 129], [48, 11], True),   # 384 rows: several tiles of 128
+    (1, 17, 8, 1, 1024, [1000], None, True),         # 136 rows: a tile of eight
+    (150, 3, 8, 1, 400, [(97 * i) % 398 for i in range(150)], None, False),  # 24 rows, many segments
     (300, 2, 2, 1, 256, [(37 * i) % 254 for i in range(300)], None, False),  # more than CTAs
     (40, 16, 8, 2, 512, [(61 * i) % 497 for i in range(40)], [i % 17 for i in range(40)], True),
 ]
@@ -126,18 +138,36 @@ def test_flat_and_peaked_scores(std, sm):
     check(x, [390, 17], None, None, run(x, [390, 17], None, None, sm), sm)
 
 
-def test_scales_far_apart():
+@pytest.mark.parametrize("hq", [4, 16])
+def test_scales_far_apart(hq):
     """V scales of 2^-60 to 2^60 in one sequence: P times the scale keeps its range."""
-    x = make(1, 4, 4, 1, 256, seed=3)
+    x = make(1, 4, hq, 1, 256, seed=3)
     e = torch.arange(256, device="cuda").float() % 121 - 60
     x["v_scale"] = torch.exp2(e)[None, None].contiguous()
     check(x, [250], None, None, run(x, [250], None, None, 0.01), 0.01)
 
 
+@pytest.mark.parametrize("hq", [2, 16])
+def test_v_scales_of_zero(hq):
+    """Keys whose V scale is 0 take their share of the softmax and add nothing; where
+    all are, the output is 0."""
+    x = make(2, 4, hq, 1, 256, seed=13)
+    x["v_scale"][0, 0, ::2] = 0.0
+    x["v_scale"][1] = 0.0
+    out = run(x, [250, 100], sm=0.05)
+    assert not out[1].any()
+    v = x["v_cache"][0, 0, :254].double() * x["v_scale"][0, 0, :254, None].double()
+    k = x["k_cache"][0, 0, :254].double() * x["k_scale"][0, 0, :254, None].double()
+    q = x["q8"][0, 3].double() * x["q_scale"][0, 3, :, None].double()
+    p = torch.softmax(q @ k.T * 0.05, -1)
+    assert bool(((out[0, 3].double() - p @ v).abs() <= 1e-5 * (p @ v.abs())).all())
+
+
 @pytest.mark.parametrize("junk", [math.nan, math.inf, -math.inf, 3.4e38])
-def test_rows_nobody_sees_add_nothing(junk):
+@pytest.mark.parametrize("hq", [2, 8])  # 8 and 32 query rows: both kernels
+def test_rows_nobody_sees_add_nothing(junk, hq):
     """Scales behind the drafts, and of a sibling's row, that are not numbers."""
-    x = make(2, 4, 8, 1, 260, seed=5)
+    x = make(2, 4, hq, 1, 260, seed=5)
     parents = [[-1, 0, 0, 1], [-1, 0, 1, 2]]  # nodes 1 and 2 of sequence 0 are siblings
     lens = [126, 200]
     want = run(x, lens, parents, None, 0.1)
