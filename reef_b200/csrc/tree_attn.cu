@@ -33,13 +33,12 @@
 //
 // More rows, tree_tc_kernel: tcgen05 with a tile of 128 query rows, bound by
 // the exponentials and conversions of the softmax warps and the tensor pipe (S in
-// int8, P'.V twice in f16).  The CTA's key tiles go alternately to two lanes,
-// each with a score tile S_x and an accumulator O_x in TMEM and a softmax
-// warpgroup, one thread per query row; P' overwrites S_x (head in its first 64
-// columns, remainder in the last) and the product reads it there.  Another
-// warpgroup turns V's codes into f16, [key][dim] as they stand: the product
-// takes B with the dims contiguous.  The two lanes are joined at the segment's
-// end.
+// int8, P'.V twice in f16).  Scores go into two TMEM tiles in turn, so that the
+// next are there when the softmax of one ends; two warpgroups share a tile, a
+// thread holding half of a query row's 128 scores (a whole row spills); P'
+// overwrites the scores (its heads in the first 64 columns, the rests in the
+// last) and the product reads it there.  Another warpgroup turns V's codes into
+// f16, [key][dim] as they stand: the product takes B with the dims contiguous.
 #include "attn_mma.cuh"
 #include "common.cuh"
 #include "ops.h"
@@ -143,7 +142,8 @@ __device__ __forceinline__ void split_codes(uint32_t w, uint32_t& even, uint32_t
 }
 
 // log2 and reciprocal of a V scale (2^-22 off at most); of one that counts as
-// 0, of kNoScale instead (its codes are taken as zeros)
+// 0, of kNoScale instead (its codes are taken as zeros).  The reciprocal is
+// finite whatever the scale, so a masked key's P' = 0 times it is 0.
 __device__ __forceinline__ float scale_log2(float vs) {
   float y;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaxf(vs, kNoScale)));
@@ -165,7 +165,7 @@ __device__ __forceinline__ int drafts_of(const TreeArgs& a, int b, int len, bool
 template <int kThreads>
 __device__ __forceinline__ void count_tiles(const TreeArgs& a, int* pre, int* scratch) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  constexpr int kPer = kMaxBatch / kThreads;
+  constexpr int kPer = (kMaxBatch + kThreads - 1) / kThreads;
   const int b0 = tid * kPer;
   int t[kPer], sum = 0;
 #pragma unroll
@@ -450,13 +450,8 @@ __global__ void __launch_bounds__(kTThreads, 2)
         const float r1 = (m[nt][1] == -INFINITY ? 0.0f : m[nt][1]) - kLift;
         float p0 = fast_exp2(sc[nt][0] - r0), p1 = fast_exp2(sc[nt][1] - r1);
         float p2 = fast_exp2(sc[nt][2] - r0), p3 = fast_exp2(sc[nt][3] - r1);
-        if (edge) {  // what is masked adds nothing, whatever its scales
-          l[nt][0] += (p0 == 0.0f ? 0.0f : p0 * rv_lo) + (p2 == 0.0f ? 0.0f : p2 * rv_hi);
-          l[nt][1] += (p1 == 0.0f ? 0.0f : p1 * rv_lo) + (p3 == 0.0f ? 0.0f : p3 * rv_hi);
-        } else {
-          l[nt][0] = fmaf(p2, rv_hi, fmaf(p0, rv_lo, l[nt][0]));
-          l[nt][1] = fmaf(p3, rv_hi, fmaf(p1, rv_lo, l[nt][1]));
-        }
+        l[nt][0] = fmaf(p2, rv_hi, fmaf(p0, rv_lo, l[nt][0]));
+        l[nt][1] = fmaf(p3, rv_hi, fmaf(p1, rv_lo, l[nt][1]));
         if (vs_lo < kNoScale) p0 = p1 = 0.0f;
         if (vs_hi < kNoScale) p2 = p3 = 0.0f;
         const uint32_t h0 = half2_of(p0, p1), h1 = half2_of(p2, p3);
@@ -591,23 +586,18 @@ __global__ void __launch_bounds__(kTThreads, 2)
 constexpr int kCThreads = 512;  // control, converter and two softmax warpgroups
 constexpr int kKStages = 4;     // K tiles in flight (int8, 16 KiB)
 constexpr int kVStages = 3;     // V tiles in flight (the same)
-// Registers: 128 a thread at launch; the control warpgroup drops to 56 and the
-// converters to 72, the softmax warpgroups rise to 192 (a row's 128 scores).
-constexpr uint32_t kRegsControl = 56, kRegsConvert = 72, kRegsSoftmax = 192;
-static_assert(kRegsControl + kRegsConvert + 2 * kRegsSoftmax <= 4 * (65536 / kCThreads),
-              "register split exceeds the launch allocation");
 
 struct CL {  // shared memory layout (bytes from a 1024-aligned base)
   static constexpr int kQ = 0;                            // int8 [128][128] SW128
   static constexpr int kK = 16384;                        // kKStages x 16 KiB
   static constexpr int kV = kK + kKStages * 16384;        // kVStages x 16 KiB
   static constexpr int kVf = kV + kVStages * 16384;       // 2 x f16 [2 dim halves][128 keys][64] SW128
-  static constexpr int kScales = kVf + 2 * 32768;         // [8 warps][ks, log2 vs, 1 / vs][128]
-  static constexpr int kML = kScales + 8 * 3 * 128 * 4;   // [2 lanes][128] (m, l)
+  static constexpr int kScales = kVf + 2 * 32768;         // [8 warps][ks, log2 vs, 1 / vs][64]
+  static constexpr int kML = kScales + 8 * 3 * 64 * 4;    // [2 tiles][2 halves][128] maxima, then sums
   static constexpr int kPar = kML + 2 * 128 * 8;          // int[64]
   static constexpr int kPre = kPar + kMaxDrafts * 4;      // int[batch + 1]
   static constexpr int kBars = kPre + (kMaxBatch + 4) * 4;
-  static constexpr int kNumBars = 9 + 2 * kKStages + 2 * kVStages + 4;
+  static constexpr int kNumBars = 8 + 2 * kKStages + 2 * kVStages + 4;
   static constexpr int kTmemSlot = kBars + kNumBars * 8;
   static constexpr int kBytes = kTmemSlot + 16 + 1024;
 };
@@ -649,12 +639,12 @@ __global__ void __launch_bounds__(kCThreads, 1)
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) &
                                            ~static_cast<uintptr_t>(1023));
   uint64_t* q_full = reinterpret_cast<uint64_t*>(sm + CL::kBars);  // the segment's Q is in
-  uint64_t* o_free = q_full + 1;    // its accumulators have been read
+  uint64_t* o_free = q_full + 1;    // its accumulator has been read
   uint64_t* drain = q_full + 2;
-  uint64_t* s_full = q_full + 3;    // [2] S_x and every product before it done
-  uint64_t* p_full = q_full + 5;    // [2] P' is in S_x
-  uint64_t* o_done = q_full + 7;    // [2] the lane's last product done
-  uint64_t* k_full = q_full + 9;
+  uint64_t* s_full = q_full + 3;    // [2] S_x done
+  uint64_t* p_full = q_full + 5;    // P' of the next tile is in its S_x
+  uint64_t* o_done = q_full + 6;    // [2] an even / odd tile's product is in O
+  uint64_t* k_full = q_full + 8;
   uint64_t* k_empty = k_full + kKStages;
   uint64_t* v_full = k_empty + kKStages;
   uint64_t* v_empty = v_full + kVStages;
@@ -673,10 +663,10 @@ __global__ void __launch_bounds__(kCThreads, 1)
     mbar_init(q_full, 256);
     mbar_init(o_free, 256);
     mbar_init(drain, 1);
+    mbar_init(p_full, 256);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
       mbar_init(&o_done[i], 1);
+      mbar_init(&s_full[i], 1);
       mbar_init(&f_full[i], 4);
       mbar_init(&f_empty[i], 1);
     }
@@ -700,7 +690,7 @@ __global__ void __launch_bounds__(kCThreads, 1)
   count_tiles<kCThreads>(a, pre, par);
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // columns: S_0 [0, 128), S_1 [128, 256), O_0 [256, 384), O_1 [384, 512)
+  // columns: S_0 [0, 128), S_1 [128, 256), O [256, 384)
   const uint32_t tS = tmem, tO = tmem + 256;
 
   const int per_seq = a.heads_kv * a.qtiles;
@@ -715,7 +705,6 @@ __global__ void __launch_bounds__(kCThreads, 1)
   if (nunits == 0 && tid == 0) a.meta[cta] = make_int4(-1, 0, -1, 0);
 
   if (warp < 4) {
-    setmaxnreg_dec<kRegsControl>();
     if (warp == 0 && lane < 2) {
       // ---------------- TMA: lane 0 the K ring, lane 1 the V ring ----------------
       const int stages = lane == 0 ? kKStages : kVStages;
@@ -740,10 +729,10 @@ __global__ void __launch_bounds__(kCThreads, 1)
       constexpr uint32_t kIdescS = idesc_i8(128, 128);
       constexpr uint32_t kIdescO = idesc_f16(128, 128, true);
       const uint32_t sq = smem_u32(sm + CL::kQ);
-      int kc = 0, fc = 0, pc[2] = {0, 0};
+      int kc = 0, tc = 0;  // K tiles multiplied, tiles' products issued
       bool ok = true;
-      auto issue_s = [&](int x) {  // the next K tile against Q into S_x
-        const int s = kc % kKStages;
+      auto issue_s = [&] {  // the next K tile against Q into its S_x
+        const int s = kc % kKStages, x = kc & 1;
         if (!mbar_wait(&k_full[s], (kc / kKStages) & 1, err, kDevTimeoutFull)) return false;
         tc_fence_after();
         const uint32_t sk = smem_u32(sm + CL::kK + s * 16384);
@@ -759,25 +748,24 @@ __global__ void __launch_bounds__(kCThreads, 1)
       for (int piece = 0; left > 0 && ok; ++piece) {
         const Piece w = piece_at(at, left);
         ok = mbar_wait(q_full, piece & 1, err, kDevTimeoutFull);
-        if (ok) ok = issue_s(0);
-        if (ok && w.n > 1) ok = issue_s(1);
+        if (ok) ok = issue_s();
+        if (ok && w.n > 1) ok = issue_s();
         for (int j = 0; j < w.n && ok; ++j) {
-          const int x = j & 1, f = fc & 1;
-          ok = mbar_wait(&p_full[x], pc[x]++ & 1, err, kDevTimeoutFull) &&
-               mbar_wait(&f_full[f], (fc >> 1) & 1, err, kDevTimeoutFull) &&
+          const int x = tc & 1;
+          ok = mbar_wait(p_full, x, err, kDevTimeoutFull) &&
+               mbar_wait(&f_full[x], (tc >> 1) & 1, err, kDevTimeoutFull) &&
                (j > 0 || piece == 0 || mbar_wait(o_free, (piece - 1) & 1, err, kDevTimeoutAccEmpty));
           if (!ok) break;
           tc_fence_after();
-          const uint32_t sv = smem_u32(sm + CL::kVf + f * 32768);
+          const uint32_t sv = smem_u32(sm + CL::kVf + x * 32768);
 #pragma unroll
           for (int kk = 0; kk < 16; ++kk)  // 16 keys a step: 8 columns of the heads, then the rests
-            mma_f16_tmem_a(tO + x * 128, tS + x * 128 + kk * 8,
-                           smem_desc_mn_sw128(sv + (kk & 7) * 2048), kIdescO,
-                           (j > 1 || kk > 0) ? 1u : 0u);
-          mma_commit(&f_empty[f]);
-          ++fc;
-          if (j + 2 < w.n) ok = issue_s(x);
-          else mma_commit(&o_done[x]);
+            mma_f16_tmem_a(tO, tS + x * 128 + kk * 8, smem_desc_mn_sw128(sv + (kk & 7) * 2048),
+                           kIdescO, (j > 0 || kk > 0) ? 1u : 0u);
+          mma_commit(&f_empty[x]);
+          mma_commit(&o_done[x]);
+          ++tc;
+          if (j + 2 < w.n) ok = issue_s();
         }
         next_piece(pre, a.batch, per_seq, at, w.n, left);
       }
@@ -785,64 +773,64 @@ __global__ void __launch_bounds__(kCThreads, 1)
       mbar_wait(drain, 0, err, kDevTimeoutDrain);
     }
   } else if (warp < 8) {
-    setmaxnreg_dec<kRegsConvert>();
     // ---------------- V's codes to f16: thread t takes key t of every tile ----------------
     const int t = tid - 128;
     bool ok = true;
+    auto scale = [&] {  // of the tile at `at`
+      const int key = at.tile * kTileKeys + t;
+      return key < a.max_len ? __ldg(a.v_scale + (static_cast<long long>(at.b) * a.heads_kv +
+                                                  at.hq / a.qtiles) * a.max_len + key)
+                             : 0.0f;
+    };
+    float vs = nunits > 0 ? scale() : 0.0f;
     for (int j = 0; j < nunits; ++j) {
       const int s = j % kVStages, f = j & 1;
-      const int key = at.tile * kTileKeys + t;
-      const float vs = key < a.max_len
-                           ? __ldg(a.v_scale + (static_cast<long long>(at.b) * a.heads_kv +
-                                                at.hq / a.qtiles) * a.max_len + key)
-                           : 0.0f;
+      const bool zero = vs < kNoScale;
+      next_unit(pre, a.batch, per_seq, at);
+      if (j + 1 < nunits) vs = scale();  // a tile ahead
       if (ok) ok = mbar_wait(&v_full[s], (j / kVStages) & 1, err, kDevTimeoutFull);
-      uint4 v[8];
       const uint8_t* row = sm + CL::kV + s * 16384 + t * 128;
+      uint8_t* out = sm + CL::kVf + f * 32768 + t * 128;
+      uint4 v[8];
 #pragma unroll
       for (int c = 0; c < 8; ++c) v[c] = *reinterpret_cast<const uint4*>(row + ((c ^ (t & 7)) << 4));
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&v_empty[s]);
       if (ok) ok = mbar_wait(&f_empty[f], ((j >> 1) & 1) ^ 1u, err, kDevTimeoutEmpty);
-      uint8_t* out = sm + CL::kVf + f * 32768 + t * 128;
-      const bool zero = vs < kNoScale;
 #pragma unroll
       for (int c = 0; c < 8; ++c) {  // 16 dims: two 16-byte pieces of f16
         const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
-        uint32_t h[8];
+        uint32_t u[8];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const uint32_t u = zero ? 0x80808080u : w[e] ^ 0x80808080u;
-          h[2 * e] = unbias(__byte_perm(u, 0x64646464u, 0x4140));
-          h[2 * e + 1] = unbias(__byte_perm(u, 0x64646464u, 0x4342));
+          const uint32_t x = zero ? 0x80808080u : w[e] ^ 0x80808080u;
+          u[2 * e] = unbias(__byte_perm(x, 0x64646464u, 0x4140));
+          u[2 * e + 1] = unbias(__byte_perm(x, 0x64646464u, 0x4342));
         }
         uint8_t* o = out + (c >> 2) * 16384;
         const int p = (c & 3) * 2;
-        *reinterpret_cast<uint4*>(o + ((p ^ (t & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(o + ((p ^ (t & 7)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
         *reinterpret_cast<uint4*>(o + (((p + 1) ^ (t & 7)) << 4)) =
-            make_uint4(h[4], h[5], h[6], h[7]);
+            make_uint4(u[4], u[5], u[6], u[7]);
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&f_full[f]);
-      next_unit(pre, a.batch, per_seq, at);
+      if (lane == 0) {
+        mbar_arrive(&v_empty[s]);
+        mbar_arrive(&f_full[f]);
+      }
     }
   } else {
-    setmaxnreg_inc<kRegsSoftmax>();
-    // ---------------- softmax of lane x; thread t owns query row t of the tile ----------------
+    // ---------------- softmax: thread (x, t) has keys [64x, 64x + 64) of query row t ----------------
     const int x = (warp - 8) >> 2;
     const int t = (warp & 3) * 32 + lane;  // == TMEM lane
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t tSx = tS + x * 128 + lane_off;
-    float* scw = reinterpret_cast<float*>(sm + CL::kScales) + (warp - 8) * 384;
-    float2* ml = reinterpret_cast<float2*>(sm + CL::kML);  // [2][128]
+    float* scw = reinterpret_cast<float*>(sm + CL::kScales) + (warp - 8) * 192;
+    float* ml = reinterpret_cast<float*>(sm + CL::kML);  // [2][2][128]
     const float base = a.sm_scale * kLog2e;
-    int sphase = 0, ophase = 0;
+    int tc = 0;  // tiles done
     bool ok = true;
     while (left > 0) {
       const Piece w = piece_at(at, left);
       const int b = w.at.b, hkv = w.at.hq / a.qtiles;
-      const int seg = b * per_seq + w.at.hq;
       const int len = a.lens[b];
       bool bad;
       const int d = drafts_of(a, b, len, &bad);
@@ -851,7 +839,7 @@ __global__ void __launch_bounds__(kCThreads, 1)
       const int node = r / a.group;
       const long long qrow = (static_cast<long long>(b) * a.drafts + node) * a.heads_q +
                              hkv * a.group + (r - node * a.group);
-      {  // this group's half of the row of Q
+      {  // this half of the row of Q
         uint8_t* q = sm + CL::kQ + t * 128;
 #pragma unroll
         for (int c = 4 * x; c < 4 * x + 4; ++c) {
@@ -878,175 +866,165 @@ __global__ void __launch_bounds__(kCThreads, 1)
         }
       }
       const float amul = live ? a.q_scale[qrow] * base : 0.0f;
-      // a warp without a live row only keeps the barriers going
+      // a warp without a live row (as its partner in the other half) only keeps
+      // the barriers going
       const bool idle = !__any_sync(0xffffffffu, live);
-      const long long srow =
-          (static_cast<long long>(b) * a.heads_kv + hkv) * a.max_len;
-      const float4* ks4 = reinterpret_cast<const float4*>(a.k_scale + srow);
-      const float4* vs4 = reinterpret_cast<const float4*>(a.v_scale + srow);
-      auto scales = [&](int i, float4& k, float4& v) {  // this lane's four keys of tile i
-        const int key = (w.at.tile + i) * kTileKeys + 4 * lane;
-        k = v = make_float4(0.f, 0.f, 0.f, 0.f);
+      const long long srow = (static_cast<long long>(b) * a.heads_kv + hkv) * a.max_len;
+      auto scales = [&](int i, float2& k, float2& v) {  // this lane's two keys of tile i
+        const int key = (w.at.tile + i) * kTileKeys + 64 * x + 2 * lane;
+        k = v = make_float2(0.f, 0.f);
         if (i < w.n && key < a.max_len) {
-          k = __ldg(ks4 + (key >> 2));
-          v = __ldg(vs4 + (key >> 2));
+          k = __ldg(reinterpret_cast<const float2*>(a.k_scale + srow + key));
+          v = __ldg(reinterpret_cast<const float2*>(a.v_scale + srow + key));
         }
       };
-      float4 nk, nv;
-      scales(x, nk, nv);
+      float2 nk, nv;
+      scales(0, nk, nv);
       float m = -INFINITY, l = 0.0f;
-      for (int i = x; i < w.n; i += 2) {
+      for (int i = 0; i < w.n; ++i, ++tc) {
+        const uint32_t tSx = tS + (tc & 1) * 128 + lane_off;
         __syncwarp();  // the warp is done with the last tile's scales
-        reinterpret_cast<float4*>(scw)[lane] = nk;
-        reinterpret_cast<float4*>(scw + 128)[lane] = make_float4(
-            scale_log2(nv.x), scale_log2(nv.y), scale_log2(nv.z), scale_log2(nv.w));
-        reinterpret_cast<float4*>(scw + 256)[lane] =
-            make_float4(scale_rcp(nv.x), scale_rcp(nv.y), scale_rcp(nv.z), scale_rcp(nv.w));
+        reinterpret_cast<float2*>(scw)[lane] = nk;
+        reinterpret_cast<float2*>(scw + 64)[lane] =
+            make_float2(scale_log2(nv.x), scale_log2(nv.y));
+        reinterpret_cast<float2*>(scw + 128)[lane] = make_float2(scale_rcp(nv.x), scale_rcp(nv.y));
         __syncwarp();
-        scales(i + 2, nk, nv);
-        if (ok) ok = mbar_wait(&s_full[x], sphase & 1, err, kDevTimeoutAccFull);
-        ++sphase;
+        scales(i + 1, nk, nv);
+        if (ok) ok = mbar_wait(&s_full[tc & 1], (tc >> 1) & 1, err, kDevTimeoutAccFull);
         ok = __all_sync(0xffffffffu, ok);  // reconverge before warp-collective tcgen05.ld
+        tc_fence_after();
+        uint32_t s[64];
+        float mt = -INFINITY;
+        if (!idle) {
+          tmem_ld_32x32b_x32(tSx + x * 64, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+          tmem_ld_32x32b_x32(tSx + x * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
+          tmem_ld_wait();
+          // scores in log2 units, with the key's V scale
+          const float4* k4 = reinterpret_cast<const float4*>(scw);
+          const float4* lv4 = reinterpret_cast<const float4*>(scw + 64);
+#pragma unroll
+          for (int e = 0; e < 64; e += 4) {
+            const float4 k = k4[e >> 2], lv = lv4[e >> 2];
+            s[e] = __float_as_uint(fmaf(small_i2f(static_cast<int>(s[e])) * amul, k.x, lv.x));
+            s[e + 1] = __float_as_uint(fmaf(small_i2f(static_cast<int>(s[e + 1])) * amul, k.y, lv.y));
+            s[e + 2] = __float_as_uint(fmaf(small_i2f(static_cast<int>(s[e + 2])) * amul, k.z, lv.z));
+            s[e + 3] = __float_as_uint(fmaf(small_i2f(static_cast<int>(s[e + 3])) * amul, k.w, lv.w));
+          }
+          const int over = (w.at.tile + i) * kTileKeys + 64 * x - len;  // key e: drafted token over + e
+          if (over + 64 > 0) {
+#pragma unroll
+            for (int e = 0; e < 64; ++e) {
+              const int n = over + e;
+              if (n >= 0 && (n >= kMaxDrafts || ((bits >> n) & 1ull) == 0)) s[e] = 0xff800000u;
+            }
+          }
+          float mx[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx[e] = __uint_as_float(s[e]);
+#pragma unroll
+          for (int e = 4; e < 64; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(s[e]));
+          mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        }
+        // the other half's maximum; after the barrier both halves' scores are in
+        // registers, so P' may overwrite them
+        float* mrow = ml + (tc & 1) * 256;
+        mrow[x * 128 + t] = mt;
+        named_barrier(1, 256);
         if (idle) {
-          mbar_arrive(&p_full[x]);
+          mbar_arrive(p_full);
           continue;
         }
-        tc_fence_after();
-        uint32_t s[128];
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          tmem_ld_32x32b_x32(tSx + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
-        tmem_ld_wait();
-        // scores in log2 units, with the key's V scale
-        const float4* k4 = reinterpret_cast<const float4*>(scw);
-        const float4* lv4 = reinterpret_cast<const float4*>(scw + 128);
-        const float4* rv4 = reinterpret_cast<const float4*>(scw + 256);
-        float mt = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < 128; e += 4) {
-          const float4 k = k4[e >> 2], lv = lv4[e >> 2];
-          const float f0 = fmaf(small_i2f(static_cast<int>(s[e])) * amul, k.x, lv.x);
-          const float f1 = fmaf(small_i2f(static_cast<int>(s[e + 1])) * amul, k.y, lv.y);
-          const float f2 = fmaf(small_i2f(static_cast<int>(s[e + 2])) * amul, k.z, lv.z);
-          const float f3 = fmaf(small_i2f(static_cast<int>(s[e + 3])) * amul, k.w, lv.w);
-          s[e] = __float_as_uint(f0);
-          s[e + 1] = __float_as_uint(f1);
-          s[e + 2] = __float_as_uint(f2);
-          s[e + 3] = __float_as_uint(f3);
-        }
-        const int over = (w.at.tile + i) * kTileKeys - len;  // key e is drafted token over + e
-        const bool edge = over + kTileKeys > 0;
-        if (edge) {
-#pragma unroll
-          for (int e = 0; e < 128; ++e) {
-            const int n = over + e;
-            if (n >= 0 && (n >= kMaxDrafts || ((bits >> n) & 1ull) == 0))
-              s[e] = 0xff800000u;  // -inf
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 128; ++e) mt = fmaxf(mt, __uint_as_float(s[e]));
-        // The rescale is warp-collective, so the warp decides: when any row
-        // passes its maximum, every row moves to its own new one.
-        const bool first = i == x;
+        mt = fmaxf(mt, mrow[(x ^ 1) * 128 + t]);
+        // The rescale is warp-collective, so the warp decides (and its partner
+        // alike): when any row passes its maximum, every row moves to its own.
         float alpha = 1.0f;
         bool rescale = false;
         if (__any_sync(0xffffffffu, mt > m + kLazy)) {
           const float m_new = fmaxf(m, mt);
           alpha = m == -INFINITY ? 0.0f : fast_exp2(m - m_new);
           m = m_new;
-          rescale = !first;
+          rescale = i > 0;
         }
         const float nm = kLift - (m == -INFINITY ? 0.0f : m);
-        float ls = 0.0f;
+        const float4* rv4 = reinterpret_cast<const float4*>(scw + 128);
+        float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {  // 64 keys: 32 columns of heads, 32 of rests
-          uint32_t hi[32], lo[32];
+        for (int h = 0; h < 2; ++h) {  // 32 keys: 16 columns of heads, 16 of rests
+          uint32_t hi[16], lo[16];
 #pragma unroll
-          for (int e = 0; e < 64; e += 4) {
-            const float4 rv = rv4[h * 16 + (e >> 2)];
-            const float p0 = fast_exp2(__uint_as_float(s[h * 64 + e]) + nm);
-            const float p1 = fast_exp2(__uint_as_float(s[h * 64 + e + 1]) + nm);
-            const float p2 = fast_exp2(__uint_as_float(s[h * 64 + e + 2]) + nm);
-            const float p3 = fast_exp2(__uint_as_float(s[h * 64 + e + 3]) + nm);
-            if (edge) {  // what is masked adds nothing, whatever its scales
-              ls += (p0 == 0.0f ? 0.0f : p0 * rv.x) + (p1 == 0.0f ? 0.0f : p1 * rv.y) +
-                    (p2 == 0.0f ? 0.0f : p2 * rv.z) + (p3 == 0.0f ? 0.0f : p3 * rv.w);
-            } else {
-              ls = fmaf(p3, rv.w, fmaf(p2, rv.z, fmaf(p1, rv.y, fmaf(p0, rv.x, ls))));
-            }
+          for (int e = 0; e < 32; e += 4) {
+            const float4 rv = rv4[h * 8 + (e >> 2)];
+            const float p0 = fast_exp2(__uint_as_float(s[h * 32 + e]) + nm);
+            const float p1 = fast_exp2(__uint_as_float(s[h * 32 + e + 1]) + nm);
+            const float p2 = fast_exp2(__uint_as_float(s[h * 32 + e + 2]) + nm);
+            const float p3 = fast_exp2(__uint_as_float(s[h * 32 + e + 3]) + nm);
+            ls[0] = fmaf(p0, rv.x, ls[0]);
+            ls[1] = fmaf(p1, rv.y, ls[1]);
+            ls[2] = fmaf(p2, rv.z, ls[2]);
+            ls[3] = fmaf(p3, rv.w, ls[3]);
             hi[e >> 1] = half2_of(p0, p1);
             hi[(e >> 1) + 1] = half2_of(p2, p3);
             lo[e >> 1] = rest_of(p0, p1, hi[e >> 1]);
             lo[(e >> 1) + 1] = rest_of(p2, p3, hi[(e >> 1) + 1]);
           }
-          tmem_st_32x32b_x32(tSx + h * 32, hi);
-          tmem_st_32x32b_x32(tSx + 64 + h * 32, lo);
+          tmem_st_32x32b_x16(tSx + x * 32 + h * 16, hi);
+          tmem_st_32x32b_x16(tSx + 64 + x * 32 + h * 16, lo);
         }
-        l = fmaf(l, alpha, ls);
-        if (rescale) {  // S_x(i) complete: so is every product on O_x before it
-          const uint32_t tOx = tO + x * 128 + lane_off;
+        l = fmaf(l, alpha, (ls[0] + ls[1]) + (ls[2] + ls[3]));
+        if (rescale) {  // this half of O, once the products so far are in it
+          if (ok) ok = mbar_wait(&o_done[(tc - 1) & 1], ((tc - 1) >> 1) & 1, err, kDevTimeoutAccFull);
+          ok = __all_sync(0xffffffffu, ok);
+          tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            uint32_t o[32];
-            tmem_ld_32x32b_x32(tOx + c * 32, o);
+          for (int c = 4 * x; c < 4 * x + 4; ++c) {
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(tO + lane_off + c * 16, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st_32x32b_x32(tOx + c * 32, o);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st_32x32b_x16(tO + lane_off + c * 16, o);
           }
         }
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(&p_full[x]);
+        mbar_arrive(p_full);
       }
-      // ---- the segment's end in this CTA: join the two lanes, half of the dims
-      // each
-      if (w.n > x) {
-        if (ok) ok = mbar_wait(&o_done[x], ophase & 1, err, kDevTimeoutAccFull);
-        ++ophase;
-      }
-      ml[x * 128 + t] = make_float2(m, l);
-      named_barrier(1, 256);  // both lanes' products are done, m and l in
+      // ---- the segment's end in this CTA
+      // (S of the last tile came after the product two tiles before it, so each
+      // barrier is at most one phase behind)
+      if (ok) ok = mbar_wait(&o_done[(tc - 1) & 1], ((tc - 1) >> 1) & 1, err, kDevTimeoutAccFull);
       ok = __all_sync(0xffffffffu, ok);
+      float* lrow = ml + (tc & 1) * 256;  // (the other buffer may still be read)
+      lrow[x * 128 + t] = l;
+      named_barrier(1, 256);  // every product is done (Q may be overwritten), the sums in
       tc_fence_after();
-      const float2 a0 = ml[t], a1 = ml[128 + t];
-      const float mx = fmaxf(a0.x, a1.x);
-      const float w0 = a0.x == -INFINITY ? 0.0f : exp2f(a0.x - mx);
-      const float w1 = a1.x == -INFINITY ? 0.0f : exp2f(a1.x - mx);
-      const float ls = a0.y * w0 + a1.y * w1;
+      const float lsum = lrow[t] + lrow[128 + t];
+      const int seg = b * per_seq + w.at.hq;
       const bool ends = w.at.tile + w.n == w.at.tiles;
       const bool cut_before = seg == first_seg && first_cut;
       const bool whole = ends && !cut_before;
       float* prow = a.part + ((static_cast<long long>(cta) * 2 + (cut_before ? 0 : 1)) * kTcRows +
                               t) * kPartRow;
       float* dst = whole ? a.out + qrow * 128 : prow + 4;
-      const float scale = whole ? 1.0f / ls : 1.0f;
+      const float scale = whole ? 1.0f / lsum : 1.0f;
       if (!idle) {
 #pragma unroll 1
-        for (int c = 2 * x; c < 2 * x + 2; ++c) {
-          uint32_t o0[32], o1[32];
-          tmem_ld_32x32b_x32(tO + lane_off + c * 32, o0);
-          if (w.n > 1) tmem_ld_32x32b_x32(tO + 128 + lane_off + c * 32, o1);
+        for (int c = 4 * x; c < 4 * x + 4; ++c) {
+          uint32_t o[16];
+          tmem_ld_32x32b_x16(tO + lane_off + c * 16, o);
           tmem_ld_wait();
           if (live) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              float v[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                v[k] = w0 == 0.0f ? 0.0f : __uint_as_float(o0[e + k]) * w0;
-                if (w.n > 1 && w1 != 0.0f) v[k] = fmaf(__uint_as_float(o1[e + k]), w1, v[k]);
-                v[k] *= scale;
-              }
-              *reinterpret_cast<float4*>(dst + c * 32 + e) = make_float4(v[0], v[1], v[2], v[3]);
-            }
+            for (int e = 0; e < 16; e += 4)
+              *reinterpret_cast<float4*>(dst + c * 16 + e) = make_float4(
+                  __uint_as_float(o[e]) * scale, __uint_as_float(o[e + 1]) * scale,
+                  __uint_as_float(o[e + 2]) * scale, __uint_as_float(o[e + 3]) * scale);
           }
         }
       }
       if (!whole && x == 0) {
-        prow[0] = mx;
-        prow[1] = ls;
+        prow[0] = m;
+        prow[1] = lsum;
       }
       tc_fence_before();
       mbar_arrive(o_free);
