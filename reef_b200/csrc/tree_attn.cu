@@ -33,12 +33,13 @@
 //
 // More rows, tree_tc_kernel: tcgen05 with a tile of 128 query rows, bound by
 // the exponentials and conversions of the softmax warps and the tensor pipe (S in
-// int8, P'.V twice in f16).  Scores go into two TMEM tiles in turn, so that the
-// next are there when the softmax of one ends; two warpgroups share a tile, a
-// thread holding half of a query row's 128 scores (a whole row spills); P'
-// overwrites the scores (its heads in the first 64 columns, the rests in the
-// last) and the product reads it there.  Another warpgroup turns V's codes into
-// f16, [key][dim] as they stand: the product takes B with the dims contiguous.
+// int8, P'.V twice in f16).  Scores go into three TMEM tiles in turn, so that the
+// next are there before the softmax of one begins; two warpgroups share a tile, a
+// thread holding half of a query row's 128 scores and taking in the next tile's
+// while it exponentiates these; P' overwrites the scores (its heads in the first
+// 64 columns, the rests in the last) and the product reads it there.  Another
+// warpgroup turns V's codes into f16, [key][dim] as they stand: the product takes
+// B with the dims contiguous.
 #include "attn_mma.cuh"
 #include "common.cuh"
 #include "ops.h"
@@ -112,6 +113,42 @@ __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
 __device__ __forceinline__ uint32_t rest_of(float lo, float hi, uint32_t pair) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pair));
   return half2_of(lo - f.x, hi - f.y);
+}
+
+// two f32 in a register pair, and arithmetic on both at once
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float lo, float hi) {
+  f32x2 v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ f32x2 sub2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 // D (16x8 f32) += A (16x16 f16, row) x B (16x8 f16, col)
@@ -583,7 +620,15 @@ __global__ void __launch_bounds__(kTThreads, 2)
 
 // ---- more rows: tcgen05 -----------------------------------------------------------
 
-constexpr int kCThreads = 512;  // control, converter and two softmax warpgroups
+constexpr int kParts = 2;       // softmax warpgroups: parts of a row
+constexpr int kCols = kTileKeys / kParts;  // keys of a row that a thread holds
+constexpr int kSoftmax = 128 * kParts;     // their threads
+constexpr int kCThreads = 256 + kSoftmax;  // and the control and converter warpgroups
+// Registers: 128 a thread at launch; the control warpgroup drops to 64 and the
+// converters to 72, each softmax warpgroup rises to 184.
+constexpr uint32_t kRegsControl = 64, kRegsConvert = 72, kRegsSoftmax = 184;
+static_assert(kRegsControl + kRegsConvert + kParts * kRegsSoftmax <= 65536 / 128,
+              "register split exceeds the launch allocation");
 constexpr int kKStages = 4;     // K tiles in flight (int8, 16 KiB)
 constexpr int kVStages = 3;     // V tiles in flight (the same)
 
@@ -592,12 +637,12 @@ struct CL {  // shared memory layout (bytes from a 1024-aligned base)
   static constexpr int kK = 16384;                        // kKStages x 16 KiB
   static constexpr int kV = kK + kKStages * 16384;        // kVStages x 16 KiB
   static constexpr int kVf = kV + kVStages * 16384;       // 2 x f16 [2 dim halves][128 keys][64] SW128
-  static constexpr int kScales = kVf + 2 * 32768;         // [8 warps][ks, log2 vs, 1 / vs][64]
-  static constexpr int kML = kScales + 8 * 3 * 64 * 4;    // [2 tiles][2 halves][128] maxima, then sums
-  static constexpr int kPar = kML + 2 * 128 * 8;          // int[64]
+  static constexpr int kScales = kVf + 2 * 32768;         // [2 tiles][warps][ks, log2 vs, 1 / vs][kCols]
+  static constexpr int kML = kScales + 2 * kSoftmax / 32 * 3 * kCols * 4;  // [2 tiles][parts][128]
+  static constexpr int kPar = kML + 2 * kSoftmax * 4;         // int[64]
   static constexpr int kPre = kPar + kMaxDrafts * 4;      // int[batch + 1]
   static constexpr int kBars = kPre + (kMaxBatch + 4) * 4;
-  static constexpr int kNumBars = 8 + 2 * kKStages + 2 * kVStages + 4;
+  static constexpr int kNumBars = 11 + 2 * kKStages + 2 * kVStages + 4;
   static constexpr int kTmemSlot = kBars + kNumBars * 8;
   static constexpr int kBytes = kTmemSlot + 16 + 1024;
 };
@@ -615,6 +660,13 @@ __device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t smem_addr) {
   d |= static_cast<uint64_t>(1u) << 46;
   d |= static_cast<uint64_t>(2u) << 61;
   return d;
+}
+
+// a load that stays where it is written (a plain one would sink to its use)
+__device__ __forceinline__ float load_now(const float* p) {
+  float v;
+  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
 }
 
 // A CTA's tiles of one segment.
@@ -641,10 +693,10 @@ __global__ void __launch_bounds__(kCThreads, 1)
   uint64_t* q_full = reinterpret_cast<uint64_t*>(sm + CL::kBars);  // the segment's Q is in
   uint64_t* o_free = q_full + 1;    // its accumulator has been read
   uint64_t* drain = q_full + 2;
-  uint64_t* s_full = q_full + 3;    // [2] S_x done
-  uint64_t* p_full = q_full + 5;    // P' of the next tile is in its S_x
-  uint64_t* o_done = q_full + 6;    // [2] an even / odd tile's product is in O
-  uint64_t* k_full = q_full + 8;
+  uint64_t* p_full = q_full + 3;    // [2] P' of an even / odd tile is in its S_x
+  uint64_t* s_full = q_full + 5;    // [3] S_x done, x = tile mod 3
+  uint64_t* o_done = q_full + 8;    // [3] the tile's product is in O
+  uint64_t* k_full = q_full + 11;
   uint64_t* k_empty = k_full + kKStages;
   uint64_t* v_full = k_empty + kKStages;
   uint64_t* v_empty = v_full + kVStages;
@@ -660,13 +712,15 @@ __global__ void __launch_bounds__(kCThreads, 1)
   if (tid == 0) {
     prefetch_tensormap(&kmap);
     prefetch_tensormap(&vmap);
-    mbar_init(q_full, 256);
-    mbar_init(o_free, 256);
+    mbar_init(q_full, kSoftmax);
+    mbar_init(o_free, kSoftmax);
     mbar_init(drain, 1);
-    mbar_init(p_full, 256);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&o_done[i], 1);
+    for (int i = 0; i < 3; ++i) {
       mbar_init(&s_full[i], 1);
+      mbar_init(&o_done[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&p_full[i], kSoftmax);
       mbar_init(&f_full[i], 4);
       mbar_init(&f_empty[i], 1);
     }
@@ -690,8 +744,8 @@ __global__ void __launch_bounds__(kCThreads, 1)
   count_tiles<kCThreads>(a, pre, par);
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // columns: S_0 [0, 128), S_1 [128, 256), O [256, 384)
-  const uint32_t tS = tmem, tO = tmem + 256;
+  // columns: S_0 [0, 128), S_1 [128, 256), S_2 [256, 384), O [384, 512)
+  const uint32_t tS = tmem, tO = tmem + 384;
 
   const int per_seq = a.heads_kv * a.qtiles;
   const long long units = static_cast<long long>(pre[a.batch]) * per_seq;
@@ -705,6 +759,7 @@ __global__ void __launch_bounds__(kCThreads, 1)
   if (nunits == 0 && tid == 0) a.meta[cta] = make_int4(-1, 0, -1, 0);
 
   if (warp < 4) {
+    setmaxnreg_dec<kRegsControl>();
     if (warp == 0 && lane < 2) {
       // ---------------- TMA: lane 0 the K ring, lane 1 the V ring ----------------
       const int stages = lane == 0 ? kKStages : kVStages;
@@ -732,7 +787,7 @@ __global__ void __launch_bounds__(kCThreads, 1)
       int kc = 0, tc = 0;  // K tiles multiplied, tiles' products issued
       bool ok = true;
       auto issue_s = [&] {  // the next K tile against Q into its S_x
-        const int s = kc % kKStages, x = kc & 1;
+        const int s = kc % kKStages, x = kc % 3;
         if (!mbar_wait(&k_full[s], (kc / kKStages) & 1, err, kDevTimeoutFull)) return false;
         tc_fence_after();
         const uint32_t sk = smem_u32(sm + CL::kK + s * 16384);
@@ -750,22 +805,24 @@ __global__ void __launch_bounds__(kCThreads, 1)
         ok = mbar_wait(q_full, piece & 1, err, kDevTimeoutFull);
         if (ok) ok = issue_s();
         if (ok && w.n > 1) ok = issue_s();
-        for (int j = 0; j < w.n && ok; ++j) {
-          const int x = tc & 1;
-          ok = mbar_wait(p_full, x, err, kDevTimeoutFull) &&
-               mbar_wait(&f_full[x], (tc >> 1) & 1, err, kDevTimeoutFull) &&
+        for (int j = 0; j < w.n && ok; ++j, ++tc) {
+          // (the S_x of two tiles on is free: the product before this one has been
+          // issued, and the pipe runs in order)
+          if (j + 2 < w.n) ok = issue_s();
+          const int x = tc % 3, f = tc & 1;
+          // (the softmax may be a tile ahead of this thread, hence two p_full)
+          ok = ok && mbar_wait(&p_full[f], (tc >> 1) & 1, err, kDevTimeoutFull) &&
+               mbar_wait(&f_full[f], (tc >> 1) & 1, err, kDevTimeoutFull) &&
                (j > 0 || piece == 0 || mbar_wait(o_free, (piece - 1) & 1, err, kDevTimeoutAccEmpty));
           if (!ok) break;
           tc_fence_after();
-          const uint32_t sv = smem_u32(sm + CL::kVf + x * 32768);
+          const uint32_t sv = smem_u32(sm + CL::kVf + f * 32768);
 #pragma unroll
           for (int kk = 0; kk < 16; ++kk)  // 16 keys a step: 8 columns of the heads, then the rests
             mma_f16_tmem_a(tO, tS + x * 128 + kk * 8, smem_desc_mn_sw128(sv + (kk & 7) * 2048),
                            kIdescO, (j > 0 || kk > 0) ? 1u : 0u);
-          mma_commit(&f_empty[x]);
+          mma_commit(&f_empty[f]);
           mma_commit(&o_done[x]);
-          ++tc;
-          if (j + 2 < w.n) ok = issue_s();
         }
         next_piece(pre, a.batch, per_seq, at, w.n, left);
       }
@@ -773,6 +830,7 @@ __global__ void __launch_bounds__(kCThreads, 1)
       mbar_wait(drain, 0, err, kDevTimeoutDrain);
     }
   } else if (warp < 8) {
+    setmaxnreg_dec<kRegsConvert>();
     // ---------------- V's codes to f16: thread t takes key t of every tile ----------------
     const int t = tid - 128;
     bool ok = true;
@@ -819,12 +877,13 @@ __global__ void __launch_bounds__(kCThreads, 1)
       }
     }
   } else {
-    // ---------------- softmax: thread (x, t) has keys [64x, 64x + 64) of query row t ----------------
+    setmaxnreg_inc<kRegsSoftmax>();
+    // ---------------- softmax: thread (x, t) has keys [kCols x, + kCols) of query row t ----------------
     const int x = (warp - 8) >> 2;
     const int t = (warp & 3) * 32 + lane;  // == TMEM lane
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    float* scw = reinterpret_cast<float*>(sm + CL::kScales) + (warp - 8) * 192;
-    float* ml = reinterpret_cast<float*>(sm + CL::kML);  // [2][2][128]
+    float* scw0 = reinterpret_cast<float*>(sm + CL::kScales) + (warp - 8) * 3 * kCols;  // of 2
+    float* ml = reinterpret_cast<float*>(sm + CL::kML);  // [2][kParts][128]
     const float base = a.sm_scale * kLog2e;
     int tc = 0;  // tiles done
     bool ok = true;
@@ -837,22 +896,29 @@ __global__ void __launch_bounds__(kCThreads, 1)
       const int r = (w.at.hq % a.qtiles) * kTcRows + t;  // query row of the KV head
       const bool live = r < d * a.group;
       const int node = r / a.group;
-      const long long qrow = (static_cast<long long>(b) * a.drafts + node) * a.heads_q +
-                             hkv * a.group + (r - node * a.group);
-      {  // this half of the row of Q
+      // row of q8, q_scale and out
+      const int qrow = (b * a.drafts + node) * a.heads_q + hkv * a.group + (r - node * a.group);
+      const int mine = tid - 256;
+      const bool parent = a.parents != nullptr && mine < d;
+      int up = 0;
+      if (parent) up = a.parents[static_cast<long long>(b) * a.drafts + mine];
+      float amul = 0.0f;
+      {  // this part of the row of Q
         uint8_t* q = sm + CL::kQ + t * 128;
+        uint4 v[8 / kParts];
+        const uint4* src = reinterpret_cast<const uint4*>(a.q8) + static_cast<long long>(qrow) * 8 +
+                           8 / kParts * x;
 #pragma unroll
-        for (int c = 4 * x; c < 4 * x + 4; ++c) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (live) v = __ldg(reinterpret_cast<const uint4*>(a.q8 + qrow * 128) + c);
-          *reinterpret_cast<uint4*>(q + ((c ^ (t & 7)) << 4)) = v;
-        }
+        for (int c = 0; c < 8 / kParts; ++c) v[c] = live ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+        if (live) amul = a.q_scale[qrow] * base;
+        if (parent) par[mine] = up;
+#pragma unroll
+        for (int c = 0; c < 8 / kParts; ++c)
+          *reinterpret_cast<uint4*>(q + (((c + 8 / kParts * x) ^ (t & 7)) << 4)) = v[c];
         fence_proxy_async_smem();
         mbar_arrive(q_full);
       }
-      if (a.parents != nullptr && tid - 256 < d)
-        par[tid - 256] = a.parents[static_cast<long long>(b) * a.drafts + tid - 256];
-      named_barrier(1, 256);
+      named_barrier(1, kSoftmax);
       unsigned long long bits = 0;  // the drafted tokens that this row sees
       if (live) {
         if (a.parents == nullptr) {
@@ -865,77 +931,128 @@ __global__ void __launch_bounds__(kCThreads, 1)
           }
         }
       }
-      const float amul = live ? a.q_scale[qrow] * base : 0.0f;
-      // a warp without a live row (as its partner in the other half) only keeps
+      // a warp without a live row (as its partners in the other parts) only keeps
       // the barriers going
       const bool idle = !__any_sync(0xffffffffu, live);
-      const long long srow = (static_cast<long long>(b) * a.heads_kv + hkv) * a.max_len;
-      auto scales = [&](int i, float2& k, float2& v) {  // this lane's two keys of tile i
-        const int key = (w.at.tile + i) * kTileKeys + 64 * x + 2 * lane;
-        k = v = make_float2(0.f, 0.f);
-        if (i < w.n && key < a.max_len) {
-          k = __ldg(reinterpret_cast<const float2*>(a.k_scale + srow + key));
-          v = __ldg(reinterpret_cast<const float2*>(a.v_scale + srow + key));
+      const int keys0 = w.at.tile * kTileKeys + kCols * x;  // this part's first key
+      const float* ksp = a.k_scale + (static_cast<long long>(b) * a.heads_kv + hkv) * a.max_len;
+      const float* vsp = a.v_scale + (ksp - a.k_scale);
+      float nk[2], nv[2];
+      static_assert(kCols == 64, "a lane stages two keys");
+      // loads this lane's keys of tile i (past the cache's end, where nobody looks,
+      // the last one's: without a branch, the loads run on)
+      auto scales = [&](int i) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int key = min(keys0 + i * kTileKeys + 32 * k + lane, a.max_len - 1);
+          nk[k] = load_now(ksp + key);
+          nv[k] = load_now(vsp + key);
         }
       };
-      float2 nk, nv;
-      scales(0, nk, nv);
-      float m = -INFINITY, l = 0.0f;
-      for (int i = 0; i < w.n; ++i, ++tc) {
-        const uint32_t tSx = tS + (tc & 1) * 128 + lane_off;
-        __syncwarp();  // the warp is done with the last tile's scales
-        reinterpret_cast<float2*>(scw)[lane] = nk;
-        reinterpret_cast<float2*>(scw + 64)[lane] =
-            make_float2(scale_log2(nv.x), scale_log2(nv.y));
-        reinterpret_cast<float2*>(scw + 128)[lane] = make_float2(scale_rcp(nv.x), scale_rcp(nv.y));
+      auto stage = [&](int n) {  // and hands them to the warp, as the n-th tile's
+        float* scw = scw0 + (n & 1) * (kSoftmax / 32 * 3 * kCols);
         __syncwarp();
-        scales(i + 1, nk, nv);
-        if (ok) ok = mbar_wait(&s_full[tc & 1], (tc >> 1) & 1, err, kDevTimeoutAccFull);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          scw[32 * k + lane] = nk[k];
+          scw[kCols + 32 * k + lane] = scale_log2(nv[k]);
+          scw[2 * kCols + 32 * k + lane] = scale_rcp(nv[k]);
+        }
+        __syncwarp();
+      };
+      f32x2 s[kCols / 2];
+      const f32x2 lift = pack2(-12582912.0f, -12582912.0f), am = pack2(amul, amul);
+      float mt0, mt1;
+      // scores of 16 keys (chunk h of tile i, the n-th) in log2 units, with the key's
+      // V scale (small_i2f's steps, two at a time)
+      auto scores = [&](int i, int n, int h, const uint32_t (&acc)[16]) {
+        const float* scw = scw0 + (n & 1) * (kSoftmax / 32 * 3 * kCols);
+        const ulonglong2* k4 = reinterpret_cast<const ulonglong2*>(scw);
+        const ulonglong2* lv4 = reinterpret_cast<const ulonglong2*>(scw + kCols);
+        // (step by step over the chunk, so that its elements cover each other's
+        // latencies)
+        f32x2 v[8], k[8], lv[8];
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const ulonglong2 a2 = k4[h * 4 + (e >> 1)], b2 = lv4[h * 4 + (e >> 1)];
+          k[e] = a2.x;
+          k[e + 1] = a2.y;
+          lv[e] = b2.x;
+          lv[e + 1] = b2.y;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          v[e] = pack2(__uint_as_float(acc[2 * e] + 0x4B400000u),
+                       __uint_as_float(acc[2 * e + 1] + 0x4B400000u));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = add2(v[e], lift);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = mul2(v[e], am);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[h * 8 + e] = fma2(v[e], k[e], lv[e]);
+        const int over = keys0 + i * kTileKeys + 16 * h - len;  // key e: drafted token over + e
+        if (over + 16 > 0) {
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            float f0, f1;
+            unpack2(s[h * 8 + (e >> 1)], f0, f1);
+            const int q = over + e;
+            if (q >= 0 && (q >= kMaxDrafts || ((bits >> q) & 1ull) == 0)) f0 = -INFINITY;
+            if (q >= -1 && (q + 1 >= kMaxDrafts || ((bits >> (q + 1)) & 1ull) == 0)) f1 = -INFINITY;
+            s[h * 8 + (e >> 1)] = pack2(f0, f1);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          float f0, f1, f2, f3;
+          unpack2(s[h * 8 + e], f0, f1);
+          unpack2(s[h * 8 + e + 1], f2, f3);
+          mt0 = max3(mt0, f0, f1);
+          mt1 = max3(mt1, f2, f3);
+        }
+      };
+      auto wait_s = [&](int n) {  // S of the n-th tile
+        if (ok) ok = mbar_wait(&s_full[n % 3], (n / 3) & 1, err, kDevTimeoutAccFull);
         ok = __all_sync(0xffffffffu, ok);  // reconverge before warp-collective tcgen05.ld
         tc_fence_after();
-        uint32_t s[64];
-        float mt = -INFINITY;
-        if (!idle) {
-          tmem_ld_32x32b_x32(tSx + x * 64, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
-          tmem_ld_32x32b_x32(tSx + x * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
+      };
+      scales(0);
+      stage(tc);
+      scales(1);
+      mt0 = mt1 = -INFINITY;
+      wait_s(tc);
+      if (!idle) {
+#pragma unroll
+        for (int h = 0; h < kCols / 16; ++h) {
+          uint32_t acc[16];
+          tmem_ld_32x32b_x16(tS + (tc % 3) * 128 + lane_off + x * kCols + h * 16, acc);
           tmem_ld_wait();
-          // scores in log2 units, with the key's V scale
-          const float4* k4 = reinterpret_cast<const float4*>(scw);
-          const float4* lv4 = reinterpret_cast<const float4*>(scw + 64);
-#pragma unroll
-          for (int e = 0; e < 64; e += 4) {
-            const float4 k = k4[e >> 2], lv = lv4[e >> 2];
-            s[e] = __float_as_uint(fmaf(small_i2f(static_cast<int>(s[e])) * amul, k.x, lv.x));
-            s[e + 1] = __float_as_uint(fmaf(small_i2f(static_cast<int>(s[e + 1])) * amul, k.y, lv.y));
-            s[e + 2] = __float_as_uint(fmaf(small_i2f(static_cast<int>(s[e + 2])) * amul, k.z, lv.z));
-            s[e + 3] = __float_as_uint(fmaf(small_i2f(static_cast<int>(s[e + 3])) * amul, k.w, lv.w));
-          }
-          const int over = (w.at.tile + i) * kTileKeys + 64 * x - len;  // key e: drafted token over + e
-          if (over + 64 > 0) {
-#pragma unroll
-            for (int e = 0; e < 64; ++e) {
-              const int n = over + e;
-              if (n >= 0 && (n >= kMaxDrafts || ((bits >> n) & 1ull) == 0)) s[e] = 0xff800000u;
-            }
-          }
-          float mx[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mx[e] = __uint_as_float(s[e]);
-#pragma unroll
-          for (int e = 4; e < 64; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(s[e]));
-          mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          scores(0, tc, h, acc);
         }
-        // the other half's maximum; after the barrier both halves' scores are in
+      }
+      float m = -INFINITY, l = 0.0f;
+      for (int i = 0; i < w.n; ++i, ++tc) {
+        const uint32_t tSx = tS + (tc % 3) * 128 + lane_off;
+        const uint32_t tSn = tS + ((tc + 1) % 3) * 128 + lane_off + x * kCols;
+        const bool more = i + 1 < w.n;
+        // the other parts' maxima; after the barrier every part's scores are in
         // registers, so P' may overwrite them
-        float* mrow = ml + (tc & 1) * 256;
+        float mt = fmaxf(mt0, mt1);
+        float* mrow = ml + (tc & 1) * kSoftmax;
         mrow[x * 128 + t] = mt;
-        named_barrier(1, 256);
+        named_barrier(1, kSoftmax);
+        if (more) {
+          stage(tc + 1);
+          scales(i + 2);
+          wait_s(tc + 1);
+        }
         if (idle) {
-          mbar_arrive(p_full);
+          mbar_arrive(&p_full[tc & 1]);
           continue;
         }
-        mt = fmaxf(mt, mrow[(x ^ 1) * 128 + t]);
-        // The rescale is warp-collective, so the warp decides (and its partner
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) mt = fmaxf(mt, mrow[k * 128 + t]);
+        // The rescale is warp-collective, so the warp decides (and its partners
         // alike): when any row passes its maximum, every row moves to its own.
         float alpha = 1.0f;
         bool rescale = false;
@@ -946,37 +1063,69 @@ __global__ void __launch_bounds__(kCThreads, 1)
           rescale = i > 0;
         }
         const float nm = kLift - (m == -INFINITY ? 0.0f : m);
-        const float4* rv4 = reinterpret_cast<const float4*>(scw + 128);
-        float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const f32x2 nm2 = pack2(nm, nm);
+        const ulonglong2* rv4 = reinterpret_cast<const ulonglong2*>(
+            scw0 + (tc & 1) * (kSoftmax / 32 * 3 * kCols) + 2 * kCols);
+        f32x2 ls0 = 0, ls1 = 0;  // (0.0f, 0.0f)
+        mt0 = mt1 = -INFINITY;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {  // 32 keys: 16 columns of heads, 16 of rests
-          uint32_t hi[16], lo[16];
+        for (int h = 0; h < kCols / 16; ++h) {  // 16 keys: 8 columns of heads, 8 of rests
+          uint32_t acc[16];
+          if (more) tmem_ld_32x32b_x16(tSn + h * 16, acc);  // the next tile's, meanwhile
+          uint32_t hi[8], lo[8];
+          f32x2 p[8], rv[8];
+          float f0[8], f1[8];
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            const float4 rv = rv4[h * 8 + (e >> 2)];
-            const float p0 = fast_exp2(__uint_as_float(s[h * 32 + e]) + nm);
-            const float p1 = fast_exp2(__uint_as_float(s[h * 32 + e + 1]) + nm);
-            const float p2 = fast_exp2(__uint_as_float(s[h * 32 + e + 2]) + nm);
-            const float p3 = fast_exp2(__uint_as_float(s[h * 32 + e + 3]) + nm);
-            ls[0] = fmaf(p0, rv.x, ls[0]);
-            ls[1] = fmaf(p1, rv.y, ls[1]);
-            ls[2] = fmaf(p2, rv.z, ls[2]);
-            ls[3] = fmaf(p3, rv.w, ls[3]);
-            hi[e >> 1] = half2_of(p0, p1);
-            hi[(e >> 1) + 1] = half2_of(p2, p3);
-            lo[e >> 1] = rest_of(p0, p1, hi[e >> 1]);
-            lo[(e >> 1) + 1] = rest_of(p2, p3, hi[(e >> 1) + 1]);
+          for (int e = 0; e < 8; e += 2) {
+            const ulonglong2 a2 = rv4[h * 4 + (e >> 1)];
+            rv[e] = a2.x;
+            rv[e + 1] = a2.y;
           }
-          tmem_st_32x32b_x16(tSx + x * 32 + h * 16, hi);
-          tmem_st_32x32b_x16(tSx + 64 + x * 32 + h * 16, lo);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) unpack2(add2(s[h * 8 + e], nm2), f0[e], f1[e]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            f0[e] = fast_exp2(f0[e]);
+            f1[e] = fast_exp2(f1[e]);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            hi[e] = half2_of(f0[e], f1[e]);
+            p[e] = pack2(f0[e], f1[e]);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            ls0 = fma2(p[e], rv[e], ls0);
+            ls1 = fma2(p[e + 1], rv[e + 1], ls1);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+            p[e] = sub2(p[e], pack2(f.x, f.y));
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            unpack2(p[e], f0[e], f1[e]);
+            lo[e] = half2_of(f0[e], f1[e]);
+          }
+          tmem_st_32x32b_x8(tSx + x * (kCols / 2) + h * 8, hi);
+          tmem_st_32x32b_x8(tSx + 64 + x * (kCols / 2) + h * 8, lo);
+          if (more) {
+            tmem_ld_wait();
+            scores(i + 1, tc + 1, h, acc);
+          }
         }
-        l = fmaf(l, alpha, (ls[0] + ls[1]) + (ls[2] + ls[3]));
-        if (rescale) {  // this half of O, once the products so far are in it
-          if (ok) ok = mbar_wait(&o_done[(tc - 1) & 1], ((tc - 1) >> 1) & 1, err, kDevTimeoutAccFull);
+        {
+          float f0, f1;
+          unpack2(add2(ls0, ls1), f0, f1);
+          l = fmaf(l, alpha, f0 + f1);
+        }
+        if (rescale) {  // this part of O, once the products so far are in it
+          if (ok) ok = mbar_wait(&o_done[(tc - 1) % 3], ((tc - 1) / 3) & 1, err, kDevTimeoutAccFull);
           ok = __all_sync(0xffffffffu, ok);
           tc_fence_after();
 #pragma unroll 1
-          for (int c = 4 * x; c < 4 * x + 4; ++c) {
+          for (int c = 8 / kParts * x; c < 8 / kParts * (x + 1); ++c) {
             uint32_t o[16];
             tmem_ld_32x32b_x16(tO + lane_off + c * 16, o);
             tmem_ld_wait();
@@ -987,50 +1136,67 @@ __global__ void __launch_bounds__(kCThreads, 1)
         }
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(p_full);
+        mbar_arrive(&p_full[tc & 1]);
       }
       // ---- the segment's end in this CTA
-      // (S of the last tile came after the product two tiles before it, so each
-      // barrier is at most one phase behind)
-      if (ok) ok = mbar_wait(&o_done[(tc - 1) & 1], ((tc - 1) >> 1) & 1, err, kDevTimeoutAccFull);
+      // (S of the last tile came after the product three tiles before it, so no
+      // barrier is more than a phase behind)
+      if (ok) ok = mbar_wait(&o_done[(tc - 1) % 3], ((tc - 1) / 3) & 1, err, kDevTimeoutAccFull);
       ok = __all_sync(0xffffffffu, ok);
-      float* lrow = ml + (tc & 1) * 256;  // (the other buffer may still be read)
+      float* lrow = ml + (tc & 1) * kSoftmax;  // (the other buffer may still be read)
       lrow[x * 128 + t] = l;
-      named_barrier(1, 256);  // every product is done (Q may be overwritten), the sums in
+      named_barrier(1, kSoftmax);  // every product is done (Q is free), the sums in
       tc_fence_after();
-      const float lsum = lrow[t] + lrow[128 + t];
+      float lsum = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kParts; ++k) lsum += lrow[k * 128 + t];
       const int seg = b * per_seq + w.at.hq;
       const bool ends = w.at.tile + w.n == w.at.tiles;
       const bool cut_before = seg == first_seg && first_cut;
       const bool whole = ends && !cut_before;
-      float* prow = a.part + ((static_cast<long long>(cta) * 2 + (cut_before ? 0 : 1)) * kTcRows +
-                              t) * kPartRow;
-      float* dst = whole ? a.out + qrow * 128 : prow + 4;
-      const float scale = whole ? 1.0f / lsum : 1.0f;
+      // 16 columns at a time through this warp's part of Q's buffer, so that four
+      // lanes write 64 bytes of one row
+      float* part = a.part + (static_cast<long long>(cta) * 2 + (cut_before ? 0 : 1)) * kTcRows *
+                                 kPartRow;
+      float4* stg = reinterpret_cast<float4*>(sm + CL::kQ + (warp - 8) * 2048);  // [32 rows][4]
       if (!idle) {
+        const float scale = whole ? 1.0f / lsum : 1.0f;
+        const int home = live ? (whole ? qrow : t) : -1;  // row of out or of the partial
 #pragma unroll 1
-        for (int c = 4 * x; c < 4 * x + 4; ++c) {
+        for (int c = 8 / kParts * x; c < 8 / kParts * (x + 1); ++c) {
           uint32_t o[16];
           tmem_ld_32x32b_x16(tO + lane_off + c * 16, o);
           tmem_ld_wait();
-          if (live) {
+          __syncwarp();
 #pragma unroll
-            for (int e = 0; e < 16; e += 4)
-              *reinterpret_cast<float4*>(dst + c * 16 + e) = make_float4(
-                  __uint_as_float(o[e]) * scale, __uint_as_float(o[e + 1]) * scale,
-                  __uint_as_float(o[e + 2]) * scale, __uint_as_float(o[e + 3]) * scale);
+          for (int e = 0; e < 4; ++e)
+            stg[lane * 4 + (e ^ ((lane >> 1) & 3))] = make_float4(
+                __uint_as_float(o[4 * e]) * scale, __uint_as_float(o[4 * e + 1]) * scale,
+                __uint_as_float(o[4 * e + 2]) * scale, __uint_as_float(o[4 * e + 3]) * scale);
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int row = 8 * k + (lane >> 2), e = lane & 3;
+            const int to = __shfl_sync(0xffffffffu, home, row);
+            const float4 v = stg[row * 4 + (e ^ ((row >> 1) & 3))];
+            if (to >= 0) {
+              float* dst = whole ? a.out + static_cast<long long>(to) * 128
+                                 : part + static_cast<long long>(to) * kPartRow + 4;
+              *reinterpret_cast<float4*>(dst + c * 16 + 4 * e) = v;
+            }
           }
         }
       }
       if (!whole && x == 0) {
-        prow[0] = m;
-        prow[1] = lsum;
+        part[t * kPartRow] = m;
+        part[t * kPartRow + 1] = lsum;
       }
       tc_fence_before();
       mbar_arrive(o_free);
-      if (left == w.n && tid == 256)
+      if (left == w.n && mine == 0)
         a.meta[cta] = make_int4(first_seg, first_cut ? 1 : 0, seg, ends ? 0 : 1);
       next_piece(pre, a.batch, per_seq, at, w.n, left);
+      named_barrier(1, kSoftmax);  // Q's buffer is free again
     }
   }
   tc_fence_before();
