@@ -28,12 +28,15 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return t.data_ptr()
 
 
-def _take(t: torch.Tensor | None, name: str, dtype, shape, device) -> int | None:
+def _take(t: torch.Tensor | None, name: str, dtype, shape, device, other=None) -> int | None:
     """The address of an argument that must be a contiguous CUDA tensor of
-    this type and shape on this device (None passes as NULL)."""
+    this type (or the other) and shape on this device (None passes as NULL)."""
     if t is None:
         return None
-    if t.dtype is not dtype and (not isinstance(dtype, tuple) or t.dtype not in dtype):
+    if t.dtype is dtype and t.shape == shape and t.device == device and t.is_cuda and \
+            t.is_contiguous():
+        return t.data_ptr()
+    if t.dtype is not dtype and t.dtype is not other:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
@@ -45,11 +48,14 @@ def _take(t: torch.Tensor | None, name: str, dtype, shape, device) -> int | None
 def _call_on(device: torch.device, name: str, *args) -> None:
     """An entry point on `device` and its current stream (the last argument),
     whichever device is current."""
+    # (the raw handle: torch.cuda.current_stream() makes a Stream object, 3 us of
+    # a call that takes 4)
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
     if device.index == torch.cuda.current_device():
-        _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+        _lib.call(name, *args, stream)
     else:
         with torch.cuda.device(device):
-            _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+            _lib.call(name, *args, stream)
 
 
 def kpad(n: int) -> int:
@@ -109,8 +115,8 @@ def sample_f32(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor 
             _take(temperature, "temperature", f32, one, dev),
             _take(top_k, "top_k", torch.int32, one, dev), _take(top_p, "top_p", f32, one, dev),
             _take(min_p, "min_p", f32, one, dev), _take(u, "u", f32, one, dev))
-    index = torch.empty(one, dtype=torch.int32, device=dev)
-    prob = torch.empty(one, dtype=f32, device=dev)
+    prob = torch.empty_like(u)
+    index = torch.empty_like(u, dtype=torch.int32)
     _call_on(dev, "reef_b200_sample_f32", rows, n, *args, index.data_ptr(), prob.data_ptr())
     return index, prob
 
@@ -277,16 +283,14 @@ def add_rmsnorm_quant(x: torch.Tensor, residual: torch.Tensor, gain: torch.Tenso
     args = (_take(x, "x", f32, (rows, width), dev),
             _take(residual, "residual", f32, (rows, width), dev),
             _take(gain, "gain", f32, (width,), dev), _take(h, "h", f32, (rows, width), dev))
-    x_q = torch.empty((rows, width), dtype=torch.int8, device=dev)
-    xs = torch.empty((rows,), dtype=f32, device=dev)
+    x_q = torch.empty_like(x, dtype=torch.int8)
+    xs = x.new_empty(rows)
     _call_on(dev, "reef_b200_add_rmsnorm_quant", rows, width, eps, *args, x_q.data_ptr(),
              xs.data_ptr())
     return h, x_q, xs
 
 
 # ---- drafted tokens over the int8 KV cache ---------------------------------------
-
-_IDS = (torch.int32, torch.uint32)
 
 
 def tree_attn_i8(q8: torch.Tensor, q_scale: torch.Tensor, k_cache: torch.Tensor,
@@ -334,10 +338,11 @@ def tree_accept(tokens: torch.Tensor, chosen: torch.Tensor, parents: torch.Tenso
     dev, i32 = tokens.device, torch.int32
     args = (_take(draft_lens, "draft_lens", i32, (b,), dev),
             _take(parents, "parents", i32, (b, t), dev),
-            _take(tokens, "tokens", _IDS, (b, t), dev), _take(chosen, "chosen", _IDS, (b, t), dev))
-    path = torch.empty((b, t), dtype=i32, device=dev)
-    accepted = torch.empty((b,), dtype=i32, device=dev)
-    following = torch.empty((b,), dtype=chosen.dtype, device=dev)
+            _take(tokens, "tokens", i32, (b, t), dev, torch.uint32),
+            _take(chosen, "chosen", i32, (b, t), dev, torch.uint32))
+    path = torch.empty_like(tokens, dtype=i32)
+    accepted = path.new_empty(b)
+    following = chosen.new_empty(b)
     _call_on(dev, "reef_b200_tree_accept", b, t, *args, path.data_ptr(), accepted.data_ptr(),
              following.data_ptr())
     return path, accepted, following
@@ -360,7 +365,7 @@ def kv_compact_i8(k_cache: torch.Tensor, k_scale: torch.Tensor, v_cache: torch.T
             _take(k_scale, "k_scale", f32, cache[:-1], dev),
             _take(v_cache, "v_cache", i8, cache, dev),
             _take(v_scale, "v_scale", f32, cache[:-1], dev))
-    new_lens = torch.empty((b,), dtype=i32, device=dev)
+    new_lens = torch.empty_like(lens)
     _call_on(dev, "reef_b200_kv_compact_i8", n, b, hkv, d, max_len, t, *args,
              new_lens.data_ptr())
     return new_lens
