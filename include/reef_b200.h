@@ -676,6 +676,23 @@ int reef_b200_llama_decode_forward(const reef_b200_llama_layer* layer, const flo
                                    void* workspace, size_t workspace_bytes,
                                    reef_b200_stream_t stream);
 
+/* The decode step on drafted tokens (no counterpart in reef): every sequence
+ * (layer->batch of them) runs `drafts` new tokens at once, batch * drafts <= 128.
+ * x / y [batch * drafts][hidden] fp32, row b * drafts + t.  The tokens' keys and
+ * values go to cache rows lens[b] + t, rotated for position lens[b] + depth (a
+ * root's depth is 0), and each token attends as in reef_b200_tree_attn_i8, whose
+ * lens, draft_lens and parents these are; its cache and scale alignment holds too
+ * (max_len a multiple of 4).  Rows of y past a sequence's drafts, and of a
+ * sequence that does not fit the cache (0x201), are unspecified. */
+size_t reef_b200_llama_verify_workspace_bytes(const reef_b200_llama_layer* layer, size_t drafts,
+                                              size_t max_len);
+int reef_b200_llama_verify_forward(const reef_b200_llama_layer* layer, size_t drafts,
+                                   const float* x, float* y, const int32_t* lens,
+                                   const int32_t* draft_lens, const int32_t* parents,
+                                   int8_t* k_cache, float* k_scale, int8_t* v_cache,
+                                   float* v_scale, size_t max_len, void* workspace,
+                                   size_t workspace_bytes, reef_b200_stream_t stream);
+
 /* reef's GPT-Neo W8A8 block, Block<float>::forward (operator/block.hpp:97-108)
  * on `seq` positions of an empty cache (BASELINE configs 1 and 2): LayerNorm,
  * q/k/v W8A8 projections (no bias), reef's float head per head (unscaled,

@@ -101,6 +101,8 @@ SIGNATURES = {
     "reef_b200_llama_layer_forward_events": ([_p, _p, _p, _p, _sz, _p, _p], _i),
     "reef_b200_llama_decode_workspace_bytes": ([_p, _sz], _sz),
     "reef_b200_llama_decode_forward": ([_p] * 8 + [_sz, _p, _sz, _p], _i),
+    "reef_b200_llama_verify_workspace_bytes": ([_p, _sz, _sz], _sz),
+    "reef_b200_llama_verify_forward": ([_p, _sz] + [_p] * 9 + [_sz, _p, _sz, _p], _i),
     "reef_b200_gptneo_block_workspace_bytes": ([_p], _sz),
     "reef_b200_gptneo_block_forward": ([_p, _p, _p, _p, _sz, _p], _i),
 }

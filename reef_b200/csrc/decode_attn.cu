@@ -570,9 +570,19 @@ int launch_decode(const CUtensorMap& km, const CUtensorMap& vm, DecodeArgs& a, c
 // (`splits` of them, B * (Hq + 2 Hkv) * 128 apart) that this kernel sums and
 // dequantises itself with the W8A8 epilogue (linear.hpp:125-127: float(sum) *
 // (x_scale[b] * w_scale[n])), the values a separate reduce would have stored.
-template <bool kPartials>
+// kDrafts: row i is drafted token t = i % drafts of sequence i / drafts; its k
+// and v go to cache row lens_in[b] + t, its RoPE position is lens_in[b] + its
+// depth in the tree (parents as in tree_attn.cu); lens is not written.
+struct DraftRows {
+  int drafts;
+  const int* lens_in;     // [sequences]
+  const int* draft_lens;  // [sequences] or null
+  const int* parents;     // [sequences][drafts] or null
+};
+
+template <bool kPartials, bool kDrafts>
 __global__ void decode_rope_append_kernel(int batch, int hq, int hkv, int max_len, float base,
-                                          const int* __restrict__ positions,
+                                          const int* __restrict__ positions, DraftRows dr,
                                           const float* __restrict__ qkv,
                                           const int32_t* __restrict__ part, int splits,
                                           const float* __restrict__ xs,
@@ -588,12 +598,38 @@ __global__ void decode_rope_append_kernel(int batch, int hq, int hkv, int max_le
   const int heads = hq + 2 * hkv;
   if (gw >= batch * heads) return;
   const int b = gw / heads, hh = gw % heads;
-  const int pos = positions[b];
-  if (pos < 0 || pos >= max_len) {
-    if (lane == 0 && hh == 0) record_error(err, kDevBadPosition);
-    return;
+  int seq = b, pos, row;  // the cache's sequence, the RoPE position and the cache row
+  if constexpr (kDrafts) {
+    seq = b / dr.drafts;
+    const int t = b - seq * dr.drafts, len = dr.lens_in[seq];
+    const int d = dr.draft_lens == nullptr ? dr.drafts : min(dr.draft_lens[seq], dr.drafts);
+    if (t >= d) return;
+    if (len < 0 || len > max_len || d > max_len - len) {
+      if (lane == 0 && hh == 0) record_error(err, kDevBadPosition);
+      return;
+    }
+    int depth = t;
+    if (dr.parents != nullptr) {  // lane l holds the parents of l and l + 32
+      const int* par = dr.parents + static_cast<long long>(seq) * dr.drafts;
+      const int p0 = lane < d ? par[lane] : -1, p1 = lane + 32 < d ? par[lane + 32] : -1;
+      depth = 0;
+      for (int i = t;; ++depth) {  // strictly downwards: it ends
+        const int a0 = __shfl_sync(0xffffffffu, p0, i & 31), a1 = __shfl_sync(0xffffffffu, p1, i & 31);
+        const int up = i < 32 ? a0 : a1;
+        if (up < 0 || up >= i) break;
+        i = up;
+      }
+    }
+    pos = len + depth;
+    row = len + t;
+  } else {
+    pos = row = positions[b];
+    if (pos < 0 || pos >= max_len) {
+      if (lane == 0 && hh == 0) record_error(err, kDevBadPosition);
+      return;
+    }
+    if (hh == 0 && lane == 0) lens[b] = pos + 1;
   }
-  if (hh == 0 && lane == 0) lens[b] = pos + 1;
   float v[4];
   if constexpr (kPartials) {
     const long long stride = static_cast<long long>(batch) * heads * 128;
@@ -656,9 +692,9 @@ __global__ void decode_rope_append_kernel(int batch, int hq, int hkv, int max_le
   } else {
     const bool is_k = hh < hq + hkv;
     const int kh = is_k ? hh - hq : hh - hq - hkv;
-    const long long row = (static_cast<long long>(b) * hkv + kh) * max_len + pos;
-    dst = (is_k ? k_cache : v_cache) + row * 128;
-    if (lane == 0) (is_k ? k_scale : v_scale)[row] = scale;
+    const long long at = (static_cast<long long>(seq) * hkv + kh) * max_len + row;
+    dst = (is_k ? k_cache : v_cache) + at * 128;
+    if (lane == 0) (is_k ? k_scale : v_scale)[at] = scale;
   }
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
@@ -679,11 +715,28 @@ int decode_rope_append_partials(int batch, int heads_q, int heads_kv, int max_le
     return kErrInvalid;
   const long long warps = static_cast<long long>(batch) * (heads_q + 2 * heads_kv);
   // two warps per block, so the (sequence, head) rows spread over every SM
-  return launch_k(decode_rope_append_kernel<true>,
+  return launch_k(decode_rope_append_kernel<true, false>,
                   dim3(static_cast<unsigned>((warps * 32 + 63) / 64)), dim3(64), 0, stream,
-                  batch, heads_q, heads_kv, max_len, rope_base, positions,
+                  batch, heads_q, heads_kv, max_len, rope_base, positions, DraftRows{},
                   static_cast<const float*>(nullptr), part, splits, x_scale, w_scale, q8, q_scale,
                   k_cache, k_scale, v_cache, v_scale, lens, device_error_ptr());
+}
+
+int draft_rope_append_partials(int batch, int drafts, int heads_q, int heads_kv, int max_len,
+                               float rope_base, const int* lens, const int* draft_lens,
+                               const int* parents, const int32_t* part, int splits,
+                               const float* x_scale, const float* w_scale, int8_t* q8,
+                               float* q_scale, int8_t* k_cache, float* k_scale, int8_t* v_cache,
+                               float* v_scale, cudaStream_t stream) {
+  const int rows = batch * drafts;
+  const long long warps = static_cast<long long>(rows) * (heads_q + 2 * heads_kv);
+  return launch_k(decode_rope_append_kernel<true, true>,
+                  dim3(static_cast<unsigned>((warps * 32 + 63) / 64)), dim3(64), 0, stream, rows,
+                  heads_q, heads_kv, max_len, rope_base, static_cast<const int*>(nullptr),
+                  DraftRows{drafts, lens, draft_lens, parents},
+                  static_cast<const float*>(nullptr), part, splits, x_scale, w_scale, q8, q_scale,
+                  k_cache, k_scale, v_cache, v_scale, static_cast<int*>(nullptr),
+                  device_error_ptr());
 }
 
 

@@ -17,6 +17,7 @@
 #include "../../include/reef_b200.h"
 
 #include "comm.h"
+#include "layer.h"
 #include "ops.h"
 
 #include <algorithm>
@@ -1232,27 +1233,20 @@ static int llama_forward(const reef_b200_llama_layer* L, const float* x, float* 
 
 // ---- Llama-shape decode step ---------------------------------------------------------
 
-size_t reef_b200_llama_decode_workspace_bytes(const reef_b200_llama_layer* L, size_t max_len) {
+}  // extern "C"
+
+namespace reef {
+
+size_t decode_run_bytes(const reef_b200_llama_layer* L, size_t max_len) {
   if (decode_check(L, max_len) != REEF_B200_OK || check_device() != kOk) return 0;
   DecodeBufs b;
   return decode_carve(L, max_len, nullptr, &b);
 }
 
-int reef_b200_llama_decode_forward(const reef_b200_llama_layer* L, const float* x, float* y,
-                                   const int32_t* positions, int8_t* k_cache, float* k_scale,
-                                   int8_t* v_cache, float* v_scale, size_t max_len,
-                                   void* workspace, size_t workspace_bytes,
-                                   reef_b200_stream_t stream) {
-  if (int rc = decode_check(L, max_len)) return rc;
-  if (!x || !y || !positions || !k_cache || !k_scale || !v_cache || !v_scale || !workspace)
-    return REEF_B200_ERR_INVALID;
-  if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0 ||
-      (reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) % 16 != 0)
-    return REEF_B200_ERR_ALIGNMENT;
-  if (int rc = check_device()) return rc;
+int decode_run(const reef_b200_llama_layer* L, const float* x, float* y, size_t max_len,
+               void* workspace, size_t workspace_bytes, DecodeHooks& hooks, cudaStream_t st) {
   DecodeBufs b;
   if (decode_carve(L, max_len, workspace, &b) > workspace_bytes) return REEF_B200_ERR_INVALID;
-  cudaStream_t st = S(stream);
   Comm* c = C(L->comm);
   const int B = static_cast<int>(L->batch), H = static_cast<int>(L->hidden),
             hq = static_cast<int>(L->heads_q), hkv = static_cast<int>(L->heads_kv),
@@ -1269,26 +1263,8 @@ int reef_b200_llama_decode_forward(const reef_b200_llama_layer* L, const float* 
   REEF_TRY(rmsnorm_quant(B, H, L->rms_eps, x, L->attn_norm, b.xq, b.xs, st));
   const int s_qkv = skinny_split_count(B, qkv_w, H);
   REEF_TRY(gemm_i8_skinny_partials(B, qkv_w, H, b.xq, L->w_qkv, part, st, L->t_qkv));
-  REEF_TRY(decode_rope_append_partials(B, hq, hkv, static_cast<int>(max_len), L->rope_base,
-                                       positions, part, s_qkv, b.xs, L->s_qkv, b.q8, b.qs,
-                                       k_cache, k_scale, v_cache, v_scale, b.lens, st));
-  DecodeProblem dp{};
-  dp.batch = B;
-  dp.heads_q = hq;
-  dp.heads_kv = hkv;
-  dp.max_len = static_cast<int>(max_len);
-  dp.sm_scale = 0.08838834764831845f;  // 1 / sqrt(128)
-  dp.q8 = b.q8;
-  dp.q_scale = b.qs;
-  dp.k_cache = k_cache;
-  dp.k_scale = k_scale;
-  dp.v_cache = v_cache;
-  dp.v_scale = v_scale;
-  dp.lens = b.lens;
-  dp.positions = positions;
-  dp.partial = b.dpart;
-  dp.out = b.attn;
-  REEF_TRY(decode_attn_i8(dp, st));
+  REEF_TRY(hooks.append(part, s_qkv, b.xs, b.q8, b.qs, b.lens, st));
+  REEF_TRY(hooks.attend(b.q8, b.qs, b.lens, b.dpart, b.attn, st));
   // o-proj with the residual, then the MLP's pre-norm: without a peer to
   // share the rows with, the o-proj's split-K sum, the residual and RMSNorm +
   // quant run as one kernel; the gate/up input scales go to xs2
@@ -1323,6 +1299,73 @@ int reef_b200_llama_decode_forward(const reef_b200_llama_layer* L, const float* 
                            b.row_max, b.acc, b.partial, y, st, L->t_down));
   }
   return REEF_B200_OK;
+}
+
+}  // namespace reef
+
+extern "C" {
+
+size_t reef_b200_llama_decode_workspace_bytes(const reef_b200_llama_layer* L, size_t max_len) {
+  return decode_run_bytes(L, max_len);
+}
+
+int reef_b200_llama_decode_forward(const reef_b200_llama_layer* L, const float* x, float* y,
+                                   const int32_t* positions, int8_t* k_cache, float* k_scale,
+                                   int8_t* v_cache, float* v_scale, size_t max_len,
+                                   void* workspace, size_t workspace_bytes,
+                                   reef_b200_stream_t stream) {
+  if (int rc = decode_check(L, max_len)) return rc;
+  if (!x || !y || !positions || !k_cache || !k_scale || !v_cache || !v_scale || !workspace)
+    return REEF_B200_ERR_INVALID;
+  if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0 ||
+      (reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) % 16 != 0)
+    return REEF_B200_ERR_ALIGNMENT;
+  if (int rc = check_device()) return rc;
+  // one new token per sequence, at positions[b]
+  struct Decode final : DecodeHooks {
+    const reef_b200_llama_layer* L;
+    const int32_t* positions;
+    int8_t* kc;
+    float* ks;
+    int8_t* vc;
+    float* vs;
+    int max_len;
+    int append(const int32_t* part, int splits, const float* xs, int8_t* q8, float* qs, int* lens,
+               cudaStream_t st) override {
+      return decode_rope_append_partials(
+          static_cast<int>(L->batch), static_cast<int>(L->heads_q), static_cast<int>(L->heads_kv),
+          max_len, L->rope_base, positions, part, splits, xs, L->s_qkv, q8, qs, kc, ks, vc, vs,
+          lens, st);
+    }
+    int attend(const int8_t* q8, const float* qs, const int* lens, float* partial, float* out,
+               cudaStream_t st) override {
+      DecodeProblem dp{};
+      dp.batch = static_cast<int>(L->batch);
+      dp.heads_q = static_cast<int>(L->heads_q);
+      dp.heads_kv = static_cast<int>(L->heads_kv);
+      dp.max_len = max_len;
+      dp.sm_scale = 0.08838834764831845f;  // 1 / sqrt(128)
+      dp.q8 = q8;
+      dp.q_scale = qs;
+      dp.k_cache = kc;
+      dp.k_scale = ks;
+      dp.v_cache = vc;
+      dp.v_scale = vs;
+      dp.lens = lens;
+      dp.positions = positions;
+      dp.partial = partial;
+      dp.out = out;
+      return decode_attn_i8(dp, st);
+    }
+  } hooks;
+  hooks.L = L;
+  hooks.positions = positions;
+  hooks.kc = k_cache;
+  hooks.ks = k_scale;
+  hooks.vc = v_cache;
+  hooks.vs = v_scale;
+  hooks.max_len = static_cast<int>(max_len);
+  return decode_run(L, x, y, max_len, workspace, workspace_bytes, hooks, S(stream));
 }
 
 // ---- GPT-Neo W8A8 block ---------------------------------------------------------------

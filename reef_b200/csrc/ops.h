@@ -431,6 +431,15 @@ int decode_rope_append_partials(int batch, int heads_q, int heads_kv, int max_le
                                 int8_t* q8, float* q_scale, int8_t* k_cache, float* k_scale,
                                 int8_t* v_cache, float* v_scale, int* lens, cudaStream_t stream);
 int decode_attn_i8(const DecodeProblem& p, cudaStream_t stream);
+// The same for drafted tokens: row b * drafts + t of the projection is drafted
+// token t of sequence b, appended at cache row lens[b] + t and rotated for
+// position lens[b] + its depth in the tree.  Rows past draft_lens are left out.
+int draft_rope_append_partials(int batch, int drafts, int heads_q, int heads_kv, int max_len,
+                               float rope_base, const int* lens, const int* draft_lens,
+                               const int* parents, const int32_t* part, int splits,
+                               const float* x_scale, const float* w_scale, int8_t* q8,
+                               float* q_scale, int8_t* k_cache, float* k_scale, int8_t* v_cache,
+                               float* v_scale, cudaStream_t stream);
 
 // tree_attn.cu -- int8 attention of drafted tokens over the same cache
 constexpr int kMaxTreeBatch = 2048;

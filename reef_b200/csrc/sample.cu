@@ -31,7 +31,8 @@
 // most n and weigh less), so the list reaches down to half of that.  top-k lists
 // what lies above a bound instead: the k-th largest of the maxima of groups of
 // eight logits, from a histogram that the first pass makes on the way.  A
-// list short enough goes to one CTA, which ends the row alone.
+// list short enough goes to one CTA, which ends the row alone; with one element
+// to a thread (256 of them) by comparing each with each, in one go.
 // The kept set is always "x > value, or x = value and index <= index": a
 // histogram over the listed range (counts or masses, 1024 equal steps, summed
 // over the cluster through distributed shared memory) gives the step in which
@@ -60,7 +61,7 @@ constexpr int kMaxCluster = 8;
 constexpr int kSlice = 16384;   // logits per CTA: two CTAs fit on an SM
 constexpr int kList = 1016;     // of a warp's run (1024 at that slice) that are listed
 constexpr int kGather = 1024;   // of a row that one CTA takes over
-constexpr int kNear = 256;      // elements of one step, over the cluster
+constexpr int kNear = 256;      // elements of one step, over the cluster (two threads each)
 constexpr int kMaxResident = 168 * 1024;      // bytes of logits a CTA keeps
 constexpr double kOne = 8796093022208.0;      // 2^43, the weight 1
 constexpr uint32_t kKeyNegInf = 0x007fffffu;  // key_of(-inf)
@@ -98,7 +99,13 @@ struct alignas(16) Shared {
       int index[kGather];
     } all;
   };
-  uint16_t list[kWarps][kList];  // elements of a warp's run, in index order
+  union {
+    uint16_t list[kWarps][kList];  // elements of a warp's run, in index order
+    struct {                       // or the odd half of a count
+      u64 ahead[kNear];
+      int rank[kNear];
+    } sub;
+  };
   int listed[kWarps];
   int near_n[kMaxCluster];
   u64 slot[2][2][kMaxCluster];   // two values of every CTA
@@ -363,7 +370,7 @@ __device__ __noinline__ bool build(Ctx& ctx, const Row& row, float least, u64* m
 // (false in the others: they are done), else in every CTA.
 __device__ __noinline__ bool gather(Ctx& c, const Row& r, int count) {
   Shared* s = c.s;
-  if (c.ranks == 1 || count > kGather) {
+  if (count > (c.ranks == 1 ? kNear : kGather)) {
     c.mode = kListed;
     return true;
   }
@@ -629,6 +636,68 @@ __device__ __noinline__ void select_radix(Ctx& c, const Row& r, Cut* cut_io, flo
   *cut_io = Cut{value, static_cast<int>(c.s->found)};
 }
 
+// The rest of a row whose candidates (all that any filter may keep, in index
+// order) are one to a thread: the ranks and the masses ahead of each by comparing
+// with every other, then the draw by a prefix sum.  k: 0 is off; keeps_min(x)
+// says what min-p keeps.
+template <typename KeepsMin>
+__device__ __forceinline__ void finish_few(const Ctx& c, const Row& r, int k, float p,
+                                           KeepsMin keeps_min, float u, uint32_t* index,
+                                           float* prob) {
+  Shared* s = c.s;
+  // two threads to an element, for the even and the odd ones of the others
+  const int e = c.tid % kNear, half = c.tid / kNear;
+  const bool have = e < c.gathered;
+  const float x = have ? s->all.x[e] : 0.0f;
+  const int at = have ? s->all.index[e] : 0;
+  u64 w = have ? r.fixed(x) : 0ull;
+  if (half == 0) s->near.w[e] = w;
+  __syncthreads();
+  // the elements ahead in the order: how many, and their mass (they come before
+  // this one, so top-k keeps them if it keeps this one)
+  int rank = 0;
+  u64 ahead = 0;
+  if (have) {
+#pragma unroll 4
+    for (int j = half; j < c.gathered; j += kThreads / kNear) {
+      const float y = s->all.x[j];
+      const bool before = y > x || (y == x && j < e);
+      rank += before;
+      ahead += before ? s->near.w[j] : 0ull;
+    }
+  }
+  if (half != 0) {
+    s->sub.ahead[e] = ahead;
+    s->sub.rank[e] = rank;
+    w = 0;
+  }
+  __syncthreads();
+  if (half == 0) {
+    ahead += s->sub.ahead[e];
+    rank += s->sub.rank[e];
+  }
+  if (k > 0 && rank >= k) w = 0;
+  const u64 mass = block_sum(c, w);
+  // kept: mass ahead < p * total, as integers
+  if (p < 1.0f && rank > 0 &&
+      static_cast<double>(ahead) >= ceil(static_cast<double>(p) * static_cast<double>(mass)))
+    w = 0;
+  if (w != 0 && !keeps_min(x)) w = 0;
+  __syncthreads();  // (s->warp has been read)
+  const u64 all = block_sum(c, w);
+  u64 target = u > 0.0f ? static_cast<u64>(fmin(static_cast<double>(u), 1.0) *
+                                           static_cast<double>(all))
+                        : 0ull;
+  target = target < all ? target : all - 1;
+  u64 run = warp_prefix(w, c.lane) - w;
+  for (int i = 0; i < c.warp; ++i) run += s->warp[i];
+  if (run <= target && target < run + w) {  // (w is 0 in the second halves)
+    *index = static_cast<uint32_t>(at);
+    if (prob != nullptr)
+      *prob = static_cast<float>(r.weight(x) * kOne / static_cast<double>(all));
+  }
+}
+
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
   extern __shared__ __align__(16) uint8_t raw[];
   Ctx c{cg::this_cluster()};
@@ -725,6 +794,22 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
   r.least = r.below_top(-60.0);
   r.exp2_of = s->exp2_of;
 
+  // min-p in float but next to the border, in double there
+  const double least = mp > 0.0f ? fmin(static_cast<double>(mp), 1.0) : 0.0;
+  float sure = INFINITY, out = -INFINITY;  // x from `sure` up stays, below `out` not
+  if (least > 0.0 && r.plain) {
+    const double x = static_cast<double>(top) + log(least) * static_cast<double>(t);
+    const double slack = 1e-6 * (fabs(x) + fabs(static_cast<double>(top)) + 1e-6);
+    sure = static_cast<float>(x + slack);
+    out = static_cast<float>(x - slack);
+  }
+  auto keeps_min = [&](float x) {
+    return least == 0.0 || x >= sure || (!(x < out) && r.weight(x) >= least);
+  };
+  const float u = a.u[row];
+  uint32_t* const index = a.index + row;
+  float* const prob = a.prob != nullptr ? a.prob + row : nullptr;
+
   // ---- the kept set
   Cut cut{-INFINITY, 0x7fffffff};
   u64 mass = 0;
@@ -747,11 +832,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
       ok = scan_bins(c, 2 * kBins, k, [&](int b) -> u64 { return s->count[b]; }, &bin, &before);
     }
     // k groups have their maximum, so k logits lie, from here up
-    const float least = ok ? floor_of(static_cast<uint32_t>(bin) << 21) : -INFINITY;
-    ok = least > -INFINITY && build<false>(c, r, least, &mass, &slot, &count);
+    const float from = ok ? floor_of(static_cast<uint32_t>(bin) << 21) : -INFINITY;
+    ok = from > -INFINITY && build<false>(c, r, from, &mass, &slot, &count);
     if (ok && !gather(c, r, count)) return;
-    if (!ok || !select_steps<false>(c, r, &cut, least, static_cast<u64>(k)))
-      select_radix<false>(c, r, &cut, least, static_cast<u64>(k));
+    if (c.mode == kGathered && c.gathered <= kNear)
+      return finish_few(c, r, k, p, keeps_min, u, index, prob);
+    if (!ok || !select_steps<false>(c, r, &cut, from, static_cast<u64>(k)))
+      select_radix<false>(c, r, &cut, from, static_cast<u64>(k));
   }
   if (p < 1.0f) {
     bool listed = false;
@@ -766,29 +853,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
     const double want = ceil(static_cast<double>(p) * static_cast<double>(mass));
     const u64 target = want > 1.0 ? static_cast<u64>(want) : 1ull;
     if (target < mass) {
-      float least = cut.value;
+      float from = cut.value;
       if (r.plain)
-        least = fmaxf(least,
-                      r.below_top(log2(0.5 * static_cast<double>(mass - target) / (a.n * kOne))));
-      if (c.mode == kAll || !(least > -INFINITY) || !select_steps<true>(c, r, &cut, least, target))
-        select_radix<true>(c, r, &cut, least, target);
+        from = fmaxf(from,
+                     r.below_top(log2(0.5 * static_cast<double>(mass - target) / (a.n * kOne))));
+      if (c.mode == kAll || !(from > -INFINITY) || !select_steps<true>(c, r, &cut, from, target))
+        select_radix<true>(c, r, &cut, from, target);
     }
-  }
-  // min-p in float but next to the border, in double there
-  const double least = mp > 0.0f ? fmin(static_cast<double>(mp), 1.0) : 0.0;
-  float sure = INFINITY, out = -INFINITY;  // x from `sure` up stays, below `out` not
-  if (least > 0.0 && r.plain) {
-    const double x = static_cast<double>(top) + log(least) * static_cast<double>(t);
-    const double slack = 1e-6 * (fabs(x) + fabs(static_cast<double>(top)) + 1e-6);
-    sure = static_cast<float>(x + slack);
-    out = static_cast<float>(x - slack);
   }
   auto kept = [&](float x, int i) -> u64 {
-    if (!cut.keeps(x, i)) return 0ull;
-    if (least > 0.0 && !(x >= sure)) {
-      if (x < out || !(r.weight(x) >= least)) return 0ull;
-    }
-    return r.fixed(x);
+    return cut.keeps(x, i) && keeps_min(x) ? r.fixed(x) : 0ull;
   };
 
   // ---- the draw
@@ -797,20 +871,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
   if (c.mode == kAll && r.plain && k == 0 && !(p < 1.0f)) {
     if (least > 0.0) {  // what min-p may keep is listed
       if (build<false>(c, r, out, &mass, &slot, &count) && !gather(c, r, count)) return;
+      if (c.mode == kGathered && c.gathered <= kNear)
+        return finish_few(c, r, 0, 1.0f, keeps_min, u, index, prob);
     } else {  // every element counts: s->warp and slot hold their sums
       summed = build<true>(c, r, r.heavy, &all, &slot, &count);
     }
   }
   if (!summed) all = row_sum(c, r, kept, &slot);
-  const float u = a.u[row];
   u64 target = u > 0.0f ? static_cast<u64>(fmin(static_cast<double>(u), 1.0) *
                                            static_cast<double>(all))
                         : 0ull;
   target = target < all ? target : all - 1;
   if (locate(c, r, kept, slot, target, &at, &at_x)) {
-    a.index[row] = static_cast<uint32_t>(at);
-    if (a.prob != nullptr)
-      a.prob[row] = static_cast<float>(r.weight(at_x) * kOne / static_cast<double>(all));
+    *index = static_cast<uint32_t>(at);
+    if (prob != nullptr)
+      *prob = static_cast<float>(r.weight(at_x) * kOne / static_cast<double>(all));
   }
 }
 

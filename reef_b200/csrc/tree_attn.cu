@@ -35,11 +35,10 @@
 // the exponentials and conversions of the softmax warps and the tensor pipe (S in
 // int8, P'.V twice in f16).  Scores go into three TMEM tiles in turn, so that the
 // next are there before the softmax of one begins; two warpgroups share a tile, a
-// thread holding half of a query row's 128 scores and taking in the next tile's
-// while it exponentiates these; P' overwrites the scores (its heads in the first
-// 64 columns, the rests in the last) and the product reads it there.  Another
-// warpgroup turns V's codes into f16, [key][dim] as they stand: the product takes
-// B with the dims contiguous.
+// thread holding half of a query row's 128 scores; P' overwrites the scores (its
+// heads in the first 64 columns, the rests in the last) and the product reads it
+// there.  Another warpgroup turns V's codes into f16, [key][dim] as they stand: the
+// product takes B with the dims contiguous.
 #include "attn_mma.cuh"
 #include "common.cuh"
 #include "ops.h"
@@ -624,9 +623,9 @@ constexpr int kParts = 2;       // softmax warpgroups: parts of a row
 constexpr int kCols = kTileKeys / kParts;  // keys of a row that a thread holds
 constexpr int kSoftmax = 128 * kParts;     // their threads
 constexpr int kCThreads = 256 + kSoftmax;  // and the control and converter warpgroups
-// Registers: 128 a thread at launch; the control warpgroup drops to 64 and the
-// converters to 72, each softmax warpgroup rises to 184.
-constexpr uint32_t kRegsControl = 64, kRegsConvert = 72, kRegsSoftmax = 184;
+// Registers: 128 a thread at launch; the control warpgroup drops to 72 and the
+// converters to 88, each softmax warpgroup rises to 176.
+constexpr uint32_t kRegsControl = 72, kRegsConvert = 88, kRegsSoftmax = 176;
 static_assert(kRegsControl + kRegsConvert + kParts * kRegsSoftmax <= 65536 / 128,
               "register split exceeds the launch allocation");
 constexpr int kKStages = 4;     // K tiles in flight (int8, 16 KiB)
@@ -1017,35 +1016,27 @@ __global__ void __launch_bounds__(kCThreads, 1)
         tc_fence_after();
       };
       scales(0);
-      stage(tc);
-      scales(1);
-      mt0 = mt1 = -INFINITY;
-      wait_s(tc);
-      if (!idle) {
-#pragma unroll
-        for (int h = 0; h < kCols / 16; ++h) {
-          uint32_t acc[16];
-          tmem_ld_32x32b_x16(tS + (tc % 3) * 128 + lane_off + x * kCols + h * 16, acc);
-          tmem_ld_wait();
-          scores(0, tc, h, acc);
-        }
-      }
       float m = -INFINITY, l = 0.0f;
       for (int i = 0; i < w.n; ++i, ++tc) {
         const uint32_t tSx = tS + (tc % 3) * 128 + lane_off;
-        const uint32_t tSn = tS + ((tc + 1) % 3) * 128 + lane_off + x * kCols;
-        const bool more = i + 1 < w.n;
+        stage(tc);
+        scales(i + 1);
+        mt0 = mt1 = -INFINITY;
+        wait_s(tc);
+        if (!idle) {
+          uint32_t acc[4][16];
+#pragma unroll
+          for (int h = 0; h < kCols / 16; ++h) tmem_ld_32x32b_x16(tSx + x * kCols + h * 16, acc[h]);
+          tmem_ld_wait();
+#pragma unroll
+          for (int h = 0; h < kCols / 16; ++h) scores(i, tc, h, acc[h]);
+        }
         // the other parts' maxima; after the barrier every part's scores are in
         // registers, so P' may overwrite them
         float mt = fmaxf(mt0, mt1);
         float* mrow = ml + (tc & 1) * kSoftmax;
         mrow[x * 128 + t] = mt;
         named_barrier(1, kSoftmax);
-        if (more) {
-          stage(tc + 1);
-          scales(i + 2);
-          wait_s(tc + 1);
-        }
         if (idle) {
           mbar_arrive(&p_full[tc & 1]);
           continue;
@@ -1067,11 +1058,8 @@ __global__ void __launch_bounds__(kCThreads, 1)
         const ulonglong2* rv4 = reinterpret_cast<const ulonglong2*>(
             scw0 + (tc & 1) * (kSoftmax / 32 * 3 * kCols) + 2 * kCols);
         f32x2 ls0 = 0, ls1 = 0;  // (0.0f, 0.0f)
-        mt0 = mt1 = -INFINITY;
 #pragma unroll
         for (int h = 0; h < kCols / 16; ++h) {  // 16 keys: 8 columns of heads, 8 of rests
-          uint32_t acc[16];
-          if (more) tmem_ld_32x32b_x16(tSn + h * 16, acc);  // the next tile's, meanwhile
           uint32_t hi[8], lo[8];
           f32x2 p[8], rv[8];
           float f0[8], f1[8];
@@ -1110,10 +1098,6 @@ __global__ void __launch_bounds__(kCThreads, 1)
           }
           tmem_st_32x32b_x8(tSx + x * (kCols / 2) + h * 8, hi);
           tmem_st_32x32b_x8(tSx + 64 + x * (kCols / 2) + h * 8, lo);
-          if (more) {
-            tmem_ld_wait();
-            scores(i + 1, tc + 1, h, acc);
-          }
         }
         {
           float f0, f1;

@@ -101,11 +101,11 @@ def argmax_f32(x: torch.Tensor) -> torch.Tensor:
 
 def sample_f32(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor | None = None,
                top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None,
-               min_p: torch.Tensor | None = None):
+               min_p: torch.Tensor | None = None, index: torch.Tensor | None = None):
     """One token per row of logits [rows][n] fp32 from the uniform numbers u
     [rows]: softmax at `temperature` (not above 0: greedy), cut by top_k, then
     top_p, then min_p, drawn in index order.  The parameters are per row
-    (fp32 [rows]; top_k int32) or None (off).  Returns (index [rows] int32
+    (fp32 [rows]; top_k int32) or None (off); index may be given.  Returns (index [rows] int32
     holding uint32 ids, prob [rows] fp32 under the cut distribution); a row
     without a logit above -inf gives -1 (REEF_B200_NO_TOKEN) and 0."""
     rows, n = logits.shape
@@ -116,8 +116,10 @@ def sample_f32(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor 
             _take(top_k, "top_k", torch.int32, one, dev), _take(top_p, "top_p", f32, one, dev),
             _take(min_p, "min_p", f32, one, dev), _take(u, "u", f32, one, dev))
     prob = torch.empty_like(u)
-    index = torch.empty_like(u, dtype=torch.int32)
-    _call_on(dev, "reef_b200_sample_f32", rows, n, *args, index.data_ptr(), prob.data_ptr())
+    if index is None:
+        index = torch.empty_like(u, dtype=torch.int32)
+    _call_on(dev, "reef_b200_sample_f32", rows, n, *args,
+             _take(index, "index", torch.int32, one, dev, torch.uint32), prob.data_ptr())
     return index, prob
 
 

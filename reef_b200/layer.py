@@ -188,6 +188,36 @@ class LlamaLayer:
                   ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream)
         return y
 
+    def verify(self, x: torch.Tensor, lens: torch.Tensor, cache: dict,
+               parents: torch.Tensor | None = None, draft_lens: torch.Tensor | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+        """The decode step on drafted tokens: x [batch * drafts][hidden], row b *
+        drafts + t the drafted token t of sequence b (the root first), appended to
+        `cache` behind the lens [batch] committed rows; trees as in
+        kernels.tree_attn_i8.  kernels.kv_compact_i8 then keeps a path."""
+        if getattr(self, "_tiles", None) is None:
+            self._decode_tiles()
+        if x.shape[0] % self.batch != 0:
+            raise ValueError("x must hold the same number of rows for every sequence")
+        drafts, max_len, dev = x.shape[0] // self.batch, cache["max_len"], x.device
+        ws = getattr(self, "_verify_ws", None)
+        if ws is None or self._verify_for != (drafts, max_len):
+            n = _lib.lib().reef_b200_llama_verify_workspace_bytes(C.byref(self.desc), drafts,
+                                                                  max_len)
+            if n == 0:
+                raise ValueError("invalid description of a pass over drafted tokens")
+            self._verify_ws = ws = torch.empty(n, dtype=torch.uint8, device=dev)
+            self._verify_for = (drafts, max_len)
+        y = torch.empty_like(x) if out is None else out
+        tree = (self.batch, drafts)
+        _lib.call("reef_b200_llama_verify_forward", C.byref(self.desc), drafts, x.data_ptr(),
+                  y.data_ptr(), K._take(lens, "lens", torch.int32, tree[:1], dev),
+                  K._take(draft_lens, "draft_lens", torch.int32, tree[:1], dev),
+                  K._take(parents, "parents", torch.int32, tree, dev), cache["k"].data_ptr(),
+                  cache["ks"].data_ptr(), cache["v"].data_ptr(), cache["vs"].data_ptr(), max_len,
+                  ws.data_ptr(), ws.numel(), torch.cuda.current_stream(dev).cuda_stream)
+        return y
+
     def host_weights(self) -> dict:
         """This rank's weights on the host (numpy), for the reference checks."""
         return {k: getattr(self, k).cpu().numpy() for k in
@@ -308,15 +338,27 @@ class GptNeoModel:
                   torch.cuda.current_stream(self.device).cuda_stream)
         self.position += count
 
-    def generate(self, prompt, new_tokens: int):
-        """Greedy generation (GPTNeo::generate): the prompt at once, then one
-        token a time.  Returns (tokens [new_tokens] int64, logits
-        [new_tokens][vocab]), the logits behind each token."""
+    def generate(self, prompt, new_tokens: int, u=None, temperature: float = 1.0,
+                 top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0):
+        """Generation, the prompt at once, then one token a time: greedy
+        (GPTNeo::generate), or with uniform numbers u [new_tokens] in [0, 1)
+        sampled (kernels.sample_f32), each id fed back on the device.  Returns
+        (tokens [new_tokens] int64, logits [new_tokens][vocab]), the logits behind
+        each token."""
         dev = self.device
         ids = torch.tensor(list(prompt), dtype=torch.int32, device=dev)
         tokens = torch.empty(new_tokens, dtype=torch.int32, device=dev)
         logits = torch.empty((new_tokens, self.info.vocab), dtype=torch.float32, device=dev)
-        self.step(ids, logits[0], tokens[0:1])
-        for i in range(1, new_tokens):
-            self.step(tokens[i - 1:i], logits[i], tokens[i:i + 1])
+        if u is not None:
+            u = torch.as_tensor(u, dtype=torch.float32, device=dev).contiguous()
+            if u.shape != (new_tokens,):
+                raise ValueError("u must hold one number per new token")
+            one = lambda v, t: torch.full((1,), v, dtype=t, device=dev)  # noqa: E731
+            how = dict(temperature=one(temperature, torch.float32), top_k=one(top_k, torch.int32),
+                       top_p=one(top_p, torch.float32), min_p=one(min_p, torch.float32))
+        for i in range(new_tokens):
+            self.step(ids if i == 0 else tokens[i - 1:i], logits[i],
+                      tokens[i:i + 1] if u is None else None)
+            if u is not None:
+                K.sample_f32(logits[i:i + 1], u[i:i + 1], **how, index=tokens[i:i + 1])
         return tokens.to(torch.int64).cpu(), logits.cpu()

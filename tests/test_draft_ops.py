@@ -121,3 +121,29 @@ def test_wrappers_refuse_tensors_before_any_call():
         K.tree_attn_i8(f(1, 2, 4, 128, dtype=torch.int8), f(1, 2, 4),
                        f(1, 2, 8, 128, dtype=torch.int8), f(1, 2, 8),
                        f(1, 2, 8, 128, dtype=torch.int8), f(1, 2, 8), f(1))
+
+
+def test_verify_refusals(L):
+    """The layer description is checked like the decode step's; sizes by arithmetic."""
+    need = L.reef_b200_llama_verify_workspace_bytes
+    d = _lib.LlamaLayerDesc(batch=2, seq=8, hidden=512, heads_q=4, heads_kv=2, head_dim=128,
+                            ffn=1024, rms_eps=1e-5, rope_base=1e4)
+    ref = C.byref(d)
+    assert need(None, 2, 64) == 0 and need(ref, 0, 64) == 0 and need(ref, 65, 64) == 0
+    assert need(ref, 2, 62) == 0
+    f = L.reef_b200_llama_verify_forward
+    args = [P, P, P, None, None, P, P, P, P]
+    assert f(None, 2, *args, 64, P, 1 << 40, None) == INVALID
+    assert f(ref, 0, *args, 64, P, 1 << 40, None) == INVALID
+    assert f(ref, 65, *args, 64, P, 1 << 40, None) == INVALID
+    for i in (0, 1, 2, 5, 6, 7, 8):
+        a = list(args)
+        a[i] = None
+        assert f(ref, 2, *a, 64, P, 1 << 40, None) == INVALID
+    assert f(ref, 2, *args, 64, None, 1 << 40, None) == INVALID
+    assert f(ref, 2, *args, 62, P, 1 << 40, None) == ALIGNMENT
+    assert f(ref, 2, *args, 64, C.c_void_p(4096 + 16), 1 << 40, None) == ALIGNMENT
+    for i in (5, 6, 7, 8):
+        a = list(args)
+        a[i] = C.c_void_p(4096 + 4)
+        assert f(ref, 2, *a, 64, P, 1 << 40, None) == ALIGNMENT
