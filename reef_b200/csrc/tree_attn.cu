@@ -71,6 +71,7 @@ struct TreeArgs {
   int rows;    // group * drafts
   int qtiles;  // segments per (sequence, KV head)
   int ctas;
+  int per_cta;           // 1: a segment per CTA, nothing to join; 0: equal shares of the units
   float sm_scale;
   const int8_t* q8;      // [B][T][Hq][128]
   const float* q_scale;  // [B][T][Hq]
@@ -239,6 +240,36 @@ __device__ __forceinline__ void count_tiles(const TreeArgs& a, int* pre, int* sc
 struct Place {
   int b, hq, tile, tiles;
 };
+__device__ __forceinline__ Place place_of(const int* pre, int batch, int per_seq, long long u);
+
+// The first unit of CTA `cta` and how many it has.  With a segment per CTA the
+// sequence's length alone says so; otherwise every sequence's does (count_tiles:
+// all threads come here).
+template <int kThreads>
+__device__ __forceinline__ Place share_of(const TreeArgs& a, int cta, int* pre, int* scratch,
+                                          int* nunits) {
+  const int per_seq = a.heads_kv * a.qtiles;
+  Place p{};
+  if (a.per_cta) {
+    p.b = cta / per_seq;
+    p.hq = cta % per_seq;
+    const int len = a.lens[p.b];
+    bool bad;
+    const int d = drafts_of(a, p.b, len, &bad);
+    if (bad && p.hq == 0 && threadIdx.x == 0) record_error(a.err, kDevBadPosition);
+    p.tiles = d > 0 ? (len + d + kTileKeys - 1) / kTileKeys : 0;
+    *nunits = p.tiles;
+    __syncthreads();  // (as count_tiles: what the caller wrote before is in)
+    return p;
+  }
+  count_tiles<kThreads>(a, pre, scratch);
+  const long long units = static_cast<long long>(pre[a.batch]) * per_seq;
+  const long long u0 = units * cta / a.ctas, u1 = units * (cta + 1) / a.ctas;
+  *nunits = static_cast<int>(u1 - u0);
+  if (*nunits > 0) p = place_of(pre, a.batch, per_seq, u0);
+  return p;
+}
+
 __device__ __forceinline__ Place place_of(const int* pre, int batch, int per_seq, long long u) {
   int lo = 0, hi = batch - 1;  // the last b with pre[b] * per_seq <= u and tiles
   while (lo < hi) {
@@ -297,17 +328,13 @@ __global__ void __launch_bounds__(kTThreads, 2)
   }
   pdl_wait();
   pdl_trigger();  // the joining kernel waits for this grid's completion
-  count_tiles<kTThreads>(a, pre, par);  // (its barriers also publish the mbarriers)
-
   const int per_seq = a.heads_kv * a.qtiles;
-  const long long units = static_cast<long long>(pre[a.batch]) * per_seq;
-  const long long u0 = units * cta / a.ctas, u1 = units * (cta + 1) / a.ctas;
-  const int nunits = static_cast<int>(u1 - u0);
+  int nunits;
+  Place at = share_of<kTThreads>(a, cta, pre, par, &nunits);  // (publishes the mbarriers too)
   if (nunits == 0) {
-    if (tid == 0) a.meta[cta] = make_int4(-1, 0, -1, 0);
+    if (tid == 0 && !a.per_cta) a.meta[cta] = make_int4(-1, 0, -1, 0);
     return;
   }
-  Place at = place_of(pre, a.batch, per_seq, u0);
   Place ahead = at;  // next unit to issue (thread 0)
   const int first_seg = at.b * per_seq + at.hq;
   const bool first_cut = at.tile > 0;
@@ -326,7 +353,7 @@ __global__ void __launch_bounds__(kTThreads, 2)
     tma_load_3d(kv + kTileKeys * 128, &vmap, &full[s], 0, key0, pair);
     bulk_load(sc, a.k_scale + srow, n4 * 4, &full[s]);
     bulk_load(sc + kTileKeys, a.v_scale + srow, n4 * 4, &full[s]);
-    next_unit(pre, a.batch, per_seq, ahead);
+    if (j + 1 < nunits) next_unit(pre, a.batch, per_seq, ahead);
   };
   int issued = 0;  // units issued (thread 0)
   if (tid == 0)
@@ -539,7 +566,7 @@ __global__ void __launch_bounds__(kTThreads, 2)
       const bool whole = ends && !cut_before;
       float* slot = a.part + (static_cast<long long>(cta) * 2 + (cut_before ? 0 : 1)) * kRows *
                                  kPartRow;
-      if (j + 1 == nunits && tid == 0)
+      if (j + 1 == nunits && tid == 0 && !a.per_cta)
         a.meta[cta] = make_int4(first_seg, first_cut ? 1 : 0, seg, ends ? 0 : 1);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -607,7 +634,7 @@ __global__ void __launch_bounds__(kTThreads, 2)
         if (ok) issue(issued++);
       }
     }
-    next_unit(pre, a.batch, per_seq, at);
+    if (j + 1 < nunits) next_unit(pre, a.batch, per_seq, at);
   }
   // copies still in flight land before exit (only after a timeout can any
   // remain)
@@ -680,7 +707,7 @@ __device__ __forceinline__ void next_piece(const int* pre, int batch, int per_se
                                            int n, int& left) {
   left -= n;
   at.tile += n - 1;
-  next_unit(pre, batch, per_seq, at);
+  if (left > 0) next_unit(pre, batch, per_seq, at);
 }
 
 __global__ void __launch_bounds__(kCThreads, 1)
@@ -740,22 +767,18 @@ __global__ void __launch_bounds__(kCThreads, 1)
     tmem_relinquish();
   }
   tc_fence_before();
-  count_tiles<kCThreads>(a, pre, par);
+  int nunits;
+  Place at = share_of<kCThreads>(a, cta, pre, par, &nunits);
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   // columns: S_0 [0, 128), S_1 [128, 256), S_2 [256, 384), O [384, 512)
   const uint32_t tS = tmem, tO = tmem + 384;
 
   const int per_seq = a.heads_kv * a.qtiles;
-  const long long units = static_cast<long long>(pre[a.batch]) * per_seq;
-  const long long u0 = units * cta / a.ctas, u1 = units * (cta + 1) / a.ctas;
-  const int nunits = static_cast<int>(u1 - u0);
-  Place at{};
   int left = nunits;
-  if (nunits > 0) at = place_of(pre, a.batch, per_seq, u0);
   const int first_seg = at.b * per_seq + at.hq;
   const bool first_cut = at.tile > 0;
-  if (nunits == 0 && tid == 0) a.meta[cta] = make_int4(-1, 0, -1, 0);
+  if (nunits == 0 && tid == 0 && !a.per_cta) a.meta[cta] = make_int4(-1, 0, -1, 0);
 
   if (warp < 4) {
     setmaxnreg_dec<kRegsControl>();
@@ -773,7 +796,7 @@ __global__ void __launch_bounds__(kCThreads, 1)
         mbar_arrive_expect_tx(&full[s], 16384);
         tma_load_3d(ring + s * 16384, map, &full[s], 0, at.tile * kTileKeys,
                     at.b * a.heads_kv + at.hq / a.qtiles);
-        next_unit(pre, a.batch, per_seq, at);
+        if (issued + 1 < nunits) next_unit(pre, a.batch, per_seq, at);
       }
       // copies in flight land before exit
       for (int j = issued > stages ? issued - stages : 0; j < issued; ++j)
@@ -843,8 +866,10 @@ __global__ void __launch_bounds__(kCThreads, 1)
     for (int j = 0; j < nunits; ++j) {
       const int s = j % kVStages, f = j & 1;
       const bool zero = vs < kNoScale;
-      next_unit(pre, a.batch, per_seq, at);
-      if (j + 1 < nunits) vs = scale();  // a tile ahead
+      if (j + 1 < nunits) {  // a tile ahead
+        next_unit(pre, a.batch, per_seq, at);
+        vs = scale();
+      }
       if (ok) ok = mbar_wait(&v_full[s], (j / kVStages) & 1, err, kDevTimeoutFull);
       const uint8_t* row = sm + CL::kV + s * 16384 + t * 128;
       uint8_t* out = sm + CL::kVf + f * 32768 + t * 128;
@@ -1177,7 +1202,7 @@ __global__ void __launch_bounds__(kCThreads, 1)
       }
       tc_fence_before();
       mbar_arrive(o_free);
-      if (left == w.n && mine == 0)
+      if (left == w.n && mine == 0 && !a.per_cta)
         a.meta[cta] = make_int4(first_seg, first_cut ? 1 : 0, seg, ends ? 0 : 1);
       next_piece(pre, a.batch, per_seq, at, w.n, left);
       named_barrier(1, kSoftmax);  // Q's buffer is free again
@@ -1190,13 +1215,17 @@ __global__ void __launch_bounds__(kCThreads, 1)
 
 // Joins the partials of the segments that several CTAs share.  Block (c, i):
 // the segment that CTA c leaves unfinished after beginning it, query rows
-// [8i, 8i + 8) of it, one warp each (a lane holds four dims); the partials are
-// taken in the CTAs' order, i.e. the keys'.
+// [8i, 8i + 8) of it, one warp each (a lane holds four dims).  The CTAs that follow
+// are looked at 32 at a time, a lane each; the partials are added in their
+// order, i.e. the keys'.
 __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a, int tile_rows) {
   pdl_wait();
   pdl_trigger();
   const int c = blockIdx.x, rr = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int4 first = a.meta[c];
+  const int4 none = make_int4(-1, 0, -1, 0);
+  int4 mk = c + lane < a.ctas ? a.meta[c + lane] : none;
+  const int4 first = make_int4(__shfl_sync(0xffffffffu, mk.x, 0), __shfl_sync(0xffffffffu, mk.y, 0),
+                               __shfl_sync(0xffffffffu, mk.z, 0), __shfl_sync(0xffffffffu, mk.w, 0));
   // unfinished at the end of c, and begun in c
   if (first.x < 0 || first.w == 0 || (first.z == first.x && first.y != 0)) return;
   const int seg = first.z;
@@ -1207,44 +1236,74 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a, int tile_row
   const int r = (hq % a.qtiles) * tile_rows + rr;
   if (r >= d * a.group) return;
   const long long step = static_cast<long long>(2) * tile_rows * kPartRow;  // one CTA
-  const float* p = a.part + c * step + (static_cast<long long>(tile_rows) + rr) * kPartRow;
-  float m = p[0], l = p[1];
-  float4 o = reinterpret_cast<const float4*>(p + 4)[lane];
-  p = a.part + c * step + static_cast<long long>(rr) * kPartRow;  // slot 0 from here on
-  for (int k = c + 1; k < a.ctas; ++k) {
-    const int4 mk = a.meta[k];
-    p += step;
-    if (mk.x < 0) continue;  // a CTA without units
+  // c's own part is its slot 1, the others' their slot 0
+  const float* row = a.part + static_cast<long long>(rr) * kPartRow;
+  float m = -INFINITY, l = 0.0f;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int k0 = c; k0 < a.ctas; k0 += 32) {
+    if (k0 > c) mk = k0 + lane < a.ctas ? a.meta[k0 + lane] : none;
+    // lanes of the segment up to the CTA in which it ends (CTAs without units lie
+    // between)
+    const bool self = k0 + lane == c, mine = self || mk.x == seg;
+    const unsigned end = __ballot_sync(0xffffffffu, mine && !self && (mk.z != seg || mk.w == 0));
+    unsigned in = __ballot_sync(0xffffffffu, mine);
+    if (end != 0) in &= (2u << (__ffs(static_cast<int>(end)) - 1)) - 1;
+    const float* p = row + (k0 + lane) * step +
+                     (self ? static_cast<long long>(tile_rows) * kPartRow : 0);
+    float pm = -INFINITY, pl = 0.0f;
+    if (in >> lane & 1u) {
+      pm = p[0];
+      pl = p[1];
+    }
+    float mx = fmaxf(m, pm);
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
     // a CTA whose keys this row does not see has m = -inf
-    const float mx = fmaxf(m, p[0]);
     const float w0 = m == -INFINITY ? 0.0f : exp2f(m - mx);
-    const float w1 = p[0] == -INFINITY ? 0.0f : exp2f(p[0] - mx);
-    const float4 v = reinterpret_cast<const float4*>(p + 4)[lane];
-    l = l * w0 + p[1] * w1;
-    o = make_float4(o.x * w0 + v.x * w1, o.y * w0 + v.y * w1, o.z * w0 + v.z * w1,
-                    o.w * w0 + v.w * w1);
+    const float w = pm == -INFINITY ? 0.0f : exp2f(pm - mx);
+    pl *= w;
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) pl += __shfl_xor_sync(0xffffffffu, pl, s);
+    l = l * w0 + pl;
+    o = make_float4(o.x * w0, o.y * w0, o.z * w0, o.w * w0);
     m = mx;
-    if (mk.z != seg || mk.w == 0) break;  // it ends there
+#pragma unroll 4
+    for (unsigned left = in; left != 0; left &= left - 1) {
+      const int k = __ffs(static_cast<int>(left)) - 1;
+      const float wk = __shfl_sync(0xffffffffu, w, k);
+      const float* q = row + (k0 + k) * step +
+                       (k0 + k == c ? static_cast<long long>(tile_rows) * kPartRow : 0);
+      const float4 v = reinterpret_cast<const float4*>(q + 4)[lane];
+      o = make_float4(fmaf(v.x, wk, o.x), fmaf(v.y, wk, o.y), fmaf(v.z, wk, o.z),
+                      fmaf(v.w, wk, o.w));
+    }
+    if (end != 0) break;
   }
   const int t = r / a.group;
-  const long long row = (static_cast<long long>(b) * a.drafts + t) * a.heads_q +
-                        hq / a.qtiles * a.group + (r - t * a.group);
-  reinterpret_cast<float4*>(a.out + row * 128)[lane] =
+  const long long at = (static_cast<long long>(b) * a.drafts + t) * a.heads_q +
+                       hq / a.qtiles * a.group + (r - t * a.group);
+  reinterpret_cast<float4*>(a.out + at * 128)[lane] =
       make_float4(o.x / l, o.y / l, o.z / l, o.w / l);
 }
 
-// One kernel over one wave of CTAs, then the join.
+// A segment per CTA where the cache holds few tiles of keys: what the shares and
+// the join cost (4 us) is more than those tiles one after the other.  Else one
+// wave of CTAs with equal shares, and the join.  alone: the most tiles for the
+// first.
 int launch_tree(void (*kernel)(CUtensorMap, CUtensorMap, TreeArgs), int threads, int smem,
-                int per_sm, int tile_rows, const CUtensorMap& km, const CUtensorMap& vm,
-                TreeArgs& a, cudaStream_t st) {
+                int per_sm, int tile_rows, int alone, const CUtensorMap& km,
+                const CUtensorMap& vm, TreeArgs& a, cudaStream_t st) {
   a.qtiles = (a.rows + tile_rows - 1) / tile_rows;
-  // no more CTAs than the cache has room for units
-  const long long most = static_cast<long long>(a.batch) * a.heads_kv * a.qtiles *
-                         ((a.max_len + kTileKeys - 1) / kTileKeys);
-  a.ctas = static_cast<int>(std::min<long long>(static_cast<long long>(per_sm) * num_sms(), most));
+  const long long segs = static_cast<long long>(a.batch) * a.heads_kv * a.qtiles;
+  const int tiles = (a.max_len + kTileKeys - 1) / kTileKeys;
+  a.per_cta = tiles <= alone;
+  a.ctas = static_cast<int>(
+      a.per_cta ? segs
+                : std::min<long long>(static_cast<long long>(per_sm) * num_sms(), segs * tiles));
   if (int rc = launch_k(kernel, dim3(static_cast<unsigned>(a.ctas)), dim3(threads), smem, st, km,
                         vm, a))
     return rc;
+  if (a.per_cta) return kOk;
   PdlScope pdl;
   return launch_k(tree_join_kernel, dim3(static_cast<unsigned>(a.ctas), tile_rows / 8), dim3(256),
                   0, st, a, tile_rows);
@@ -1305,10 +1364,10 @@ int tree_attn_i8(const TreeProblem& p, cudaStream_t st) {
     return rc;
   if (!opt_in()) return kErrCuda;
   if (a.rows <= 8)
-    return launch_tree(tree_mma_kernel<1>, kTThreads, TL::kBytes, 2, 8, km, vm, a, st);
+    return launch_tree(tree_mma_kernel<1>, kTThreads, TL::kBytes, 2, 8, 4, km, vm, a, st);
   if (a.rows <= 16)
-    return launch_tree(tree_mma_kernel<2>, kTThreads, TL::kBytes, 2, 16, km, vm, a, st);
-  return launch_tree(tree_tc_kernel, kCThreads, CL::kBytes, 1, kTcRows, km, vm, a, st);
+    return launch_tree(tree_mma_kernel<2>, kTThreads, TL::kBytes, 2, 16, 4, km, vm, a, st);
+  return launch_tree(tree_tc_kernel, kCThreads, CL::kBytes, 1, kTcRows, 2, km, vm, a, st);
 }
 
 }  // namespace reef
