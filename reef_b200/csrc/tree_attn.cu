@@ -26,8 +26,8 @@
 // terms, head and remainder (22 bits together, where one f16 leaves 11), with
 // fp32 sums; the softmax sum takes P' / v_scale.  Two kernels:
 //
-// Up to 16 query rows, tree_mma_kernel: bound by the cache's bytes.  K and V
-// tiles by TMA through a 3-stage ring; warp w owns keys [16w, 16w + 16) of every
+// Up to 16 query rows, tree_mma_kernel: meant to be bound by the cache's bytes.  K
+// and V tiles by TMA through a ring; warp w owns keys [16w, 16w + 16) of every
 // tile with its own running maximum, S^T = K . q^T by int8 mma.sync, O^T = V^T .
 // P^T by f16 mma.sync (the rows are the n = 8 side, so few are padding).
 //
@@ -54,7 +54,6 @@ namespace {
 constexpr int kTThreads = 256;  // eight warps
 constexpr int kTWarps = kTThreads / 32;
 constexpr int kTileKeys = 128;  // keys per unit
-constexpr int kStages = 3;
 constexpr int kMaxBatch = kMaxTreeBatch;  // a CTA holds every sequence's length
 constexpr int kPartRow = 132;     // floats per row of a partial: m, l, 2 unused, O[128]
 constexpr int kMaxTileRows = 16;  // query rows per segment (tree_mma_kernel)
@@ -89,7 +88,8 @@ struct TreeArgs {
 // meta[c]: x first segment, y 1 when it began in an earlier CTA, z last
 // segment, w 1 when it goes on in the next CTA; x = -1 for a CTA without
 // units.
-struct TL {  // shared memory layout (bytes from a 1024-aligned base)
+template <int kStages>
+struct TLayout {  // shared memory layout (bytes from a 1024-aligned base)
   static constexpr int kKV = 2 * kTileKeys * 128;  // K then V, int8 [128][128] SW128
   static constexpr int kScales = kStages * kKV;    // per stage ks[128], vs[128]
   static constexpr int kWarpM = kScales + kStages * 1024;  // m[8][16], then l[8][16]
@@ -100,9 +100,10 @@ struct TL {  // shared memory layout (bytes from a 1024-aligned base)
   static constexpr int kEnd = kBars + 2 * kStages * 8;
   static constexpr int kBytes = kEnd + 1024;  // + alignment slack
 };
-static_assert(TL::kBars % 8 == 0 && TL::kAnc % 8 == 0, "aligned");
-static_assert(TL::kBytes <= 232448 / 2 - 1024, "two CTAs per SM");
-static_assert(kTWarps * 8 * 128 * 4 <= TL::kKV, "eight rows merge inside a stage");
+static_assert(TLayout<3>::kBars % 8 == 0 && TLayout<3>::kAnc % 8 == 0, "aligned");
+static_assert(TLayout<3>::kBytes <= 232448 / 2 - 1024, "two CTAs per SM");
+static_assert(TLayout<6>::kBytes <= 232448 - 1024, "one CTA per SM");
+static_assert(kTWarps * 8 * 128 * 4 <= TLayout<3>::kKV, "eight rows merge inside a stage");
 
 // two f32 -> f16 pair, the first in the low half
 __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
@@ -296,11 +297,15 @@ __device__ __forceinline__ void next_unit(const int* pre, int batch, int per_seq
   } while (p.tiles == 0);
 }
 
-// NT: query rows of a segment / 8
-template <int NT>
-__global__ void __launch_bounds__(kTThreads, 2)
+// NT: query rows of a segment / 8; with two the accumulators take 237 registers, and
+// one CTA per SM with a ring twice as deep (41 us for 16 x 4 drafts, 4 heads each
+// of 8 KV heads, 2k keys) beats two that spill (50 us): what the ring leaves of the
+// L1 is too little for spills.
+template <int NT, int kStages, int kPerSm>
+__global__ void __launch_bounds__(kTThreads, kPerSm)
     tree_mma_kernel(const __grid_constant__ CUtensorMap kmap,
                     const __grid_constant__ CUtensorMap vmap, TreeArgs a) {
+  using TL = TLayout<kStages>;
   constexpr int kRows = 8 * NT;
   extern __shared__ uint8_t sm_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) &
@@ -1316,8 +1321,8 @@ bool opt_in() {
   if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return false;
   if (!done[dev]) {
     const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
-    done[dev] = cudaFuncSetAttribute(tree_mma_kernel<1>, attr, TL::kBytes) == cudaSuccess &&
-                cudaFuncSetAttribute(tree_mma_kernel<2>, attr, TL::kBytes) == cudaSuccess &&
+    done[dev] = cudaFuncSetAttribute(tree_mma_kernel<1, 3, 2>, attr, TLayout<3>::kBytes) == cudaSuccess &&
+                cudaFuncSetAttribute(tree_mma_kernel<2, 6, 1>, attr, TLayout<6>::kBytes) == cudaSuccess &&
                 cudaFuncSetAttribute(tree_tc_kernel, attr, CL::kBytes) == cudaSuccess;
   }
   return done[dev];
@@ -1364,9 +1369,9 @@ int tree_attn_i8(const TreeProblem& p, cudaStream_t st) {
     return rc;
   if (!opt_in()) return kErrCuda;
   if (a.rows <= 8)
-    return launch_tree(tree_mma_kernel<1>, kTThreads, TL::kBytes, 2, 8, 4, km, vm, a, st);
+    return launch_tree(tree_mma_kernel<1, 3, 2>, kTThreads, TLayout<3>::kBytes, 2, 8, 4, km, vm, a, st);
   if (a.rows <= 16)
-    return launch_tree(tree_mma_kernel<2>, kTThreads, TL::kBytes, 2, 16, 4, km, vm, a, st);
+    return launch_tree(tree_mma_kernel<2, 6, 1>, kTThreads, TLayout<6>::kBytes, 1, 16, 4, km, vm, a, st);
   return launch_tree(tree_tc_kernel, kCThreads, CL::kBytes, 1, kTcRows, 2, km, vm, a, st);
 }
 
