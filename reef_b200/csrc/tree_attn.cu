@@ -33,12 +33,15 @@
 //
 // More rows, tree_tc_kernel: tcgen05 with a tile of 128 query rows, bound by
 // the exponentials and conversions of the softmax warps and the tensor pipe (S in
-// int8, P'.V twice in f16).  Scores go into three TMEM tiles in turn, so that the
-// next are there before the softmax of one begins; two warpgroups share a tile, a
+// int8, P'.V twice in f16).  Scores go into two TMEM tiles in turn, so that the
+// next are there before the softmax of one ends; two warpgroups share a tile, a
 // thread holding half of a query row's 128 scores; P' overwrites the scores (its
 // heads in the first 64 columns, the rests in the last) and the product reads it
 // there.  Another warpgroup turns V's codes into f16, [key][dim] as they stand: the
-// product takes B with the dims contiguous.
+// product takes B with the dims contiguous.  The tensor pipe truncates when it adds
+// to O (1.4e-5 of the result over 16k keys), so every six tiles O is added to a
+// second accumulator by the softmax threads, with rounding, and begins anew (5 of
+// 180 us over 16k keys).
 #include "attn_mma.cuh"
 #include "common.cuh"
 #include "ops.h"
@@ -542,10 +545,18 @@ __global__ void __launch_bounds__(kTThreads, kPerSm)
         split_codes(r[3], vc[2], vc[3]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          mma_f16(o[2 * cc][nt], va, ph[nt][0], ph[nt][1]);
-          mma_f16(o[2 * cc + 1][nt], vc, ph[nt][0], ph[nt][1]);
-          mma_f16(o[2 * cc][nt], va, pl[nt][0], pl[nt][1]);
-          mma_f16(o[2 * cc + 1][nt], vc, pl[nt][0], pl[nt][1]);
+          // the tile's own sum, then one rounded add: the tensor cores' adds
+          // truncate, and a long row of them would show
+          float t0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, t1[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          mma_f16(t0, va, pl[nt][0], pl[nt][1]);
+          mma_f16(t1, vc, pl[nt][0], pl[nt][1]);
+          mma_f16(t0, va, ph[nt][0], ph[nt][1]);
+          mma_f16(t1, vc, ph[nt][0], ph[nt][1]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            o[2 * cc][nt][e] += t0[e];
+            o[2 * cc + 1][nt][e] += t1[e];
+          }
         }
       }
     }
@@ -660,6 +671,7 @@ constexpr int kCThreads = 256 + kSoftmax;  // and the control and converter warp
 constexpr uint32_t kRegsControl = 72, kRegsConvert = 88, kRegsSoftmax = 176;
 static_assert(kRegsControl + kRegsConvert + kParts * kRegsSoftmax <= 65536 / 128,
               "register split exceeds the launch allocation");
+constexpr int kFlush = 6;       // tiles (and one more at the end) that O adds up
 constexpr int kKStages = 4;     // K tiles in flight (int8, 16 KiB)
 constexpr int kVStages = 3;     // V tiles in flight (the same)
 
@@ -672,8 +684,9 @@ struct CL {  // shared memory layout (bytes from a 1024-aligned base)
   static constexpr int kML = kScales + 2 * kSoftmax / 32 * 3 * kCols * 4;  // [2 tiles][parts][128]
   static constexpr int kPar = kML + 2 * kSoftmax * 4;         // int[64]
   static constexpr int kPre = kPar + kMaxDrafts * 4;      // int[batch + 1]
-  static constexpr int kBars = kPre + (kMaxBatch + 4) * 4;
-  static constexpr int kNumBars = 11 + 2 * kKStages + 2 * kVStages + 4;
+  static constexpr int kKeep = kPre + (kMaxBatch + 4) * 4;  // int[7][softmax threads]
+  static constexpr int kBars = kKeep + 7 * kSoftmax * 4;
+  static constexpr int kNumBars = 9 + 2 * kKStages + 2 * kVStages + 4;
   static constexpr int kTmemSlot = kBars + kNumBars * 8;
   static constexpr int kBytes = kTmemSlot + 16 + 1024;
 };
@@ -697,6 +710,16 @@ __device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t smem_addr) {
 __device__ __forceinline__ float load_now(const float* p) {
   float v;
   asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+
+// a word put aside in shared memory while registers are short
+__device__ __forceinline__ void put_aside(uint32_t at, int v) {
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(v));
+}
+__device__ __forceinline__ int take_back(uint32_t at) {
+  int v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at));
   return v;
 }
 
@@ -725,9 +748,9 @@ __global__ void __launch_bounds__(kCThreads, 1)
   uint64_t* o_free = q_full + 1;    // its accumulator has been read
   uint64_t* drain = q_full + 2;
   uint64_t* p_full = q_full + 3;    // [2] P' of an even / odd tile is in its S_x
-  uint64_t* s_full = q_full + 5;    // [3] S_x done, x = tile mod 3
-  uint64_t* o_done = q_full + 8;    // [3] the tile's product is in O
-  uint64_t* k_full = q_full + 11;
+  uint64_t* s_full = q_full + 5;    // [2] S_x done
+  uint64_t* o_done = q_full + 7;    // [2] the tile's product is in O
+  uint64_t* k_full = q_full + 9;
   uint64_t* k_empty = k_full + kKStages;
   uint64_t* v_full = k_empty + kKStages;
   uint64_t* v_empty = v_full + kVStages;
@@ -746,11 +769,9 @@ __global__ void __launch_bounds__(kCThreads, 1)
     mbar_init(q_full, kSoftmax);
     mbar_init(o_free, kSoftmax);
     mbar_init(drain, 1);
-    for (int i = 0; i < 3; ++i) {
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&o_done[i], 1);
-    }
-    for (int i = 0; i < 2; ++i) {
       mbar_init(&p_full[i], kSoftmax);
       mbar_init(&f_full[i], 4);
       mbar_init(&f_empty[i], 1);
@@ -776,8 +797,9 @@ __global__ void __launch_bounds__(kCThreads, 1)
   Place at = share_of<kCThreads>(a, cta, pre, par, &nunits);
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // columns: S_0 [0, 128), S_1 [128, 256), S_2 [256, 384), O [384, 512)
-  const uint32_t tS = tmem, tO = tmem + 384;
+  // columns: S_0 [0, 128), S_1 [128, 256), O [256, 384), the second accumulator
+  // [384, 512)
+  const uint32_t tS = tmem, tO = tmem + 256, tSum = tmem + 384;
 
   const int per_seq = a.heads_kv * a.qtiles;
   int left = nunits;
@@ -814,7 +836,7 @@ __global__ void __launch_bounds__(kCThreads, 1)
       int kc = 0, tc = 0;  // K tiles multiplied, tiles' products issued
       bool ok = true;
       auto issue_s = [&] {  // the next K tile against Q into its S_x
-        const int s = kc % kKStages, x = kc % 3;
+        const int s = kc % kKStages, x = kc & 1;
         if (!mbar_wait(&k_full[s], (kc / kKStages) & 1, err, kDevTimeoutFull)) return false;
         tc_fence_after();
         const uint32_t sk = smem_u32(sm + CL::kK + s * 16384);
@@ -833,23 +855,23 @@ __global__ void __launch_bounds__(kCThreads, 1)
         if (ok) ok = issue_s();
         if (ok && w.n > 1) ok = issue_s();
         for (int j = 0; j < w.n && ok; ++j, ++tc) {
-          // (the S_x of two tiles on is free: the product before this one has been
-          // issued, and the pipe runs in order)
-          if (j + 2 < w.n) ok = issue_s();
-          const int x = tc % 3, f = tc & 1;
+          const int x = tc & 1;
           // (the softmax may be a tile ahead of this thread, hence two p_full)
-          ok = ok && mbar_wait(&p_full[f], (tc >> 1) & 1, err, kDevTimeoutFull) &&
-               mbar_wait(&f_full[f], (tc >> 1) & 1, err, kDevTimeoutFull) &&
+          ok = mbar_wait(&p_full[x], (tc >> 1) & 1, err, kDevTimeoutFull) &&
+               mbar_wait(&f_full[x], (tc >> 1) & 1, err, kDevTimeoutFull) &&
                (j > 0 || piece == 0 || mbar_wait(o_free, (piece - 1) & 1, err, kDevTimeoutAccEmpty));
           if (!ok) break;
           tc_fence_after();
-          const uint32_t sv = smem_u32(sm + CL::kVf + f * 32768);
+          const bool fresh = j == 0 || (j % kFlush == 0 && j + 1 < w.n);
+          const uint32_t sv = smem_u32(sm + CL::kVf + x * 32768);
 #pragma unroll
           for (int kk = 0; kk < 16; ++kk)  // 16 keys a step: 8 columns of the heads, then the rests
             mma_f16_tmem_a(tO, tS + x * 128 + kk * 8, smem_desc_mn_sw128(sv + (kk & 7) * 2048),
-                           kIdescO, (j > 0 || kk > 0) ? 1u : 0u);
-          mma_commit(&f_empty[f]);
+                           kIdescO, (!fresh || kk > 0) ? 1u : 0u);
+          mma_commit(&f_empty[x]);
           mma_commit(&o_done[x]);
+          // (the pipe runs in order: S_x is overwritten once the product has read it)
+          if (j + 2 < w.n) ok = issue_s();
         }
         next_piece(pre, a.batch, per_seq, at, w.n, left);
       }
@@ -916,13 +938,23 @@ __global__ void __launch_bounds__(kCThreads, 1)
     const float base = a.sm_scale * kLog2e;
     int tc = 0;  // tiles done
     bool ok = true;
+    // What the segments' ends need alone waits in shared memory, so that the loop over
+    // the tiles has registers enough
+    const uint32_t keep = smem_u32(sm + CL::kKeep) + (tid - 256) * 4;
+    constexpr int kNext = kSoftmax * 4;
+    put_aside(keep + 6 * kNext, first_cut ? -1 - first_seg : first_seg);
     while (left > 0) {
-      const Piece w = piece_at(at, left);
-      const int b = w.at.b, hkv = w.at.hq / a.qtiles;
+      const int ntiles = piece_at(at, left).n;
+      put_aside(keep, at.b);
+      put_aside(keep + kNext, at.hq);
+      put_aside(keep + 2 * kNext, at.tile);
+      put_aside(keep + 3 * kNext, at.tiles);
+      put_aside(keep + 4 * kNext, left);
+      const int b = at.b, hkv = at.hq / a.qtiles;
       const int len = a.lens[b];
       bool bad;
       const int d = drafts_of(a, b, len, &bad);
-      const int r = (w.at.hq % a.qtiles) * kTcRows + t;  // query row of the KV head
+      const int r = (at.hq % a.qtiles) * kTcRows + t;  // query row of the KV head
       const bool live = r < d * a.group;
       const int node = r / a.group;
       // row of q8, q_scale and out
@@ -931,6 +963,7 @@ __global__ void __launch_bounds__(kCThreads, 1)
       const bool parent = a.parents != nullptr && mine < d;
       int up = 0;
       if (parent) up = a.parents[static_cast<long long>(b) * a.drafts + mine];
+      put_aside(keep + 5 * kNext, live ? qrow : -1);
       float amul = 0.0f;
       {  // this part of the row of Q
         uint8_t* q = sm + CL::kQ + t * 128;
@@ -963,7 +996,7 @@ __global__ void __launch_bounds__(kCThreads, 1)
       // a warp without a live row (as its partners in the other parts) only keeps
       // the barriers going
       const bool idle = !__any_sync(0xffffffffu, live);
-      const int keys0 = w.at.tile * kTileKeys + kCols * x;  // this part's first key
+      const int keys0 = at.tile * kTileKeys + kCols * x;  // this part's first key
       const float* ksp = a.k_scale + (static_cast<long long>(b) * a.heads_kv + hkv) * a.max_len;
       const float* vsp = a.v_scale + (ksp - a.k_scale);
       float nk[2], nv[2];
@@ -1041,122 +1074,157 @@ __global__ void __launch_bounds__(kCThreads, 1)
         }
       };
       auto wait_s = [&](int n) {  // S of the n-th tile
-        if (ok) ok = mbar_wait(&s_full[n % 3], (n / 3) & 1, err, kDevTimeoutAccFull);
+        if (ok) ok = mbar_wait(&s_full[n & 1], (n >> 1) & 1, err, kDevTimeoutAccFull);
         ok = __all_sync(0xffffffffu, ok);  // reconverge before warp-collective tcgen05.ld
         tc_fence_after();
       };
       scales(0);
       float m = -INFINITY, l = 0.0f;
-      for (int i = 0; i < w.n; ++i, ++tc) {
-        const uint32_t tSx = tS + (tc % 3) * 128 + lane_off;
-        stage(tc);
-        scales(i + 1);
-        mt0 = mt1 = -INFINITY;
-        wait_s(tc);
-        if (!idle) {
-          uint32_t acc[4][16];
+      float carry = 1.0f;  // the second accumulator's scale to the new maxima
+      int i = 0, flush = kFlush;  // the tile, and the one before whose product O is moved
+      for (;;) {
+        const int stop = min(ntiles - 1, flush);
+        for (;; ++i, ++tc) {
+          const uint32_t tSx = tS + (tc & 1) * 128 + lane_off;
+          stage(tc);
+          scales(i + 1);
+          mt0 = mt1 = -INFINITY;
+          wait_s(tc);
+          if (!idle) {
+            uint32_t acc[4][16];
 #pragma unroll
-          for (int h = 0; h < kCols / 16; ++h) tmem_ld_32x32b_x16(tSx + x * kCols + h * 16, acc[h]);
-          tmem_ld_wait();
-#pragma unroll
-          for (int h = 0; h < kCols / 16; ++h) scores(i, tc, h, acc[h]);
-        }
-        // the other parts' maxima; after the barrier every part's scores are in
-        // registers, so P' may overwrite them
-        float mt = fmaxf(mt0, mt1);
-        float* mrow = ml + (tc & 1) * kSoftmax;
-        mrow[x * 128 + t] = mt;
-        named_barrier(1, kSoftmax);
-        if (idle) {
-          mbar_arrive(&p_full[tc & 1]);
-          continue;
-        }
-#pragma unroll
-        for (int k = 0; k < kParts; ++k) mt = fmaxf(mt, mrow[k * 128 + t]);
-        // The rescale is warp-collective, so the warp decides (and its partners
-        // alike): when any row passes its maximum, every row moves to its own.
-        float alpha = 1.0f;
-        bool rescale = false;
-        if (__any_sync(0xffffffffu, mt > m + kLazy)) {
-          const float m_new = fmaxf(m, mt);
-          alpha = m == -INFINITY ? 0.0f : fast_exp2(m - m_new);
-          m = m_new;
-          rescale = i > 0;
-        }
-        const float nm = kLift - (m == -INFINITY ? 0.0f : m);
-        const f32x2 nm2 = pack2(nm, nm);
-        const ulonglong2* rv4 = reinterpret_cast<const ulonglong2*>(
-            scw0 + (tc & 1) * (kSoftmax / 32 * 3 * kCols) + 2 * kCols);
-        f32x2 ls0 = 0, ls1 = 0;  // (0.0f, 0.0f)
-#pragma unroll
-        for (int h = 0; h < kCols / 16; ++h) {  // 16 keys: 8 columns of heads, 8 of rests
-          uint32_t hi[8], lo[8];
-          f32x2 p[8], rv[8];
-          float f0[8], f1[8];
-#pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            const ulonglong2 a2 = rv4[h * 4 + (e >> 1)];
-            rv[e] = a2.x;
-            rv[e + 1] = a2.y;
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) unpack2(add2(s[h * 8 + e], nm2), f0[e], f1[e]);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            f0[e] = fast_exp2(f0[e]);
-            f1[e] = fast_exp2(f1[e]);
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            hi[e] = half2_of(f0[e], f1[e]);
-            p[e] = pack2(f0[e], f1[e]);
-          }
-#pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            ls0 = fma2(p[e], rv[e], ls0);
-            ls1 = fma2(p[e + 1], rv[e + 1], ls1);
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
-            p[e] = sub2(p[e], pack2(f.x, f.y));
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            unpack2(p[e], f0[e], f1[e]);
-            lo[e] = half2_of(f0[e], f1[e]);
-          }
-          tmem_st_32x32b_x8(tSx + x * (kCols / 2) + h * 8, hi);
-          tmem_st_32x32b_x8(tSx + 64 + x * (kCols / 2) + h * 8, lo);
-        }
-        {
-          float f0, f1;
-          unpack2(add2(ls0, ls1), f0, f1);
-          l = fmaf(l, alpha, f0 + f1);
-        }
-        if (rescale) {  // this part of O, once the products so far are in it
-          if (ok) ok = mbar_wait(&o_done[(tc - 1) % 3], ((tc - 1) / 3) & 1, err, kDevTimeoutAccFull);
-          ok = __all_sync(0xffffffffu, ok);
-          tc_fence_after();
-#pragma unroll 1
-          for (int c = 8 / kParts * x; c < 8 / kParts * (x + 1); ++c) {
-            uint32_t o[16];
-            tmem_ld_32x32b_x16(tO + lane_off + c * 16, o);
+            for (int h = 0; h < kCols / 16; ++h)
+              tmem_ld_32x32b_x16(tSx + x * kCols + h * 16, acc[h]);
             tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st_32x32b_x16(tO + lane_off + c * 16, o);
+            for (int h = 0; h < kCols / 16; ++h) scores(i, tc, h, acc[h]);
           }
+          // the other parts' maxima; after the barrier every part's scores are in
+          // registers, so P' may overwrite them
+          float mt = fmaxf(mt0, mt1);
+          float* mrow = ml + (tc & 1) * kSoftmax;
+          mrow[x * 128 + t] = mt;
+          named_barrier(1, kSoftmax);
+          if (!idle) {
+#pragma unroll
+            for (int k = 0; k < kParts; ++k) mt = fmaxf(mt, mrow[k * 128 + t]);
+            // The rescale is warp-collective, so the warp decides (and its partners
+            // alike): when any row passes its maximum, every row moves to its own.
+            float alpha = 1.0f;
+            bool rescale = false;
+            if (__any_sync(0xffffffffu, mt > m + kLazy)) {
+              const float m_new = fmaxf(m, mt);
+              alpha = m == -INFINITY ? 0.0f : fast_exp2(m - m_new);
+              m = m_new;
+              rescale = i > 0;
+              carry *= alpha;
+            }
+            const float nm = kLift - (m == -INFINITY ? 0.0f : m);
+            const f32x2 nm2 = pack2(nm, nm);
+            const ulonglong2* rv4 = reinterpret_cast<const ulonglong2*>(
+                scw0 + (tc & 1) * (kSoftmax / 32 * 3 * kCols) + 2 * kCols);
+            f32x2 ls0 = 0, ls1 = 0;  // (0.0f, 0.0f)
+#pragma unroll
+            for (int h = 0; h < kCols / 16; ++h) {  // 16 keys: 8 columns of heads, 8 of rests
+              uint32_t hi[8], lo[8];
+              f32x2 p[8], rv[8];
+              float f0[8], f1[8];
+#pragma unroll
+              for (int e = 0; e < 8; e += 2) {
+                const ulonglong2 a2 = rv4[h * 4 + (e >> 1)];
+                rv[e] = a2.x;
+                rv[e + 1] = a2.y;
+              }
+#pragma unroll
+              for (int e = 0; e < 8; ++e) unpack2(add2(s[h * 8 + e], nm2), f0[e], f1[e]);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                f0[e] = fast_exp2(f0[e]);
+                f1[e] = fast_exp2(f1[e]);
+              }
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                hi[e] = half2_of(f0[e], f1[e]);
+                p[e] = pack2(f0[e], f1[e]);
+              }
+#pragma unroll
+              for (int e = 0; e < 8; e += 2) {
+                ls0 = fma2(p[e], rv[e], ls0);
+                ls1 = fma2(p[e + 1], rv[e + 1], ls1);
+              }
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+                p[e] = sub2(p[e], pack2(f.x, f.y));
+              }
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                unpack2(p[e], f0[e], f1[e]);
+                lo[e] = half2_of(f0[e], f1[e]);
+              }
+              tmem_st_32x32b_x8(tSx + x * (kCols / 2) + h * 8, hi);
+              tmem_st_32x32b_x8(tSx + 64 + x * (kCols / 2) + h * 8, lo);
+            }
+            {
+              float f0, f1;
+              unpack2(add2(ls0, ls1), f0, f1);
+              l = fmaf(l, alpha, f0 + f1);
+            }
+            if (rescale) {  // this part of O, once the products so far are in it
+              if (ok)
+                ok = mbar_wait(&o_done[(tc - 1) & 1], ((tc - 1) >> 1) & 1, err, kDevTimeoutAccFull);
+              ok = __all_sync(0xffffffffu, ok);
+              tc_fence_after();
+#pragma unroll 1
+              for (int c = 8 / kParts * x; c < 8 / kParts * (x + 1); ++c) {
+                uint32_t o[16];
+                tmem_ld_32x32b_x16(tO + lane_off + c * 16, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                tmem_st_32x32b_x16(tO + lane_off + c * 16, o);
+              }
+            }
+            tmem_st_wait();
+            tc_fence_before();
+          }
+          if (i == stop) break;
+          mbar_arrive(&p_full[tc & 1]);
         }
-        tmem_st_wait();
-        tc_fence_before();
+        // P' of tile i is there; O goes to the second accumulator before its product,
+        // or after it if it is the last
+        const bool last = i == ntiles - 1;
+        if (last) {
+          mbar_arrive(&p_full[tc & 1]);
+          ++tc;
+        }
+        if (ok) ok = mbar_wait(&o_done[(tc - 1) & 1], ((tc - 1) >> 1) & 1, err, kDevTimeoutAccFull);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+        if (ntiles > kFlush + 1 && !idle) {
+#pragma unroll 1
+          for (int c = 0; c < 128 / kParts; c += 8) {
+            const uint32_t col = tO + lane_off + 128 / kParts * x + c;
+            uint32_t o[8], q[8];
+            tmem_ld_32x32b_x8(col, o);
+            if (flush > kFlush) tmem_ld_32x32b_x8(col + 128, q);
+            tmem_ld_wait();
+            if (flush > kFlush) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                o[e] = __float_as_uint(fmaf(__uint_as_float(q[e]), carry, __uint_as_float(o[e])));
+            }
+            tmem_st_32x32b_x8(col + 128, o);
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          carry = 1.0f;
+        }
+        if (last) break;
         mbar_arrive(&p_full[tc & 1]);
+        ++i, ++tc, flush += kFlush;
       }
       // ---- the segment's end in this CTA
-      // (S of the last tile came after the product three tiles before it, so no
-      // barrier is more than a phase behind)
-      if (ok) ok = mbar_wait(&o_done[(tc - 1) % 3], ((tc - 1) / 3) & 1, err, kDevTimeoutAccFull);
-      ok = __all_sync(0xffffffffu, ok);
       float* lrow = ml + (tc & 1) * kSoftmax;  // (the other buffer may still be read)
       lrow[x * 128 + t] = l;
       named_barrier(1, kSoftmax);  // every product is done (Q is free), the sums in
@@ -1164,9 +1232,14 @@ __global__ void __launch_bounds__(kCThreads, 1)
       float lsum = 0.0f;
 #pragma unroll
       for (int k = 0; k < kParts; ++k) lsum += lrow[k * 128 + t];
-      const int seg = b * per_seq + w.at.hq;
+      const int home = take_back(keep + 5 * kNext), cut = take_back(keep + 6 * kNext);
+      at = Place{take_back(keep), take_back(keep + kNext), take_back(keep + 2 * kNext),
+                 take_back(keep + 3 * kNext)};
+      left = take_back(keep + 4 * kNext);
+      const Piece w = piece_at(at, left);
+      const int seg = at.b * per_seq + at.hq;
       const bool ends = w.at.tile + w.n == w.at.tiles;
-      const bool cut_before = seg == first_seg && first_cut;
+      const bool cut_before = cut == -1 - seg;
       const bool whole = ends && !cut_before;
       // 16 columns at a time through this warp's part of Q's buffer, so that four
       // lanes write 64 bytes of one row
@@ -1174,12 +1247,13 @@ __global__ void __launch_bounds__(kCThreads, 1)
                                  kPartRow;
       float4* stg = reinterpret_cast<float4*>(sm + CL::kQ + (warp - 8) * 2048);  // [32 rows][4]
       if (!idle) {
+        const uint32_t from = w.n > kFlush + 1 ? tSum : tO;
         const float scale = whole ? 1.0f / lsum : 1.0f;
-        const int home = live ? (whole ? qrow : t) : -1;  // row of out or of the partial
+        const int dst_row = home < 0 ? -1 : whole ? home : t;  // row of out or of the partial
 #pragma unroll 1
         for (int c = 8 / kParts * x; c < 8 / kParts * (x + 1); ++c) {
           uint32_t o[16];
-          tmem_ld_32x32b_x16(tO + lane_off + c * 16, o);
+          tmem_ld_32x32b_x16(from + lane_off + c * 16, o);
           tmem_ld_wait();
           __syncwarp();
 #pragma unroll
@@ -1191,7 +1265,7 @@ __global__ void __launch_bounds__(kCThreads, 1)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int row = 8 * k + (lane >> 2), e = lane & 3;
-            const int to = __shfl_sync(0xffffffffu, home, row);
+            const int to = __shfl_sync(0xffffffffu, dst_row, row);
             const float4 v = stg[row * 4 + (e ^ ((row >> 1) & 3))];
             if (to >= 0) {
               float* dst = whole ? a.out + static_cast<long long>(to) * 128
@@ -1207,8 +1281,8 @@ __global__ void __launch_bounds__(kCThreads, 1)
       }
       tc_fence_before();
       mbar_arrive(o_free);
-      if (left == w.n && mine == 0 && !a.per_cta)
-        a.meta[cta] = make_int4(first_seg, first_cut ? 1 : 0, seg, ends ? 0 : 1);
+      if (left == w.n && tid == 256 && !a.per_cta)
+        a.meta[cta] = make_int4(cut < 0 ? -1 - cut : cut, cut < 0 ? 1 : 0, seg, ends ? 0 : 1);
       next_piece(pre, a.batch, per_seq, at, w.n, left);
       named_barrier(1, kSoftmax);  // Q's buffer is free again
     }
