@@ -61,7 +61,8 @@ constexpr int kMaxCluster = 8;
 constexpr int kSlice = 16384;   // logits per CTA: two CTAs fit on an SM
 constexpr int kList = 1016;     // of a warp's run (1024 at that slice) that are listed
 constexpr int kGather = 1024;   // of a row that one CTA takes over
-constexpr int kNear = 256;      // elements of one step, over the cluster (two threads each)
+constexpr int kNear = kThreads; // elements of one step, over the cluster
+constexpr int kFew = 256;       // candidates of a row that are compared each with each
 constexpr int kMaxResident = 168 * 1024;      // bytes of logits a CTA keeps
 constexpr double kOne = 8796093022208.0;      // 2^43, the weight 1
 constexpr uint32_t kKeyNegInf = 0x007fffffu;  // key_of(-inf)
@@ -80,6 +81,7 @@ struct SampleArgs {
   const float* u;
   uint32_t* index;
   float* prob;
+  int* err;
 };
 
 struct alignas(16) Shared {
@@ -102,17 +104,18 @@ struct alignas(16) Shared {
   union {
     uint16_t list[kWarps][kList];  // elements of a warp's run, in index order
     struct {                       // or the odd half of a count
-      u64 ahead[kNear];
-      int rank[kNear];
+      u64 ahead[kFew];
+      int rank[kFew];
     } sub;
   };
   int listed[kWarps];
   int near_n[kMaxCluster];
   u64 slot[2][2][kMaxCluster];   // two values of every CTA
-  double exp2_of[64];            // 2^(j / 64)
+  double exp2_of[16];            // 2^(j / 16), one to a pair of banks
   u64 warp[kWarps], part[kWarps];
   u64 pick[2];                   // a result of one thread for all
   u64 found;                     // a result of one CTA for all
+  uint64_t loaded;               // mbarrier: the slice is in shared memory
 };
 
 // Order-preserving key: x < y exactly when key_of(x) < key_of(y); -0 equals
@@ -146,15 +149,15 @@ __device__ __forceinline__ u64 warp_prefix(u64 v, int lane) {
 }
 
 struct Row {
-  const float* x;   // this CTA's slice, global
+  const float* x;   // this CTA's slice, global, from a 16-byte boundary on
   const float* sm;  // its resident part
   int resident, count;
-  int first;        // index of its first element in the row
+  int first;        // index of its first element in the row (below 0: not of the row, -inf)
   float top;        // the row's maximum
   bool plain;       // magnitudes at which light() holds
   float heavy;      // values from here up weigh 2^-20 or (barely) less
   float least;      // values below weigh nothing
-  double c, rcp_t;  // log2(e) / T, 1 / T
+  double c, rcp_t, per_bit;  // log2(e) / T, 1 / T, T ln 2
   float c_hi, c_lo, k_hi, k_lo;  // c, and top * c - 43, in two terms
   const double* exp2_of;
   __device__ __forceinline__ float at(int i) const { return i < resident ? sm[i] : __ldg(x + i); }
@@ -179,27 +182,32 @@ struct Row {
   __device__ __forceinline__ u64 fixed(float v) const {
     if (!plain) return __double2ull_rn(weight(v) * kOne);
     if (!(v >= heavy)) return light(v);
-    // 2^t = 2^(n / 64) * 2^r, |r| <= 1/128: a table, and the series of e^(r ln 2)
-    // to the fifth power (2^-53 of it is left out)
+    return full(v);
+  }
+  // weight * 2^43 of a value not far below `heavy` (of a row that is plain)
+  __device__ __forceinline__ u64 full(float v) const {
+    // 2^t = 2^(n / 16) * 2^r, |r| <= 1/32: a table, and the series of e^(r ln 2)
+    // to the sixth power (2^-51 of it is left out)
     const double t = (static_cast<double>(v) - static_cast<double>(top)) * c;
-    const double kShift = 105553116266496.0;  // 1.5 * 2^46: a sum's last bit is 1/64
+    const double kShift = 422212465065984.0;  // 1.5 * 2^48: a sum's last bit is 1/16
     const double m = t + kShift;
     const int n = __double2loint(m);
     const double r = t - (m - kShift);
-    double q = __fma_rn(r, 0x1.5d87fe78a6730p-10, 0x1.3b2ab6fba4e77p-7);
+    double q = __fma_rn(r, 0x1.430912f86c786p-13, 0x1.5d87fe78a6730p-10);
+    q = __fma_rn(q, r, 0x1.3b2ab6fba4e77p-7);
     q = __fma_rn(q, r, 0x1.c6b08d704a0bfp-5);
     q = __fma_rn(q, r, 0x1.ebfbdff82c58ep-3);
     q = __fma_rn(q, r, 0x1.62e42fefa39efp-1);
-    const double s = exp2_of[n & 63];
-    const double w = __fma_rn(q * r, s, s);  // in [2^-1, 2), times 2^(n >> 6)
-    const double up = __hiloint2double(__double2hiint(w) + (((n >> 6) + 43) << 20),
+    const double s = exp2_of[n & 15];
+    const double w = __fma_rn(q * r, s, s);  // in [2^-1, 2), times 2^(n >> 4)
+    const double up = __hiloint2double(__double2hiint(w) + (((n >> 4) + 43) << 20),
                                        __double2loint(w));
     // the integer next to it, from the low bits of a sum with 2^52
     return static_cast<u64>(__double_as_longlong(up + 4503599627370496.0)) & 0xfffffffffffffull;
   }
   // a value that weighs a little less than 2^log2w
   __device__ __forceinline__ float below_top(double log2w) const {
-    const double d = log2w / c;
+    const double d = log2w * per_bit;
     return static_cast<float>(top + d - 1e-6 * (fabs(d) + fabsf(top)));
   }
 };
@@ -240,10 +248,12 @@ struct Ctx {
     i0 = min(count, warp * per);
     i1 = min(count, i0 + per);
   }
-  // four neighbours of the slice, -inf from i1 on
+  // four neighbours of the slice (i divides by 4), -inf from i1 on (up to which the
+  // run goes: a multiple of 4, or the slice's end, behind which -inf stands)
   __device__ __forceinline__ float4 four(const Row& r, int i, int i1) const {
-    if (i + 3 < min(i1, r.resident)) return *reinterpret_cast<const float4*>(r.sm + i);
-    return make_float4(i < i1 ? r.at(i) : -INFINITY, i + 1 < i1 ? r.at(i + 1) : -INFINITY,
+    if (i < min(i1, r.resident)) return *reinterpret_cast<const float4*>(r.sm + i);
+    if (i >= i1) return make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    return make_float4(r.at(i), i + 1 < i1 ? r.at(i + 1) : -INFINITY,
                        i + 2 < i1 ? r.at(i + 2) : -INFINITY, i + 3 < i1 ? r.at(i + 3) : -INFINITY);
   }
   // f(x, index) for the elements of the warp's run
@@ -299,18 +309,14 @@ __device__ __forceinline__ u64 row_sum(Ctx& c, const Row& r, F f, const u64** sl
   return all;
 }
 
-// Lists the elements from `least` up (above -inf, and in `weigh` not above
-// r.heavy), and counts them; with `weigh` also sums all weights, per warp and
-// CTA as row_sum does.  Whether every warp's list fits.
-template <bool kWeigh>
-__device__ __noinline__ bool build(Ctx& ctx, const Row& row, float least, u64* mass,
-                                   const u64** slot, int* count) {
+// Lists the elements from `least` up (above -inf) and counts them.  Whether every
+// warp's list fits.
+__device__ __noinline__ bool build(Ctx& ctx, const Row& row, float least, int* count) {
   const Ctx c = ctx;
   const Row r = row;
   Shared* s = c.s;
   uint16_t* list = s->list[c.warp];
   int i0, i1, n = 0;
-  uint32_t light = 0;  // 256 elements per lane at most, each under 2^23
   c.run_of(r.count, i0, i1);
   const unsigned below = (1u << c.lane) - 1;
   for (int i = i0; i < i1; i += 128) {
@@ -318,35 +324,23 @@ __device__ __noinline__ bool build(Ctx& ctx, const Row& row, float least, u64* m
     const float4 v4 = c.four(r, j, i1);
     const float v[4] = {v4.x, v4.y, v4.z, v4.w};
     unsigned ballot[4];
-    bool in[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      in[e] = v[e] >= least;
-      ballot[e] = __ballot_sync(0xffffffffu, in[e]);
-      if (kWeigh) {
-        const uint32_t w = r.light(v[e]);
-        light += in[e] ? 0u : w;
-      }
-    }
+    for (int e = 0; e < 4; ++e) ballot[e] = __ballot_sync(0xffffffffu, v[e] >= least);
     if ((ballot[0] | ballot[1] | ballot[2] | ballot[3]) == 0) continue;
     int at = n;
 #pragma unroll
     for (int e = 0; e < 4; ++e) at += __popc(ballot[e] & below);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      if (in[e]) {
+      if (v[e] >= least) {
         if (at < kList) list[at] = static_cast<uint16_t>(j + e);
         ++at;
       }
       n += __popc(ballot[e]);
     }
   }
-  u64 sum = light;
   if (c.lane == 0) s->listed[c.warp] = n;
-  __syncwarp();
-  if (kWeigh)
-    for (int j = c.lane; j < min(n, kList); j += 32) sum += r.fixed(r.at(list[j]));
-  const u64 all = block_sum(c, sum);
+  __syncthreads();
   int total = 0;
   bool fits = r.count <= 65536;
 #pragma unroll
@@ -354,14 +348,11 @@ __device__ __noinline__ bool build(Ctx& ctx, const Row& row, float least, u64* m
     total += s->listed[w];
     fits = fits && s->listed[w] <= kList;
   }
-  u64(*got)[kMaxCluster] = ctx.exchange(all, fits ? static_cast<u64>(total) : ~0ull);
-  *slot = got[0];
-  *mass = 0;
+  const u64* got = ctx.exchange(fits ? static_cast<u64>(total) : ~0ull)[0];
   *count = 0;
   for (int k = 0; k < c.ranks; ++k) {
-    *mass += got[0][k];
-    fits = fits && got[1][k] != ~0ull;
-    *count += static_cast<int>(got[1][k]);
+    fits = fits && got[k] != ~0ull;
+    *count += static_cast<int>(got[k]);
   }
   return fits;
 }
@@ -370,12 +361,12 @@ __device__ __noinline__ bool build(Ctx& ctx, const Row& row, float least, u64* m
 // (false in the others: they are done), else in every CTA.
 __device__ __noinline__ bool gather(Ctx& c, const Row& r, int count) {
   Shared* s = c.s;
-  if (count > (c.ranks == 1 ? kNear : kGather)) {
+  if (count > kGather) {
     c.mode = kListed;
     return true;
   }
   int at = 0;
-  for (int k = 0; k < c.rank; ++k) at += static_cast<int>(s->slot[c.flip][1][k]);
+  for (int k = 0; k < c.rank; ++k) at += static_cast<int>(s->slot[c.flip][0][k]);
   for (int w = 0; w < c.warp; ++w) at += s->listed[w];
   Shared* o = c.of(0);
   for (int j = c.lane; j < s->listed[c.warp]; j += 32) {
@@ -491,28 +482,38 @@ __device__ __forceinline__ bool scan_bins(const Ctx& c, int bins, u64 target, Of
   return s->pick[0] != ~0ull;
 }
 
-// One histogram of the cluster: bin_of(x, index) is an element's bin, or -1.
-// As scan_bins; every CTA gets the same answer.
-template <bool kMass, typename BinOf>
-__device__ __forceinline__ bool histogram(const Ctx& c, const Row& r, BinOf bin_of, u64 target,
-                                          int* bin, u64* before) {
+// Equal steps of the range from `least` up to the row's maximum.  Rounding is
+// monotone, and so are the steps.
+struct Steps {
+  float least, scale;
+  __device__ __forceinline__ Steps(float from, float top)
+      : least(from), scale((kBins - 0.25f) / (top - from)) {}
+  __device__ __forceinline__ bool part() const { return scale > 0.0f && scale < 1e30f; }
+  __device__ __forceinline__ int bin(float x) const {  // of x from `least` up
+    return min(kBins - 1, static_cast<int>((x - least) * scale));
+  }
+  // a little less than what lies in bin b
+  __device__ __forceinline__ float below(int b, float top) const {
+    return least + static_cast<float>(b) / scale -
+           1e-6f * (top - least + fabsf(least) + fabsf(top));
+  }
+};
+
+// A mass into this CTA's histogram: a 64-bit add of two 32-bit ones (the carry goes
+// on, the order is free).
+__device__ __forceinline__ void add_mass(Shared* s, int b, u64 v) {
+  const uint32_t vl = static_cast<uint32_t>(v), vh = static_cast<uint32_t>(v >> 32);
+  uint32_t carry = 0;
+  if (vl != 0) carry = atomicAdd(&s->hist[b], vl) > ~vl;
+  if (vh + carry != 0) atomicAdd(&s->hist[kBins + b], vh + carry);
+}
+
+// The CTAs' histograms (counts or masses; all done) added up, and scan_bins: every
+// CTA gets the same answer.
+template <bool kMass>
+__device__ __noinline__ bool scan_cluster(const Ctx& ctx, u64 target, int* bin, u64* before) {
+  const Ctx c = ctx;
   Shared* s = c.s;
-  for (int i = c.tid; i < (kMass ? 2 : 1) * kBins; i += kThreads) s->hist[i] = 0;
-  __syncthreads();
-  c.each(r, [&](float x, int i) {
-    const int b = bin_of(x, i);
-    if (b < 0) return;
-    if (kMass) {  // a 64-bit add of two 32-bit ones: the carry goes on, the order is free
-      const u64 v = r.fixed(x);
-      const uint32_t vl = static_cast<uint32_t>(v), vh = static_cast<uint32_t>(v >> 32);
-      uint32_t carry = 0;
-      if (vl != 0) carry = atomicAdd(&s->hist[b], vl) > ~vl;
-      if (vh + carry != 0) atomicAdd(&s->hist[kBins + b], vh + carry);
-    } else {
-      atomicAdd(&s->hist[b], 1u);
-    }
-  });
-  c.sync();  // every CTA's histogram is done
   auto local = [&](const Shared* o, int b) -> u64 {
     return o->hist[b] + (kMass ? static_cast<u64>(o->hist[kBins + b]) << 32 : 0ull);
   };
@@ -528,32 +529,81 @@ __device__ __forceinline__ bool histogram(const Ctx& c, const Row& r, BinOf bin_
   return scan_bins(c, kBins, target, [&](int b) { return s->sum[b]; }, bin, before);
 }
 
-// Of the elements that `cut` keeps from `least` up (finite), the shortest
-// prefix of the order whose sum (count or mass) reaches `target` (>= 1), as a
-// tighter cut.  False, with the cut as it was, where equal steps do not part
-// them.
+// One histogram of the cluster: bin_of(x, index) is an element's bin, or -1.
+// As scan_bins.
+template <bool kMass, typename BinOf>
+__device__ __forceinline__ bool histogram(const Ctx& c, const Row& r, BinOf bin_of, u64 target,
+                                          int* bin, u64* before) {
+  Shared* s = c.s;
+  for (int i = c.tid; i < (kMass ? 2 : 1) * kBins; i += kThreads) s->hist[i] = 0;
+  __syncthreads();
+  c.each(r, [&](float x, int i) {
+    const int b = bin_of(x, i);
+    if (b < 0) return;
+    if (kMass) add_mass(s, b, r.fixed(x));
+    else atomicAdd(&s->hist[b], 1u);
+  });
+  c.sync();
+  return scan_cluster<kMass>(c, target, bin, before);
+}
+
+// The mass of a row that is plain: s->warp holds this CTA's per warp, slot the
+// cluster's per CTA, as after row_sum; with kHist also this CTA's histogram of the
+// elements from steps.least up.  A warp that has no heavy (no light) one among 32
+// neighbours leaves out what is for those.
+template <bool kHist>
+__device__ __noinline__ u64 weigh(Ctx& ctx, const Row& row, const Steps& st, const u64** slot) {
+  const Ctx c = ctx;
+  const Row r = row;
+  const Steps steps = st;
+  Shared* s = c.s;
+  if (kHist) {
+    for (int i = c.tid; i < 2 * kBins; i += kThreads) s->hist[i] = 0;
+    __syncthreads();
+  }
+  int i0, i1;
+  c.run_of(r.count, i0, i1);
+  u64 sum = 0;
+  for (int i = i0; i < i1; i += 128) {
+    const float4 v4 = c.four(r, i + 4 * c.lane, i1);
+    const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool heavy = v[e] >= r.heavy;
+      const unsigned ballot = __ballot_sync(0xffffffffu, heavy);
+      u64 w = 0;
+      if (ballot != 0) w = r.full(fmaxf(v[e], r.least));
+      if (ballot != 0xffffffffu) {
+        const uint32_t l = r.light(v[e]);
+        w = heavy ? w : l;
+      }
+      sum += w;
+      if (kHist && v[e] >= steps.least) add_mass(s, steps.bin(v[e]), w);
+    }
+  }
+  *slot = ctx.exchange(block_sum(c, sum))[0];
+  u64 all = 0;
+  for (int k = 0; k < c.ranks; ++k) all += (*slot)[k];
+  return all;
+}
+
+// Of the elements of step `bin` that `cut` keeps, the shortest prefix of the order
+// whose sum (count or mass) reaches `target` (>= 1), as a tighter cut.  False, with
+// the cut as it was, where they are too many.
 template <bool kMass>
-__device__ __noinline__ bool select_steps(const Ctx& ctx, const Row& row, Cut* cut_io, float least,
-                                          u64 target) {
+__device__ __noinline__ bool select_near(const Ctx& ctx, const Row& row, Cut* cut_io,
+                                         const Steps& st, int bin, u64 target) {
   const Ctx c = ctx;
   const Row r = row;
   const Cut cut = *cut_io;
+  const Steps steps = st;
   Shared* s = c.s;
-  const float scale = (kBins - 0.25f) / (r.top - least);
-  if (!(scale > 0.0f && scale < 1e30f)) return false;
-  auto bin_of = [&](float x, int i) {  // rounding is monotone: so are the steps
-    if (!(x >= least) || !cut.keeps(x, i)) return -1;
-    return min(kBins - 1, static_cast<int>((x - least) * scale));
-  };
   if (c.tid == 0) s->near_n[c.rank] = 0;
-  int bin;
-  u64 before;
-  if (!histogram<kMass>(c, r, bin_of, target, &bin, &before)) return false;
-  target -= before;
+  __syncthreads();
   // the elements of that step to every CTA, each into its own part
   const int room = kNear / c.ranks;
   c.each(r, [&](float x, int i) {
-    if (bin_of(x, i) != bin) return;
+    if (!(x >= steps.least) || steps.bin(x) != bin || !cut.keeps(x, i)) return;
     const int at = atomicAdd(&s->near_n[c.rank], 1);
     if (at >= room) return;
     for (int k = 0; k < c.ranks; ++k) {
@@ -591,6 +641,23 @@ __device__ __noinline__ bool select_steps(const Ctx& ctx, const Row& row, Cut* c
   *cut_io = Cut{__uint_as_float(static_cast<uint32_t>(s->found >> 32)),
                 static_cast<int>(static_cast<uint32_t>(s->found))};
   return true;
+}
+
+// Of the elements that `cut` keeps from `least` up (finite), the shortest
+// prefix of the order whose sum reaches `target`, as a tighter cut.  False, with the
+// cut as it was, where equal steps do not part them.
+template <bool kMass>
+__device__ __forceinline__ bool select_steps(const Ctx& c, const Row& r, Cut* cut, float least,
+                                             u64 target) {
+  const Steps steps(least, r.top);
+  if (!steps.part()) return false;
+  int bin;
+  u64 before;
+  auto bin_of = [&](float x, int i) {
+    return x >= least && cut->keeps(x, i) ? steps.bin(x) : -1;
+  };
+  return histogram<kMass>(c, r, bin_of, target, &bin, &before) &&
+         select_near<kMass>(c, r, cut, steps, bin, target - before);
 }
 
 // select_steps by radix, for any values: ten bits of the key at a time (the
@@ -636,6 +703,14 @@ __device__ __noinline__ void select_radix(Ctx& c, const Row& r, Cut* cut_io, flo
   *cut_io = Cut{value, static_cast<int>(c.s->found)};
 }
 
+// u times the total, below it
+__device__ __forceinline__ u64 drawn(float u, u64 all) {
+  const u64 at = u > 0.0f ? static_cast<u64>(fmin(static_cast<double>(u), 1.0) *
+                                             static_cast<double>(all))
+                          : 0ull;
+  return at < all ? at : all - 1;
+}
+
 // The rest of a row whose candidates (all that any filter may keep, in index
 // order) are one to a thread: the ranks and the masses ahead of each by comparing
 // with every other, then the draw by a prefix sum.  k: 0 is off; keeps_min(x)
@@ -646,7 +721,7 @@ __device__ __forceinline__ void finish_few(const Ctx& c, const Row& r, int k, fl
                                            float* prob) {
   Shared* s = c.s;
   // two threads to an element, for the even and the odd ones of the others
-  const int e = c.tid % kNear, half = c.tid / kNear;
+  const int e = c.tid % kFew, half = c.tid / kFew;
   const bool have = e < c.gathered;
   const float x = have ? s->all.x[e] : 0.0f;
   const int at = have ? s->all.index[e] : 0;
@@ -659,7 +734,7 @@ __device__ __forceinline__ void finish_few(const Ctx& c, const Row& r, int k, fl
   u64 ahead = 0;
   if (have) {
 #pragma unroll 4
-    for (int j = half; j < c.gathered; j += kThreads / kNear) {
+    for (int j = half; j < c.gathered; j += kThreads / kFew) {
       const float y = s->all.x[j];
       const bool before = y > x || (y == x && j < e);
       rank += before;
@@ -685,10 +760,7 @@ __device__ __forceinline__ void finish_few(const Ctx& c, const Row& r, int k, fl
   if (w != 0 && !keeps_min(x)) w = 0;
   __syncthreads();  // (s->warp has been read)
   const u64 all = block_sum(c, w);
-  u64 target = u > 0.0f ? static_cast<u64>(fmin(static_cast<double>(u), 1.0) *
-                                           static_cast<double>(all))
-                        : 0ull;
-  target = target < all ? target : all - 1;
+  const u64 target = drawn(u, all);
   u64 run = warp_prefix(w, c.lane) - w;
   for (int i = 0; i < c.warp; ++i) run += s->warp[i];
   if (run <= target && target < run + w) {  // (w is 0 in the second halves)
@@ -696,6 +768,74 @@ __device__ __forceinline__ void finish_few(const Ctx& c, const Row& r, int k, fl
     if (prob != nullptr)
       *prob = static_cast<float>(r.weight(x) * kOne / static_cast<double>(all));
   }
+}
+
+// The rest of a row for top-p (and min-p) in the one CTA that has gathered the
+// elements from step `bin` up, in index order, two to a thread: those above the step
+// stay, those in it while the mass ahead of them is below `target` (`before` is that
+// of the steps above), and the draw is a prefix sum.  False where too many lie in the
+// step.
+template <typename KeepsMin>
+__device__ __forceinline__ bool finish_steps(const Ctx& c, const Row& r, const Steps& steps,
+                                             int bin, u64 before, u64 target, KeepsMin keeps_min,
+                                             float u, uint32_t* index, float* prob) {
+  static_assert(kGather == 2 * kThreads, "two to a thread");
+  Shared* s = c.s;
+  if (c.tid == 0) s->near_n[0] = 0;
+  __syncthreads();
+  float x[2];
+  u64 w[2];
+  bool near[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int j = 2 * c.tid + e;
+    x[e] = j < c.gathered ? s->all.x[j] : -INFINITY;
+    const int b = x[e] >= steps.least ? steps.bin(x[e]) : -1;
+    near[e] = b == bin;
+    w[e] = b >= bin ? r.fixed(x[e]) : 0ull;
+    if (near[e]) {
+      const int at = atomicAdd(&s->near_n[0], 1);
+      if (at < kNear) {
+        s->near.x[at] = x[e];
+        s->near.index[at] = j;
+        s->near.w[at] = w[e];
+      }
+    }
+  }
+  __syncthreads();
+  const int n = s->near_n[0];
+  if (n > kNear) return false;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    if (near[e]) {
+      u64 ahead = before;
+      for (int j = 0; j < n; ++j) {
+        const float y = s->near.x[j];
+        if (y > x[e] || (y == x[e] && s->near.index[j] < 2 * c.tid + e)) ahead += s->near.w[j];
+      }
+      if (ahead >= target) w[e] = 0;
+    }
+    if (w[e] != 0 && !keeps_min(x[e])) w[e] = 0;
+  }
+  const u64 own = w[0] + w[1];
+  u64 run = warp_prefix(own, c.lane);
+  if (c.lane == 31) s->warp[c.warp] = run;
+  __syncthreads();
+  u64 all = 0;
+  run -= own;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    if (i < c.warp) run += s->warp[i];
+    all += s->warp[i];
+  }
+  const u64 at = drawn(u, all);
+  if (run <= at && at < run + own) {
+    const int e = at < run + w[0] ? 0 : 1;
+    *index = static_cast<uint32_t>(s->all.index[2 * c.tid + e]);
+    if (prob != nullptr)
+      *prob = static_cast<float>(r.weight(x[e]) * kOne / static_cast<double>(all));
+  }
+  return true;
 }
 
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
@@ -713,44 +853,78 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
   c.mode = kAll;
   c.gathered = 0;
   const long long row = blockIdx.x / c.ranks;
+  // The slices begin on 16-byte boundaries: rank 0's with up to three elements that
+  // are not of the row.
+  const float* x = a.logits + row * a.n;
+  const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(x) >> 2) & 3);
   Row r;
-  r.first = min(a.n, c.rank * a.slice);
-  r.count = min(a.n, (c.rank + 1) * a.slice) - r.first;
-  r.x = a.logits + row * a.n + r.first;
+  r.first = c.rank * a.slice - shift;
+  r.count = max(0, min(a.n - r.first, a.slice));
+  r.x = x + r.first;
   r.sm = sm;
   r.resident = min(r.count, a.resident);
+  const int lo = min(c.rank == 0 ? shift : 0, r.resident);
+  const int al = min((lo + 3) & ~3, r.resident), ah = max(al, r.resident & ~3);
+  if (c.tid == 0) {
+    mbar_init(&s->loaded, 1);
+    fence_barrier_init();
+    mbar_arrive_expect_tx(&s->loaded, (ah - al) * 4);
+    if (ah > al) bulk_load(sm + al, r.x + al, (ah - al) * 4, &s->loaded);
+  }
+  if (c.tid < 4) {  // what stands before and behind whole pieces, and the padding
+    if (c.tid < lo) sm[c.tid] = -INFINITY;
+    if (lo + c.tid < al) sm[lo + c.tid] = __ldg(r.x + lo + c.tid);
+    if (ah + c.tid < ((r.resident + 3) & ~3))
+      sm[ah + c.tid] = ah + c.tid < r.resident ? __ldg(r.x + ah + c.tid) : -INFINITY;
+  }
   const float t = a.temperature != nullptr ? a.temperature[row] : 1.0f;
   const float p = a.top_p != nullptr ? a.top_p[row] : 1.0f;
   const float mp = a.min_p != nullptr ? a.min_p[row] : 0.0f;
+  const float u = a.u[row];
   int k = a.top_k != nullptr ? a.top_k[row] : 0;
   if (k >= a.n || !(t > 0.0f)) k = 0;
 
   // (every CTA of the cluster takes the same branches: row-wide values only)
-  if (k > 0) {
+  if (k > 0)
     for (int i = c.tid; i < 2 * kBins; i += kThreads) s->hist[i] = 0;
-    __syncthreads();
-  }
+  if (c.tid < 16 && t > 0.0f) s->exp2_of[c.tid] = exp2(c.tid / 16.0);
+  __syncthreads();
   // the others have started when the wait below ends: nothing is written to them before
   if (c.ranks > 1) cg::this_cluster().barrier_arrive();
 
-  // ---- the slice into shared memory, the row's maximum, and for top-k the
-  // histogram of the maxima of eight logits
+  // what does not need the logits, while they come
+  r.rcp_t = 1.0 / static_cast<double>(t);
+  r.per_bit = 0.6931471805599453 * static_cast<double>(t);
+  r.c = 1.4426950408889634 * r.rcp_t;
+  r.c_hi = static_cast<float>(r.c);
+  r.c_lo = static_cast<float>(r.c - static_cast<double>(r.c_hi));
+  // What top-p keeps last weighs more than (1 - p) / n of the total (what it leaves
+  // out is n at most, and weighs less), which is 1 at least; half of that, for the
+  // roundings on the way
+  const double p_bits =
+      p < 1.0f ? log2(0.5 * (1.0 - static_cast<double>(fmaxf(p, 0.0f))) / a.n) : 0.0;
+  const double least = mp > 0.0f ? fmin(static_cast<double>(mp), 1.0) : 0.0;
+  const double min_ln = least > 0.0 ? log(least) * static_cast<double>(t) : 0.0;
+
+  // ---- the row's maximum, and for top-k the histogram of the maxima of groups of
+  // eight logits
+  mbar_wait(&s->loaded, 0, a.err, kDevTimeoutFull);
   float top = -INFINITY;  // (fmaxf passes NaN over)
-  for (int i = c.tid; i < r.count; i += 8 * kThreads) {
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      v[j] = i + j * kThreads < r.count ? __ldg(r.x + i + j * kThreads) : -INFINITY;
-    float m = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (i + j * kThreads < r.resident) sm[i + j * kThreads] = v[j];
-      m = fmaxf(m, v[j]);
+  for (int i = 4 * c.tid; i < r.resident; i += 8 * kThreads) {
+    const float4 v = *reinterpret_cast<const float4*>(sm + i);
+    float m = fmaxf(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)), -INFINITY);
+    if (i + 4 * kThreads < r.resident) {
+      const float4 w = *reinterpret_cast<const float4*>(sm + i + 4 * kThreads);
+      m = fmaxf(m, fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)));
     }
     if (k > 0) atomicAdd(&s->hist[key_of(m) >> 21], 1u);
     top = fmaxf(top, m);
   }
-  if (c.tid < 64 && t > 0.0f) s->exp2_of[c.tid] = exp2(c.tid / 64.0);
+  for (int i = r.resident + c.tid; i < r.count; i += kThreads) {
+    const float v = fmaxf(__ldg(r.x + i), -INFINITY);
+    if (k > 0) atomicAdd(&s->hist[key_of(v) >> 21], 1u);
+    top = fmaxf(top, v);
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (c.lane == 0) s->warp[c.warp] = key_of(top);
@@ -782,23 +956,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
     }
     return;
   }
-  r.rcp_t = 1.0 / static_cast<double>(t);
-  r.c = 1.4426950408889634 * r.rcp_t;
-  r.c_hi = static_cast<float>(r.c);
-  r.c_lo = static_cast<float>(r.c - static_cast<double>(r.c_hi));
-  const double shift = static_cast<double>(top) * r.c - 43.0;
-  r.k_hi = static_cast<float>(shift);
-  r.k_lo = static_cast<float>(shift - static_cast<double>(r.k_hi));
-  r.plain = fabs(shift) < 8192.0 && fabsf(top) < 1e30f && t < 1e30f && t > 1e-30f;
+  const double k2 = static_cast<double>(top) * r.c - 43.0;
+  r.k_hi = static_cast<float>(k2);
+  r.k_lo = static_cast<float>(k2 - static_cast<double>(r.k_hi));
+  r.plain = fabs(k2) < 8192.0 && fabsf(top) < 1e30f && t < 1e30f && t > 1e-30f;
   r.heavy = r.below_top(-20.0);
   r.least = r.below_top(-60.0);
   r.exp2_of = s->exp2_of;
 
   // min-p in float but next to the border, in double there
-  const double least = mp > 0.0f ? fmin(static_cast<double>(mp), 1.0) : 0.0;
   float sure = INFINITY, out = -INFINITY;  // x from `sure` up stays, below `out` not
   if (least > 0.0 && r.plain) {
-    const double x = static_cast<double>(top) + log(least) * static_cast<double>(t);
+    const double x = static_cast<double>(top) + min_ln;
     const double slack = 1e-6 * (fabs(x) + fabs(static_cast<double>(top)) + 1e-6);
     sure = static_cast<float>(x + slack);
     out = static_cast<float>(x - slack);
@@ -806,7 +975,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
   auto keeps_min = [&](float x) {
     return least == 0.0 || x >= sure || (!(x < out) && r.weight(x) >= least);
   };
-  const float u = a.u[row];
   uint32_t* const index = a.index + row;
   float* const prob = a.prob != nullptr ? a.prob + row : nullptr;
 
@@ -833,55 +1001,68 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
     }
     // k groups have their maximum, so k logits lie, from here up
     const float from = ok ? floor_of(static_cast<uint32_t>(bin) << 21) : -INFINITY;
-    ok = from > -INFINITY && build<false>(c, r, from, &mass, &slot, &count);
+    ok = from > -INFINITY && build(c, r, from, &count);
     if (ok && !gather(c, r, count)) return;
-    if (c.mode == kGathered && c.gathered <= kNear)
+    if (c.mode == kGathered && c.gathered <= kFew)
       return finish_few(c, r, k, p, keeps_min, u, index, prob);
     if (!ok || !select_steps<false>(c, r, &cut, from, static_cast<u64>(k)))
       select_radix<false>(c, r, &cut, from, static_cast<u64>(k));
   }
+  bool summed = false;  // s->warp and slot hold the sums of all
   if (p < 1.0f) {
-    bool listed = false;
-    auto kept = [&](float x, int i) { return cut.keeps(x, i) ? r.fixed(x) : 0ull; };
-    if (k == 0 && r.plain) {
-      // the total is 1 at least; half of the bound, for the roundings on the way
-      const double l2 = log2(0.5 * (1.0 - static_cast<double>(fmaxf(p, 0.0f))) / a.n);
-      listed = build<true>(c, r, r.below_top(fmin(l2, -20.0)), &mass, &slot, &count);
-      if (listed && !gather(c, r, count)) return;
+    const Steps steps(r.below_top(p_bits), top);
+    if (k == 0 && r.plain && steps.part()) {
+      mass = weigh<true>(c, r, steps, &slot);
+      summed = true;
+    } else {
+      mass = row_sum(c, r, [&](float x, int i) { return cut.keeps(x, i) ? r.fixed(x) : 0ull; },
+                     &slot);
     }
-    if (!listed) mass = row_sum(c, r, kept, &slot);
     const double want = ceil(static_cast<double>(p) * static_cast<double>(mass));
     const u64 target = want > 1.0 ? static_cast<u64>(want) : 1ull;
     if (target < mass) {
+      bool done = false;
       float from = cut.value;
-      if (r.plain)
-        from = fmaxf(from,
-                     r.below_top(log2(0.5 * static_cast<double>(mass - target) / (a.n * kOne))));
-      if (c.mode == kAll || !(from > -INFINITY) || !select_steps<true>(c, r, &cut, from, target))
-        select_radix<true>(c, r, &cut, from, target);
+      if (summed) {
+        summed = false;
+        int bin;
+        u64 before;
+        if (scan_cluster<true>(c, target, &bin, &before)) {
+          from = steps.below(bin, top);
+          if (build(c, r, from, &count) && !gather(c, r, count)) return;
+          if (c.mode == kGathered && finish_steps(c, r, steps, bin, before, target, keeps_min, u,
+                                                  index, prob))
+            return;
+          done = select_near<true>(c, r, &cut, steps, bin, target - before);
+        }
+      } else {
+        if (r.plain)
+          from = fmaxf(from,
+                       r.below_top(log2(0.5 * static_cast<double>(mass - target) / (a.n * kOne))));
+        done = c.mode != kAll && from > -INFINITY && select_steps<true>(c, r, &cut, from, target);
+      }
+      if (!done) select_radix<true>(c, r, &cut, from, target);
     }
+    summed = summed && least == 0.0;
   }
   auto kept = [&](float x, int i) -> u64 {
     return cut.keeps(x, i) && keeps_min(x) ? r.fixed(x) : 0ull;
   };
 
   // ---- the draw
-  u64 all = 0;
-  bool summed = false;
+  u64 all = mass;
   if (c.mode == kAll && r.plain && k == 0 && !(p < 1.0f)) {
     if (least > 0.0) {  // what min-p may keep is listed
-      if (build<false>(c, r, out, &mass, &slot, &count) && !gather(c, r, count)) return;
-      if (c.mode == kGathered && c.gathered <= kNear)
+      if (build(c, r, out, &count) && !gather(c, r, count)) return;
+      if (c.mode == kGathered && c.gathered <= kFew)
         return finish_few(c, r, 0, 1.0f, keeps_min, u, index, prob);
-    } else {  // every element counts: s->warp and slot hold their sums
-      summed = build<true>(c, r, r.heavy, &all, &slot, &count);
+    } else {  // every element counts
+      all = weigh<false>(c, r, Steps(0.0f, 1.0f), &slot);
+      summed = true;
     }
   }
   if (!summed) all = row_sum(c, r, kept, &slot);
-  u64 target = u > 0.0f ? static_cast<u64>(fmin(static_cast<double>(u), 1.0) *
-                                           static_cast<double>(all))
-                        : 0ull;
-  target = target < all ? target : all - 1;
+  const u64 target = drawn(u, all);
   if (locate(c, r, kept, slot, target, &at, &at_x)) {
     *index = static_cast<uint32_t>(at);
     if (prob != nullptr)
@@ -901,7 +1082,7 @@ int sample_f32(long long rows, int n, const float* logits, const float* temperat
   while (c < kMaxCluster && (n > c * kSlice || (rows * c * 2 <= num_sms() && n > c * 4096))) c *= 2;
   SampleArgs a{};
   a.n = n;
-  a.slice = ((n + c - 1) / c + 3) & ~3;
+  a.slice = ((n + 3 + c - 1) / c + 3) & ~3;  // (up to three elements before the row)
   a.resident = static_cast<int>(std::min<long long>(a.slice, fit));
   a.logits = logits;
   a.temperature = temperature;
@@ -911,6 +1092,7 @@ int sample_f32(long long rows, int n, const float* logits, const float* temperat
   a.u = u;
   a.index = index;
   a.prob = prob;
+  a.err = device_error_ptr();
   const size_t smem = sizeof(Shared) + static_cast<size_t>(a.resident) * 4;
   static bool opted[64] = {};
   int dev = 0;
