@@ -115,8 +115,18 @@ struct alignas(16) Shared {
   u64 warp[kWarps], part[kWarps];
   u64 pick[2];                   // a result of one thread for all
   u64 found;                     // a result of one CTA for all
+  double ready[3];               // 1 / T, log2 of top-p's bound, T ln(min-p)
   uint64_t loaded;               // mbarrier: the slice is in shared memory
 };
+
+// By name, not through pointers in structs: a pointer that a function is handed is
+// generic, and loads and atomics through it cost half as much again.
+extern __shared__ __align__(16) uint8_t g_smem[];
+__device__ __forceinline__ Shared* shared() { return reinterpret_cast<Shared*>(g_smem); }
+// the resident part of this CTA's slice
+__device__ __forceinline__ float* resident_part() {
+  return reinterpret_cast<float*>(g_smem + sizeof(Shared));
+}
 
 // Order-preserving key: x < y exactly when key_of(x) < key_of(y); -0 equals
 // +0, NaN is taken as -inf.
@@ -150,8 +160,7 @@ __device__ __forceinline__ u64 warp_prefix(u64 v, int lane) {
 
 struct Row {
   const float* x;   // this CTA's slice, global, from a 16-byte boundary on
-  const float* sm;  // its resident part
-  int resident, count;
+  int resident, count;  // elements of it in shared memory, and in all
   int first;        // index of its first element in the row (below 0: not of the row, -inf)
   float top;        // the row's maximum
   bool plain;       // magnitudes at which light() holds
@@ -159,8 +168,7 @@ struct Row {
   float least;      // values below weigh nothing
   double c, rcp_t, per_bit;  // log2(e) / T, 1 / T, T ln 2
   float c_hi, c_lo, k_hi, k_lo;  // c, and top * c - 43, in two terms
-  const double* exp2_of;
-  __device__ __forceinline__ float at(int i) const { return i < resident ? sm[i] : __ldg(x + i); }
+  __device__ __forceinline__ float at(int i) const { return i < resident ? resident_part()[i] : __ldg(x + i); }
   // exp((x - top) / T), 1 for the maximum itself, 0 for -inf and NaN
   __device__ __forceinline__ double weight(float v) const {
     if (v == top) return 1.0;
@@ -198,7 +206,7 @@ struct Row {
     q = __fma_rn(q, r, 0x1.c6b08d704a0bfp-5);
     q = __fma_rn(q, r, 0x1.ebfbdff82c58ep-3);
     q = __fma_rn(q, r, 0x1.62e42fefa39efp-1);
-    const double s = exp2_of[n & 15];
+    const double s = shared()->exp2_of[n & 15];
     const double w = __fma_rn(q * r, s, s);  // in [2^-1, 2), times 2^(n >> 4)
     const double up = __hiloint2double(__double2hiint(w) + (((n >> 4) + 43) << 20),
                                        __double2loint(w));
@@ -227,7 +235,6 @@ enum Mode : int { kAll, kListed, kGathered };
 
 struct Ctx {
   cg::cluster_group cluster;
-  Shared* s;
   int rank, ranks, tid, warp, lane, flip;
   Mode mode;
   int gathered;
@@ -236,7 +243,7 @@ struct Ctx {
     else cluster.sync();
   }
   __device__ __forceinline__ Shared* of(int k) const {
-    return ranks == 1 ? s : cluster.map_shared_rank(s, k);
+    return ranks == 1 ? shared() : cluster.map_shared_rank(shared(), k);
   }
   // Warp w's part of the slice (or gathered list): a contiguous run, so that
   // the warps' sums are prefix sums in index order.
@@ -251,7 +258,7 @@ struct Ctx {
   // four neighbours of the slice (i divides by 4), -inf from i1 on (up to which the
   // run goes: a multiple of 4, or the slice's end, behind which -inf stands)
   __device__ __forceinline__ float4 four(const Row& r, int i, int i1) const {
-    if (i < min(i1, r.resident)) return *reinterpret_cast<const float4*>(r.sm + i);
+    if (i < min(i1, r.resident)) return *reinterpret_cast<const float4*>(resident_part() + i);
     if (i >= i1) return make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
     return make_float4(r.at(i), i + 1 < i1 ? r.at(i + 1) : -INFINITY,
                        i + 2 < i1 ? r.at(i + 2) : -INFINITY, i + 3 < i1 ? r.at(i + 3) : -INFINITY);
@@ -264,13 +271,13 @@ struct Ctx {
       run_of(r.count, i0, i1);
       for (int i = i0 + lane; i < i1; i += 32) f(r.at(i), r.first + i);
     } else if (mode == kListed) {
-      for (int j = lane; j < s->listed[warp]; j += 32) {
-        const int i = s->list[warp][j];
+      for (int j = lane; j < shared()->listed[warp]; j += 32) {
+        const int i = shared()->list[warp][j];
         f(r.at(i), r.first + i);
       }
     } else {
       run_of(gathered, i0, i1);
-      for (int j = i0 + lane; j < i1; j += 32) f(s->all.x[j], s->all.index[j]);
+      for (int j = i0 + lane; j < i1; j += 32) f(shared()->all.x[j], shared()->all.index[j]);
     }
   }
   // Two values of every CTA to every CTA: of CTA k in [0][k] and [1][k] after it.
@@ -282,18 +289,18 @@ struct Ctx {
       o->slot[flip][1][rank] = w;
     }
     sync();
-    return s->slot[flip];
+    return shared()->slot[flip];
   }
 };
 
 // this CTA's sum of the warps' values, in s->warp after it
 __device__ __forceinline__ u64 block_sum(const Ctx& c, u64 v) {
   v = warp_sum(v);
-  if (c.lane == 0) c.s->warp[c.warp] = v;
+  if (c.lane == 0) shared()->warp[c.warp] = v;
   __syncthreads();
   u64 mine = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) mine += c.s->warp[w];
+  for (int w = 0; w < kWarps; ++w) mine += shared()->warp[w];
   return mine;
 }
 
@@ -314,7 +321,7 @@ __device__ __forceinline__ u64 row_sum(Ctx& c, const Row& r, F f, const u64** sl
 __device__ __noinline__ bool build(Ctx& ctx, const Row& row, float least, int* count) {
   const Ctx c = ctx;
   const Row r = row;
-  Shared* s = c.s;
+  Shared* s = shared();
   uint16_t* list = s->list[c.warp];
   int i0, i1, n = 0;
   c.run_of(r.count, i0, i1);
@@ -323,11 +330,12 @@ __device__ __noinline__ bool build(Ctx& ctx, const Row& row, float least, int* c
     const int j = i + 4 * c.lane;
     const float4 v4 = c.four(r, j, i1);
     const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+    // (most of the time none is there)
+    if (!__any_sync(0xffffffffu, fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) >= least)) continue;
     unsigned ballot[4];
+    int at = n;
 #pragma unroll
     for (int e = 0; e < 4; ++e) ballot[e] = __ballot_sync(0xffffffffu, v[e] >= least);
-    if ((ballot[0] | ballot[1] | ballot[2] | ballot[3]) == 0) continue;
-    int at = n;
 #pragma unroll
     for (int e = 0; e < 4; ++e) at += __popc(ballot[e] & below);
 #pragma unroll
@@ -360,7 +368,7 @@ __device__ __noinline__ bool build(Ctx& ctx, const Row& row, float least, int* c
 // After build: the row goes on with the list alone, in CTA 0 if it is short
 // (false in the others: they are done), else in every CTA.
 __device__ __noinline__ bool gather(Ctx& c, const Row& r, int count) {
-  Shared* s = c.s;
+  Shared* s = shared();
   if (count > kGather) {
     c.mode = kListed;
     return true;
@@ -393,8 +401,8 @@ __device__ __forceinline__ bool locate(Ctx& c, const Row& r, F f, const u64* slo
   }
   if (target >= slot[c.rank]) return false;
   int w = 0;
-  for (; w < kWarps - 1 && target >= c.s->warp[w]; ++w) target -= c.s->warp[w];
-  int i0 = 0, i1 = c.s->listed[w];
+  for (; w < kWarps - 1 && target >= shared()->warp[w]; ++w) target -= shared()->warp[w];
+  int i0 = 0, i1 = shared()->listed[w];
   if (c.mode != kListed) {
     const int count = c.mode == kAll ? r.count : c.gathered;
     const int per = c.run_length(count);
@@ -404,10 +412,10 @@ __device__ __forceinline__ bool locate(Ctx& c, const Row& r, F f, const u64* slo
   const int per = (i1 - i0 + kWarps - 1) / kWarps;
   auto element = [&](int j, float* x, int* index) {
     if (c.mode == kGathered) {
-      *x = c.s->all.x[j];
-      *index = c.s->all.index[j];
+      *x = shared()->all.x[j];
+      *index = shared()->all.index[j];
     } else {
-      const int i = c.mode == kListed ? c.s->list[w][j] : j;
+      const int i = c.mode == kListed ? shared()->list[w][j] : j;
       *x = r.at(i);
       *index = r.first + i;
     }
@@ -422,13 +430,13 @@ __device__ __forceinline__ bool locate(Ctx& c, const Row& r, F f, const u64* slo
     v += f(x, index);
   }
   v = warp_sum(v);
-  if (c.lane == 0) c.s->part[c.warp] = v;
+  if (c.lane == 0) shared()->part[c.warp] = v;
   __syncthreads();
   for (int k = 0; k < c.warp; ++k) {
-    if (target < c.s->part[k]) return false;
-    target -= c.s->part[k];
+    if (target < shared()->part[k]) return false;
+    target -= shared()->part[k];
   }
-  if (target >= c.s->part[c.warp]) return false;
+  if (target >= shared()->part[c.warp]) return false;
   for (int i = i0; i < i1; i += 32) {
     u64 run = 0;
     if (i + c.lane < i1) {
@@ -454,7 +462,7 @@ __device__ __forceinline__ bool locate(Ctx& c, const Row& r, F f, const u64* slo
 template <typename Of>
 __device__ __forceinline__ bool scan_bins(const Ctx& c, int bins, u64 target, Of of, int* bin,
                                           u64* before) {
-  Shared* s = c.s;
+  Shared* s = shared();
   const int m = bins / kThreads;
   u64 own = 0;
   for (int j = 0; j < m; ++j) own += of(bins - 1 - (c.tid * m + j));
@@ -501,11 +509,11 @@ struct Steps {
 
 // A mass into this CTA's histogram: a 64-bit add of two 32-bit ones (the carry goes
 // on, the order is free).
-__device__ __forceinline__ void add_mass(Shared* s, int b, u64 v) {
-  const uint32_t vl = static_cast<uint32_t>(v), vh = static_cast<uint32_t>(v >> 32);
-  uint32_t carry = 0;
-  if (vl != 0) carry = atomicAdd(&s->hist[b], vl) > ~vl;
-  if (vh + carry != 0) atomicAdd(&s->hist[kBins + b], vh + carry);
+__device__ __forceinline__ void add_mass(int b, u64 v) {
+  const uint32_t low = static_cast<uint32_t>(v);
+  const uint32_t high = static_cast<uint32_t>(v >> 32) +
+                        (atomicAdd(&shared()->hist[b], low) > ~low ? 1u : 0u);
+  if (high != 0) atomicAdd(&shared()->hist[kBins + b], high);
 }
 
 // The CTAs' histograms (counts or masses; all done) added up, and scan_bins: every
@@ -513,7 +521,7 @@ __device__ __forceinline__ void add_mass(Shared* s, int b, u64 v) {
 template <bool kMass>
 __device__ __noinline__ bool scan_cluster(const Ctx& ctx, u64 target, int* bin, u64* before) {
   const Ctx c = ctx;
-  Shared* s = c.s;
+  Shared* s = shared();
   auto local = [&](const Shared* o, int b) -> u64 {
     return o->hist[b] + (kMass ? static_cast<u64>(o->hist[kBins + b]) << 32 : 0ull);
   };
@@ -534,13 +542,13 @@ __device__ __noinline__ bool scan_cluster(const Ctx& ctx, u64 target, int* bin, 
 template <bool kMass, typename BinOf>
 __device__ __forceinline__ bool histogram(const Ctx& c, const Row& r, BinOf bin_of, u64 target,
                                           int* bin, u64* before) {
-  Shared* s = c.s;
+  Shared* s = shared();
   for (int i = c.tid; i < (kMass ? 2 : 1) * kBins; i += kThreads) s->hist[i] = 0;
   __syncthreads();
   c.each(r, [&](float x, int i) {
     const int b = bin_of(x, i);
     if (b < 0) return;
-    if (kMass) add_mass(s, b, r.fixed(x));
+    if (kMass) add_mass(b, r.fixed(x));
     else atomicAdd(&s->hist[b], 1u);
   });
   c.sync();
@@ -556,7 +564,7 @@ __device__ __noinline__ u64 weigh(Ctx& ctx, const Row& row, const Steps& st, con
   const Ctx c = ctx;
   const Row r = row;
   const Steps steps = st;
-  Shared* s = c.s;
+  Shared* s = shared();
   if (kHist) {
     for (int i = c.tid; i < 2 * kBins; i += kThreads) s->hist[i] = 0;
     __syncthreads();
@@ -578,7 +586,7 @@ __device__ __noinline__ u64 weigh(Ctx& ctx, const Row& row, const Steps& st, con
         w = heavy ? w : l;
       }
       sum += w;
-      if (kHist && v[e] >= steps.least) add_mass(s, steps.bin(v[e]), w);
+      if (kHist && v[e] >= steps.least) add_mass(steps.bin(v[e]), w);
     }
   }
   *slot = ctx.exchange(block_sum(c, sum))[0];
@@ -597,7 +605,7 @@ __device__ __noinline__ bool select_near(const Ctx& ctx, const Row& row, Cut* cu
   const Row r = row;
   const Cut cut = *cut_io;
   const Steps steps = st;
-  Shared* s = c.s;
+  Shared* s = shared();
   if (c.tid == 0) s->near_n[c.rank] = 0;
   __syncthreads();
   // the elements of that step to every CTA, each into its own part
@@ -615,21 +623,27 @@ __device__ __noinline__ bool select_near(const Ctx& ctx, const Row& row, Cut* cu
   __syncthreads();
   if (c.tid < c.ranks && c.tid != c.rank) c.of(c.tid)->near_n[c.rank] = s->near_n[c.rank];
   c.sync();
+  // thread t: the t-th of them
   bool fits = true;
-  for (int k = 0; k < c.ranks; ++k) fits = fits && s->near_n[k] <= room;
+  int total = 0, e = -1;
+  for (int k = 0; k < c.ranks; ++k) {
+    const int n = s->near_n[k];
+    fits = fits && n <= room;
+    if (c.tid >= total && c.tid < total + n) e = k * room + c.tid - total;
+    total += n;
+  }
   if (!fits) return false;
-  const bool mine = c.tid < kNear && c.tid % room < s->near_n[min(c.tid / room, c.ranks - 1)];
   float x = 0.0f;
   int index = 0;
   u64 w = 0;
-  if (mine) {
-    x = s->near.x[c.tid];
-    index = s->near.index[c.tid];
+  if (e >= 0) {
+    x = s->near.x[e];
+    index = s->near.index[e];
     w = kMass ? r.fixed(x) : 1ull;
-    s->near.w[c.tid] = w;
+    s->near.w[e] = w;
   }
   __syncthreads();
-  if (mine) {
+  if (e >= 0) {
     u64 run = 0;  // what comes before it in the order
     for (int k = 0; k < c.ranks; ++k)
       for (int j = k * room; j < k * room + s->near_n[k]; ++j)
@@ -700,7 +714,7 @@ __device__ __noinline__ void select_radix(Ctx& c, const Row& r, Cut* cut_io, flo
   if (locate(c, r, tie, slot, ties - 1, &at, &at_x))
     for (int k = 0; k < c.ranks; ++k) c.of(k)->found = static_cast<u64>(at);
   c.sync();
-  *cut_io = Cut{value, static_cast<int>(c.s->found)};
+  *cut_io = Cut{value, static_cast<int>(shared()->found)};
 }
 
 // u times the total, below it
@@ -719,7 +733,7 @@ template <typename KeepsMin>
 __device__ __forceinline__ void finish_few(const Ctx& c, const Row& r, int k, float p,
                                            KeepsMin keeps_min, float u, uint32_t* index,
                                            float* prob) {
-  Shared* s = c.s;
+  Shared* s = shared();
   // two threads to an element, for the even and the odd ones of the others
   const int e = c.tid % kFew, half = c.tid / kFew;
   const bool have = e < c.gathered;
@@ -780,7 +794,7 @@ __device__ __forceinline__ bool finish_steps(const Ctx& c, const Row& r, const S
                                              int bin, u64 before, u64 target, KeepsMin keeps_min,
                                              float u, uint32_t* index, float* prob) {
   static_assert(kGather == 2 * kThreads, "two to a thread");
-  Shared* s = c.s;
+  Shared* s = shared();
   if (c.tid == 0) s->near_n[0] = 0;
   __syncthreads();
   float x[2];
@@ -839,11 +853,9 @@ __device__ __forceinline__ bool finish_steps(const Ctx& c, const Row& r, const S
 }
 
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
-  extern __shared__ __align__(16) uint8_t raw[];
   Ctx c{cg::this_cluster()};
-  Shared* s = reinterpret_cast<Shared*>(raw);
-  float* sm = reinterpret_cast<float*>(raw + sizeof(Shared));
-  c.s = s;
+  Shared* s = shared();
+  float* sm = resident_part();
   c.rank = static_cast<int>(c.cluster.block_rank());
   c.ranks = static_cast<int>(c.cluster.num_blocks());
   c.tid = threadIdx.x;
@@ -861,7 +873,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
   r.first = c.rank * a.slice - shift;
   r.count = max(0, min(a.n - r.first, a.slice));
   r.x = x + r.first;
-  r.sm = sm;
   r.resident = min(r.count, a.resident);
   const int lo = min(c.rank == 0 ? shift : 0, r.resident);
   const int al = min((lo + 3) & ~3, r.resident), ah = max(al, r.resident & ~3);
@@ -892,19 +903,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
   // the others have started when the wait below ends: nothing is written to them before
   if (c.ranks > 1) cg::this_cluster().barrier_arrive();
 
-  // what does not need the logits, while they come
-  r.rcp_t = 1.0 / static_cast<double>(t);
-  r.per_bit = 0.6931471805599453 * static_cast<double>(t);
-  r.c = 1.4426950408889634 * r.rcp_t;
-  r.c_hi = static_cast<float>(r.c);
-  r.c_lo = static_cast<float>(r.c - static_cast<double>(r.c_hi));
+  // what does not need the logits, while they come (one thread each: a double's
+  // logarithm in all of them costs as much as a pass over the slice).
   // What top-p keeps last weighs more than (1 - p) / n of the total (what it leaves
   // out is n at most, and weighs less), which is 1 at least; half of that, for the
-  // roundings on the way
-  const double p_bits =
-      p < 1.0f ? log2(0.5 * (1.0 - static_cast<double>(fmaxf(p, 0.0f))) / a.n) : 0.0;
+  // roundings on the way.
   const double least = mp > 0.0f ? fmin(static_cast<double>(mp), 1.0) : 0.0;
-  const double min_ln = least > 0.0 ? log(least) * static_cast<double>(t) : 0.0;
+  if (c.tid == 32) s->ready[0] = 1.0 / static_cast<double>(t);
+  if (c.tid == 64 && p < 1.0f)
+    s->ready[1] = log2(0.5 * (1.0 - static_cast<double>(fmaxf(p, 0.0f))) / a.n);
+  if (c.tid == 96 && least > 0.0) s->ready[2] = log(least) * static_cast<double>(t);
 
   // ---- the row's maximum, and for top-k the histogram of the maxima of groups of
   // eight logits
@@ -929,6 +937,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (c.lane == 0) s->warp[c.warp] = key_of(top);
   __syncthreads();
+  r.rcp_t = s->ready[0];
   u64 best = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) best = s->warp[w] > best ? s->warp[w] : best;
@@ -956,18 +965,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
     }
     return;
   }
+  r.per_bit = 0.6931471805599453 * static_cast<double>(t);
+  r.c = 1.4426950408889634 * r.rcp_t;
+  r.c_hi = static_cast<float>(r.c);
+  r.c_lo = static_cast<float>(r.c - static_cast<double>(r.c_hi));
   const double k2 = static_cast<double>(top) * r.c - 43.0;
   r.k_hi = static_cast<float>(k2);
   r.k_lo = static_cast<float>(k2 - static_cast<double>(r.k_hi));
   r.plain = fabs(k2) < 8192.0 && fabsf(top) < 1e30f && t < 1e30f && t > 1e-30f;
   r.heavy = r.below_top(-20.0);
   r.least = r.below_top(-60.0);
-  r.exp2_of = s->exp2_of;
 
   // min-p in float but next to the border, in double there
   float sure = INFINITY, out = -INFINITY;  // x from `sure` up stays, below `out` not
   if (least > 0.0 && r.plain) {
-    const double x = static_cast<double>(top) + min_ln;
+    const double x = static_cast<double>(top) + s->ready[2];
     const double slack = 1e-6 * (fabs(x) + fabs(static_cast<double>(top)) + 1e-6);
     sure = static_cast<float>(x + slack);
     out = static_cast<float>(x - slack);
@@ -1010,7 +1022,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
   }
   bool summed = false;  // s->warp and slot hold the sums of all
   if (p < 1.0f) {
-    const Steps steps(r.below_top(p_bits), top);
+    const Steps steps(r.below_top(s->ready[1]), top);
     if (k == 0 && r.plain && steps.part()) {
       mass = weigh<true>(c, r, steps, &slot);
       summed = true;
