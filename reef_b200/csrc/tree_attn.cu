@@ -113,10 +113,16 @@ __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+// p - h, in one step (the difference is exact)
+__device__ __forceinline__ float less_half(float p, uint32_t h) {
+  float d;
+  asm("{.reg .b16 m; mov.b16 m, 0xBC00; fma.rn.f32.f16 %0, %1, m, %2;}"  // h * -1 + p
+      : "=f"(d) : "h"(static_cast<uint16_t>(h)), "f"(p));
+  return d;
+}
 // what the pair leaves of them, as another pair
 __device__ __forceinline__ uint32_t rest_of(float lo, float hi, uint32_t pair) {
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pair));
-  return half2_of(lo - f.x, hi - f.y);
+  return half2_of(less_half(lo, pair), less_half(hi, pair >> 16));
 }
 
 // two f32 in a register pair, and arithmetic on both at once
@@ -132,11 +138,6 @@ __device__ __forceinline__ void unpack2(f32x2 v, float& lo, float& hi) {
 __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
   f32x2 d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ f32x2 sub2(f32x2 a, f32x2 b) {
-  f32x2 d;
-  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
 __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
@@ -1153,15 +1154,7 @@ __global__ void __launch_bounds__(kCThreads, 1)
                 ls1 = fma2(p[e + 1], rv[e + 1], ls1);
               }
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
-                p[e] = sub2(p[e], pack2(f.x, f.y));
-              }
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                unpack2(p[e], f0[e], f1[e]);
-                lo[e] = half2_of(f0[e], f1[e]);
-              }
+              for (int e = 0; e < 8; ++e) lo[e] = rest_of(f0[e], f1[e], hi[e]);
               tmem_st_32x32b_x8(tSx + x * (kCols / 2) + h * 8, hi);
               tmem_st_32x32b_x8(tSx + 64 + x * (kCols / 2) + h * 8, lo);
             }
