@@ -116,6 +116,33 @@ def test_flat_rows_and_ties():
     check(x, u, m=np.full(rows, 1.0))
 
 
+@pytest.mark.parametrize("n", [900, 20000, 128000])
+@pytest.mark.parametrize("equal", [40, 300, 700, 899])
+def test_borders_among_equal_values(n, equal):
+    """Top-p's border inside a block of equal logits, from a few to more than a step
+    of the histogram is sorted for, with heavier ones above and lighter ones below."""
+    rows = 6
+    r = np.random.RandomState(n + equal)
+    x = r.randn(rows, n).astype(np.float32) - 30.0
+    for i in range(rows):
+        at = r.permutation(n)[:equal]
+        x[i, at] = 2.0
+        x[i, at[:10]] = 2.0 + np.arange(10, dtype=np.float32) / 4
+    u = r.rand(rows).astype(np.float32)
+    check(x, u, p=np.full(rows, 0.7))
+    check(x, u, p=r.uniform(0.2, 0.999, rows), m=np.full(rows, 0.05))
+    check(x, u, k=np.full(rows, equal // 2 + 5), p=r.uniform(0.2, 0.999, rows))
+
+
+@pytest.mark.parametrize("p", [0.99, 0.999999])
+def test_nearly_everything_kept(p):
+    """Flat rows of which top-p leaves out little: what is kept does not fit a list."""
+    rows, n = 4, 128000
+    r = np.random.RandomState(5)
+    x = (r.randn(rows, n) * 0.2).astype(np.float32)
+    check(x, r.rand(rows).astype(np.float32), p=np.full(rows, p))
+
+
 def test_masks_and_values_that_are_no_numbers():
     n = 3001
     low, inf, nan = np.finfo(np.float32).min, np.inf, np.nan

@@ -155,6 +155,22 @@ def test_long_rows_lose_nothing(t, hq):
     assert math.sqrt(far / norm) < 64 * 2.0**-24 + 2.0**-20
 
 
+@pytest.mark.parametrize("t", [1, 16])
+@pytest.mark.parametrize("grows", [False, True])
+def test_every_count_of_tiles(t, grows):
+    """One to sixteen tiles of 128 keys in one CTA's hands (a sequence each), the scores
+    growing from tile to tile or not: sums that are moved and rescaled."""
+    b, sm = 150, 128**-0.5
+    x = make(b, t, 8, 1, 2048, seed=60 + t)
+    if grows:
+        x["k_scale"] *= 1.0 + 0.5 * (torch.arange(2048, device="cuda") // 128)
+    for tiles in range(1, 17):
+        out = run(x, [tiles * 128 - t] * b, sm=sm)
+        for i in (0, 77, 149):
+            check({k: v[i:i + 1] for k, v in x.items()}, [tiles * 128 - t], None, None,
+                  out[i:i + 1], sm)
+
+
 @pytest.mark.parametrize("std,sm", [(0.01, 1.0), (6.0, 0.3), (1.5, 0.0)])
 def test_flat_and_peaked_scores(std, sm):
     x = make(2, 6, 8, 2, 400, seed=11, std=std)
