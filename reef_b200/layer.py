@@ -194,28 +194,34 @@ class LlamaLayer:
         """The decode step on drafted tokens: x [batch * drafts][hidden], row b *
         drafts + t the drafted token t of sequence b (the root first), appended to
         `cache` behind the lens [batch] committed rows; trees as in
-        kernels.tree_attn_i8.  kernels.kv_compact_i8 then keeps a path."""
-        if getattr(self, "_tiles", None) is None:
+        kernels.tree_attn_i8.  kernels.kv_compact_i8 then keeps a path.  The layer's
+        calls share its workspace, captured ones too: one at a time."""
+        dev, f32 = self.w_qkv.device, torch.float32
+        if getattr(self, "_tiles", None) is None and not torch.cuda.is_current_stream_capturing():
+            # (a capture would only record the packing, and other streams may call next)
             self._decode_tiles()
+            torch.cuda.current_stream(dev).synchronize()
         if x.shape[0] % self.batch != 0:
             raise ValueError("x must hold the same number of rows for every sequence")
-        drafts, max_len, dev = x.shape[0] // self.batch, cache["max_len"], x.device
-        ws = getattr(self, "_verify_ws", None)
-        if ws is None or self._verify_for != (drafts, max_len):
+        drafts, max_len = x.shape[0] // self.batch, cache["max_len"]
+        # (kept for good: a captured call goes on using its own)
+        kept = self.__dict__.setdefault("_verify_ws", {})
+        ws = kept.get((drafts, max_len))
+        if ws is None:
             n = _lib.lib().reef_b200_llama_verify_workspace_bytes(C.byref(self.desc), drafts,
                                                                   max_len)
             if n == 0:
                 raise ValueError("invalid description of a pass over drafted tokens")
-            self._verify_ws = ws = torch.empty(n, dtype=torch.uint8, device=dev)
-            self._verify_for = (drafts, max_len)
+            ws = kept[drafts, max_len] = torch.empty(n, dtype=torch.uint8, device=dev)
+        rows, tree = (x.shape[0], self.attn_norm.numel()), (self.batch, drafts)
         y = torch.empty_like(x) if out is None else out
-        tree = (self.batch, drafts)
-        _lib.call("reef_b200_llama_verify_forward", C.byref(self.desc), drafts, x.data_ptr(),
-                  y.data_ptr(), K._take(lens, "lens", torch.int32, tree[:1], dev),
-                  K._take(draft_lens, "draft_lens", torch.int32, tree[:1], dev),
-                  K._take(parents, "parents", torch.int32, tree, dev), cache["k"].data_ptr(),
-                  cache["ks"].data_ptr(), cache["v"].data_ptr(), cache["vs"].data_ptr(), max_len,
-                  ws.data_ptr(), ws.numel(), torch.cuda.current_stream(dev).cuda_stream)
+        K._call_on(dev, "reef_b200_llama_verify_forward", C.byref(self.desc), drafts,
+                   K._take(x, "x", f32, rows, dev), K._take(y, "out", f32, rows, dev),
+                   K._take(lens, "lens", torch.int32, tree[:1], dev),
+                   K._take(draft_lens, "draft_lens", torch.int32, tree[:1], dev),
+                   K._take(parents, "parents", torch.int32, tree, dev), cache["k"].data_ptr(),
+                   cache["ks"].data_ptr(), cache["v"].data_ptr(), cache["vs"].data_ptr(), max_len,
+                   ws.data_ptr(), ws.numel())
         return y
 
     def host_weights(self) -> dict:

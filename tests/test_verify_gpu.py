@@ -136,6 +136,25 @@ def test_captured_and_replayed():
     assert torch.equal(y, want)
 
 
+def test_a_capture_as_the_first_call_and_other_drafts_between_replays():
+    """Nothing that a captured call uses goes away or is still to be made."""
+    lens = i32([9, 33])
+    layer, other = (RL.LlamaLayer(SHAPE, 2, 8, seed=8) for _ in range(2))
+    cache = history(other, [9, 33], 64, 6)
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    x, x2 = (torch.randn((n, 512), device="cuda", generator=gen) for n in (10, 6))
+    want, want2 = (other.verify(v, lens, cache).clone() for v in (x, x2))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = layer.verify(x, lens, cache)
+    assert torch.equal(layer.verify(x2, lens, cache), want2)
+    assert torch.equal(layer.verify(x2, lens, cache | {"max_len": 64}), want2)
+    junk = [torch.full((1 << 20,), 0xff, dtype=torch.uint8, device="cuda") for _ in range(64)]
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want) and all(int(j[0]) == 0xff for j in junk)
+
+
 def test_refusals():
     layer = RL.LlamaLayer(SHAPE, 2, 8, seed=8)
     cache = layer.alloc_cache(64)
@@ -146,6 +165,12 @@ def test_refusals():
         layer.verify(torch.zeros((130, 512), device="cuda"), i32([1, 1]), cache)  # 65 drafts
     with pytest.raises(ValueError, match="lens"):
         layer.verify(x, i32([1, 1, 1]), cache)
+    with pytest.raises(ValueError, match="x must be"):
+        layer.verify(torch.zeros((4, 256), device="cuda"), i32([1, 1]), cache)
+    with pytest.raises(TypeError, match="x must be"):
+        layer.verify(x.half(), i32([1, 1]), cache)
+    with pytest.raises(ValueError, match="out must be"):
+        layer.verify(x, i32([1, 1]), cache, out=x[:2])
     with pytest.raises(ValueError, match="drafted tokens"):
         layer.verify(x, i32([1, 1]), layer.alloc_cache(62))
 
