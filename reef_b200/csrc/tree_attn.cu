@@ -751,6 +751,7 @@ __device__ __forceinline__ void next_piece(const int* pre, int batch, int per_se
   if (left > 0) next_unit(pre, batch, per_seq, at);
 }
 
+template <int kCopies>
 __global__ void __launch_bounds__(kCThreads, 1)
     tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
                    const __grid_constant__ CUtensorMap vmap, TreeArgs a) {
@@ -942,9 +943,13 @@ __global__ void __launch_bounds__(kCThreads, 1)
     }
   } else {
     setmaxnreg_inc<kRegsSoftmax>();
-    // ---------------- softmax: thread (x, t) has keys [kCols x, + kCols) of query row t ----------------
+    // -------- softmax: thread (x, t) has query row t % kRows and kKeys keys of every tile
+    constexpr int kRows = kTcRows / kCopies;   // query rows of the tile
+    constexpr int kKeys = kCols / kCopies;     // a thread's keys: every copy takes its own
+    constexpr int kLaneKeys = kKeys < 32 ? 1 : kKeys / 32;  // of which a lane stages the scales
     const int x = (warp - 8) >> 2;
     const int t = (warp & 3) * 32 + lane;  // == TMEM lane
+    const int tr = t % kRows, chunk = t / kRows * kParts + x;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     float* scw0 = reinterpret_cast<float*>(sm + CL::kScales) + (warp - 8) * 3 * kCols;  // of 2
     float* ml = reinterpret_cast<float*>(sm + CL::kML);  // [2][kParts][128]
@@ -967,7 +972,7 @@ __global__ void __launch_bounds__(kCThreads, 1)
       const int len = a.lens[b];
       bool bad;
       const int d = drafts_of(a, b, len, &bad);
-      const int r = (at.hq % a.qtiles) * kTcRows + t;  // query row of the KV head
+      const int r = (at.hq % a.qtiles) * kTcRows + tr;  // query row of the KV head
       const bool live = r < d * a.group;
       const int node = r / a.group;
       // row of q8, q_scale and out
@@ -1009,17 +1014,16 @@ __global__ void __launch_bounds__(kCThreads, 1)
       // a warp without a live row (as its partners in the other parts) only keeps
       // the barriers going
       const bool idle = !__any_sync(0xffffffffu, live);
-      const int keys0 = at.tile * kTileKeys + kCols * x;  // this part's first key
+      const int keys0 = at.tile * kTileKeys + kKeys * chunk;  // this part's first key
       const float* ksp = a.k_scale + (static_cast<long long>(b) * a.heads_kv + hkv) * a.max_len;
       const float* vsp = a.v_scale + (ksp - a.k_scale);
-      float nk[2], nv[2];
-      static_assert(kCols == 64, "a lane stages two keys");
+      float nk[kLaneKeys], nv[kLaneKeys];
       // loads this lane's keys of tile i (past the cache's end, where nobody looks,
       // the last one's: without a branch, the loads run on)
       auto scales = [&](int i) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int key = min(keys0 + i * kTileKeys + 32 * k + lane, a.max_len - 1);
+        for (int k = 0; k < kLaneKeys; ++k) {
+          const int key = min(keys0 + i * kTileKeys + 32 * k + lane % kKeys, a.max_len - 1);
           nk[k] = load_now(ksp + key);
           nv[k] = load_now(vsp + key);
         }
@@ -1027,15 +1031,17 @@ __global__ void __launch_bounds__(kCThreads, 1)
       auto stage = [&](int n) {  // and hands them to the warp, as the n-th tile's
         float* scw = scw0 + (n & 1) * (kSoftmax / 32 * 3 * kCols);
         __syncwarp();
+        if (kKeys >= 32 || lane < kKeys) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          scw[32 * k + lane] = nk[k];
-          scw[kCols + 32 * k + lane] = scale_log2(nv[k]);
-          scw[2 * kCols + 32 * k + lane] = scale_rcp(nv[k]);
+          for (int k = 0; k < kLaneKeys; ++k) {
+            scw[32 * k + lane] = nk[k];
+            scw[kCols + 32 * k + lane] = scale_log2(nv[k]);
+            scw[2 * kCols + 32 * k + lane] = scale_rcp(nv[k]);
+          }
         }
         __syncwarp();
       };
-      f32x2 s[kCols / 2];
+      f32x2 s[kKeys / 2];
       const f32x2 lift = pack2(-12582912.0f, -12582912.0f), am = pack2(amul, amul);
       float mt0, mt1;
       // scores of 16 keys (chunk h of tile i, the n-th) in log2 units, with the key's
@@ -1104,13 +1110,13 @@ __global__ void __launch_bounds__(kCThreads, 1)
           mt0 = mt1 = -INFINITY;
           wait_s(tc);
           if (!idle) {
-            uint32_t acc[4][16];
+            uint32_t acc[kKeys / 16][16];
 #pragma unroll
-            for (int h = 0; h < kCols / 16; ++h)
-              tmem_ld_32x32b_x16(tSx + x * kCols + h * 16, acc[h]);
+            for (int h = 0; h < kKeys / 16; ++h)
+              tmem_ld_32x32b_x16(tSx + chunk * kKeys + h * 16, acc[h]);
             tmem_ld_wait();
 #pragma unroll
-            for (int h = 0; h < kCols / 16; ++h) scores(i, tc, h, acc[h]);
+            for (int h = 0; h < kKeys / 16; ++h) scores(i, tc, h, acc[h]);
           }
           // the other parts' maxima; after the barrier every part's scores are in
           // registers, so P' may overwrite them
@@ -1120,7 +1126,8 @@ __global__ void __launch_bounds__(kCThreads, 1)
           named_barrier(1, kSoftmax);
           if (!idle) {
 #pragma unroll
-            for (int k = 0; k < kParts; ++k) mt = fmaxf(mt, mrow[k * 128 + t]);
+            for (int k = 0; k < kParts * kCopies; ++k)
+              mt = fmaxf(mt, mrow[k % kParts * 128 + k / kParts * kRows + tr]);
             // The rescale is warp-collective, so the warp decides (and its partners
             // alike): when any row passes its maximum, every row moves to its own.
             float alpha = 1.0f;
@@ -1138,7 +1145,7 @@ __global__ void __launch_bounds__(kCThreads, 1)
                 scw0 + (tc & 1) * (kSoftmax / 32 * 3 * kCols) + 2 * kCols);
             f32x2 ls0 = 0, ls1 = 0;  // (0.0f, 0.0f)
 #pragma unroll
-            for (int h = 0; h < kCols / 16; ++h) {  // 16 keys: 8 columns of heads, 8 of rests
+            for (int h = 0; h < kKeys / 16; ++h) {  // 16 keys: 8 columns of heads, 8 of rests
               uint32_t hi[8], lo[8];
               f32x2 p[8], rv[8];
               float f0[8], f1[8];
@@ -1167,8 +1174,16 @@ __global__ void __launch_bounds__(kCThreads, 1)
               }
 #pragma unroll
               for (int e = 0; e < 8; ++e) lo[e] = rest_of(f0[e], f1[e], hi[e]);
-              tmem_st_32x32b_x8(tSx + x * (kCols / 2) + h * 8, hi);
-              tmem_st_32x32b_x8(tSx + 64 + x * (kCols / 2) + h * 8, lo);
+              tmem_st_32x32b_x8(tSx + chunk * (kKeys / 2) + h * 8, hi);
+              tmem_st_32x32b_x8(tSx + 64 + chunk * (kKeys / 2) + h * 8, lo);
+            }
+            if constexpr (kCopies > 1) {  // P' of the other copies' keys: heads or rests
+              const uint32_t zeros[16] = {};
+#pragma unroll
+              for (int k = 1; k < kCopies; ++k)
+#pragma unroll
+                for (int h = 0; h < kKeys; h += 16)
+                  tmem_st_32x32b_x16(tSx + 64 * x + (t / kRows + k) % kCopies * kKeys + h, zeros);
             }
             {
               float f0, f1;
@@ -1236,7 +1251,8 @@ __global__ void __launch_bounds__(kCThreads, 1)
       tc_fence_after();
       float lsum = 0.0f;
 #pragma unroll
-      for (int k = 0; k < kParts; ++k) lsum += lrow[k * 128 + t];
+      for (int k = 0; k < kParts * kCopies; ++k)
+        lsum += lrow[k % kParts * 128 + k / kParts * kRows + tr];
       const int home = take_back(keep + 5 * kNext), cut = take_back(keep + 6 * kNext);
       at = Place{take_back(keep), take_back(keep + kNext), take_back(keep + 2 * kNext),
                  take_back(keep + 3 * kNext)};
@@ -1251,36 +1267,79 @@ __global__ void __launch_bounds__(kCThreads, 1)
       float* part = a.part + (static_cast<long long>(cta) * 2 + (cut_before ? 0 : 1)) * kTcRows *
                                  kPartRow;
       float4* stg = reinterpret_cast<float4*>(sm + CL::kQ + (warp - 8) * 2048);  // [32 rows][4]
-      if (!idle) {
-        const uint32_t from = w.n > kFlush + 1 ? tSum : tO;
-        const float scale = whole ? 1.0f / lsum : 1.0f;
-        const int dst_row = home < 0 ? -1 : whole ? home : t;  // row of out or of the partial
+      const uint32_t from = w.n > kFlush + 1 ? tSum : tO;
+      if constexpr (kCopies == 1) {
+        if (!idle) {
+          const float scale = whole ? 1.0f / lsum : 1.0f;
+          const int dst_row = home < 0 ? -1 : whole ? home : t;  // row of out or of the partial
+#pragma unroll 1
+          for (int c = 8 / kParts * x; c < 8 / kParts * (x + 1); ++c) {
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(from + lane_off + c * 16, o);
+            tmem_ld_wait();
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              stg[lane * 4 + (e ^ ((lane >> 1) & 3))] = make_float4(
+                  __uint_as_float(o[4 * e]) * scale, __uint_as_float(o[4 * e + 1]) * scale,
+                  __uint_as_float(o[4 * e + 2]) * scale, __uint_as_float(o[4 * e + 3]) * scale);
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int row = 8 * k + (lane >> 2), e = lane & 3;
+              const int to = __shfl_sync(0xffffffffu, dst_row, row);
+              const float4 v = stg[row * 4 + (e ^ ((row >> 1) & 3))];
+              if (to >= 0) {
+                float* dst = whole ? a.out + static_cast<long long>(to) * 128
+                                   : part + static_cast<long long>(to) * kPartRow + 4;
+                *reinterpret_cast<float4*>(dst + c * 16 + 4 * e) = v;
+              }
+            }
+          }
+        }
+      } else {
+        // The copies' sums are one another's rest: all stage their 16 columns, then
+        // every warp adds up kRows / 4 rows.
+        constexpr int kOwn = kRows / 4;
+        const uint32_t rows = smem_u32(sm + CL::kKeep) + 5 * kNext;  // `home` of row 0
 #pragma unroll 1
         for (int c = 8 / kParts * x; c < 8 / kParts * (x + 1); ++c) {
           uint32_t o[16];
           tmem_ld_32x32b_x16(from + lane_off + c * 16, o);
           tmem_ld_wait();
-          __syncwarp();
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            stg[lane * 4 + (e ^ ((lane >> 1) & 3))] = make_float4(
-                __uint_as_float(o[4 * e]) * scale, __uint_as_float(o[4 * e + 1]) * scale,
-                __uint_as_float(o[4 * e + 2]) * scale, __uint_as_float(o[4 * e + 3]) * scale);
-          __syncwarp();
+            stg[lane * 4 + (e ^ ((lane >> 1) & 3))] =
+                make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
+                            __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+          named_barrier(1, kSoftmax);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int row = 8 * k + (lane >> 2), e = lane & 3;
-            const int to = __shfl_sync(0xffffffffu, dst_row, row);
-            const float4 v = stg[row * 4 + (e ^ ((row >> 1) & 3))];
+          for (int k = 0; k < kOwn / 8; ++k) {
+            const int row = (warp & 3) * kOwn + 8 * k + (lane >> 2), e = lane & 3;
+            const int to = take_back(rows + row * 4);
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float all = 0.0f;
+#pragma unroll
+            for (int q = 0; q < kCopies; ++q) {
+              const int src = q * kRows + row;  // its lane
+              const float4 p = reinterpret_cast<const float4*>(
+                  sm + CL::kQ + (4 * x + (src >> 5)) * 2048)[(src & 31) * 4 + (e ^ ((src >> 1) & 3))];
+              v = make_float4(v.x + p.x, v.y + p.y, v.z + p.z, v.w + p.w);
+#pragma unroll
+              for (int h = 0; h < kParts; ++h) all += lrow[h * 128 + src];
+            }
             if (to >= 0) {
+              const float scale = whole ? 1.0f / all : 1.0f;
               float* dst = whole ? a.out + static_cast<long long>(to) * 128
-                                 : part + static_cast<long long>(to) * kPartRow + 4;
-              *reinterpret_cast<float4*>(dst + c * 16 + 4 * e) = v;
+                                 : part + static_cast<long long>(row) * kPartRow + 4;
+              *reinterpret_cast<float4*>(dst + c * 16 + 4 * e) =
+                  make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale);
             }
           }
+          named_barrier(1, kSoftmax);
         }
       }
-      if (!whole && x == 0) {
+      if (!whole && x == 0 && t < kRows) {
         part[t * kPartRow] = m;
         part[t * kPartRow + 1] = lsum;
       }
@@ -1389,8 +1448,9 @@ int launch_tree(void (*kernel)(CUtensorMap, CUtensorMap, TreeArgs), int threads,
     return rc;
   if (a.per_cta) return kOk;
   PdlScope pdl;
-  return launch_k(tree_join_kernel, dim3(static_cast<unsigned>(a.ctas), tile_rows / 8), dim3(256),
-                  0, st, a, tile_rows);
+  return launch_k(tree_join_kernel,
+                  dim3(static_cast<unsigned>(a.ctas), std::min(tile_rows, (a.rows + 7) / 8 * 8) / 8),
+                  dim3(256), 0, st, a, tile_rows);
 }
 
 // The kernels' shared memory, asked for once per device.
@@ -1402,7 +1462,9 @@ bool opt_in() {
     const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
     done[dev] = cudaFuncSetAttribute(tree_mma_kernel<1, 3, 2>, attr, TLayout<3>::kBytes) == cudaSuccess &&
                 cudaFuncSetAttribute(tree_mma_kernel<2, 6, 1>, attr, TLayout<6>::kBytes) == cudaSuccess &&
-                cudaFuncSetAttribute(tree_tc_kernel, attr, CL::kBytes) == cudaSuccess;
+                cudaFuncSetAttribute(tree_tc_kernel<4>, attr, CL::kBytes) == cudaSuccess &&
+                cudaFuncSetAttribute(tree_tc_kernel<2>, attr, CL::kBytes) == cudaSuccess &&
+                cudaFuncSetAttribute(tree_tc_kernel<1>, attr, CL::kBytes) == cudaSuccess;
   }
   return done[dev];
 }
@@ -1451,7 +1513,11 @@ int tree_attn_i8(const TreeProblem& p, cudaStream_t st) {
     return launch_tree(tree_mma_kernel<1, 3, 2>, kTThreads, TLayout<3>::kBytes, 2, 8, 4, km, vm, a, st);
   if (a.rows <= 16)
     return launch_tree(tree_mma_kernel<2, 6, 1>, kTThreads, TLayout<6>::kBytes, 1, 16, 4, km, vm, a, st);
-  return launch_tree(tree_tc_kernel, kCThreads, CL::kBytes, 1, kTcRows, 2, km, vm, a, st);
+  if (a.rows <= 32)
+    return launch_tree(tree_tc_kernel<4>, kCThreads, CL::kBytes, 1, kTcRows, 2, km, vm, a, st);
+  if (a.rows <= 64)
+    return launch_tree(tree_tc_kernel<2>, kCThreads, CL::kBytes, 1, kTcRows, 2, km, vm, a, st);
+  return launch_tree(tree_tc_kernel<1>, kCThreads, CL::kBytes, 1, kTcRows, 2, km, vm, a, st);
 }
 
 }  // namespace reef
