@@ -684,7 +684,7 @@ constexpr int kCThreads = 256 + kSoftmax;  // and the control and converter warp
 constexpr uint32_t kRegsControl = 72, kRegsConvert = 88, kRegsSoftmax = 176;
 static_assert(kRegsControl + kRegsConvert + kParts * kRegsSoftmax <= 65536 / 128,
               "register split exceeds the launch allocation");
-constexpr int kFlush = 6;       // tiles (and one more at the end) that O adds up
+constexpr int kFlushTiles = 6;  // tiles (and one more at the end) whose adds O takes
 constexpr int kKStages = 4;     // K tiles in flight (int8, 16 KiB)
 constexpr int kVStages = 3;     // V tiles in flight (the same)
 
@@ -755,6 +755,8 @@ template <int kCopies>
 __global__ void __launch_bounds__(kCThreads, 1)
     tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
                    const __grid_constant__ CUtensorMap vmap, TreeArgs a) {
+  // (each copy takes its share of a tile's; adding zeros loses nothing)
+  constexpr int kFlush = kFlushTiles * kCopies;
   extern __shared__ uint8_t sm_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) &
                                            ~static_cast<uintptr_t>(1023));
