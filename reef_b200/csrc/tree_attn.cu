@@ -407,12 +407,37 @@ __global__ void __launch_bounds__(kTThreads, kPerSm)
     if (j == 0 || at.tile == 0) {  // a new segment: its tree, q, a fresh state
       const int hkv = at.hq / a.qtiles;
       row0 = (at.hq % a.qtiles) * kRows;
+      qbase = static_cast<long long>(at.b) * a.drafts * a.heads_q + hkv * a.group;
+      // every load at once (all drafts' rows are there, whoever is live): one round trip
       len = a.lens[at.b];
+      int up = 0;
+      if (a.parents != nullptr && tid < a.drafts)
+        up = a.parents[static_cast<long long>(at.b) * a.drafts + tid];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int r = row0 + nt * 8 + g;
+        const uint32_t* q32 =
+            reinterpret_cast<const uint32_t*>(a.q8) + (r < a.rows ? qrow(r) * 32 : 0);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          qb[ks][nt][0] = q32[8 * ks + tig];
+          qb[ks][nt][1] = q32[8 * ks + 4 + tig];
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int rc = row0 + nt * 8 + 2 * tig + e;
+          qsc[nt][e] = a.q_scale[rc < a.rows ? qrow(rc) : 0];
+          m[nt][e] = -INFINITY;
+          l[nt][e] = 0.0f;
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[c][nt][e] = 0.0f;
+      }
       bool bad;
       d = drafts_of(a, at.b, len, &bad);
-      qbase = static_cast<long long>(at.b) * a.drafts * a.heads_q + hkv * a.group;
-      if (a.parents != nullptr && tid < d)
-        par[tid] = a.parents[static_cast<long long>(at.b) * a.drafts + tid];
+      if (tid < a.drafts) par[tid] = up;
       __syncthreads();
       if (tid < d) {
         unsigned long long bits = (2ull << tid) - 1;  // a chain
@@ -429,24 +454,12 @@ __global__ void __launch_bounds__(kTThreads, kPerSm)
       const int live = d * a.group;  // rows past it are computed as zeros
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const int r = row0 + nt * 8 + g;
-        const uint32_t* q32 = reinterpret_cast<const uint32_t*>(a.q8) + (r < live ? qrow(r) * 32 : 0);
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          qb[ks][nt][0] = r < live ? q32[8 * ks + tig] : 0u;
-          qb[ks][nt][1] = r < live ? q32[8 * ks + 4 + tig] : 0u;
-        }
+        for (int ks = 0; ks < 4; ++ks)
+          if (row0 + nt * 8 + g >= live) qb[ks][nt][0] = qb[ks][nt][1] = 0u;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int rc = row0 + nt * 8 + 2 * tig + e;
-          qsc[nt][e] = rc < live ? a.q_scale[qrow(rc)] * base : 0.0f;
-          m[nt][e] = -INFINITY;
-          l[nt][e] = 0.0f;
-        }
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[c][nt][e] = 0.0f;
+        for (int e = 0; e < 2; ++e)
+          qsc[nt][e] = row0 + nt * 8 + 2 * tig + e < live ? qsc[nt][e] * base : 0.0f;
       }
       __syncthreads();  // anc is in
     }
@@ -970,33 +983,54 @@ __global__ void __launch_bounds__(kCThreads, 1)
       put_aside(keep + 2 * kNext, at.tile);
       put_aside(keep + 3 * kNext, at.tiles);
       put_aside(keep + 4 * kNext, left);
+      // every load at once (all drafts' rows are there, whoever is live): one round trip
       const int b = at.b, hkv = at.hq / a.qtiles;
       const int len = a.lens[b];
-      bool bad;
-      const int d = drafts_of(a, b, len, &bad);
       const int r = (at.hq % a.qtiles) * kTcRows + tr;  // query row of the KV head
-      const bool live = r < d * a.group;
       const int node = r / a.group;
       // row of q8, q_scale and out
       const int qrow = (b * a.drafts + node) * a.heads_q + hkv * a.group + (r - node * a.group);
       const int mine = tid - 256;
-      const bool parent = a.parents != nullptr && mine < d;
       int up = 0;
-      if (parent) up = a.parents[static_cast<long long>(b) * a.drafts + mine];
-      put_aside(keep + 5 * kNext, live ? qrow : -1);
+      if (a.parents != nullptr && mine < a.drafts)
+        up = a.parents[static_cast<long long>(b) * a.drafts + mine];
+      uint4 v[8 / kParts];  // this part of the row of Q
       float amul = 0.0f;
-      {  // this part of the row of Q
-        uint8_t* q = sm + CL::kQ + t * 128;
-        uint4 v[8 / kParts];
+      {
         const uint4* src = reinterpret_cast<const uint4*>(a.q8) + static_cast<long long>(qrow) * 8 +
                            8 / kParts * x;
+        const bool there = r < a.rows;
 #pragma unroll
-        for (int c = 0; c < 8 / kParts; ++c) v[c] = live ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
-        if (live) amul = a.q_scale[qrow] * base;
-        if (parent) par[mine] = up;
+        for (int c = 0; c < 8 / kParts; ++c) v[c] = there ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+        if (there) amul = a.q_scale[qrow];
+      }
+      const int keys0 = at.tile * kTileKeys + kKeys * chunk;  // this part's first key
+      const float* ksp = a.k_scale + (static_cast<long long>(b) * a.heads_kv + hkv) * a.max_len;
+      const float* vsp = a.v_scale + (ksp - a.k_scale);
+      float nk[kLaneKeys], nv[kLaneKeys];
+      // loads this lane's keys of tile i (past the cache's end, where nobody looks,
+      // the last one's: without a branch, the loads run on)
+      auto scales = [&](int i) {
+#pragma unroll
+        for (int k = 0; k < kLaneKeys; ++k) {
+          const int key = min(keys0 + i * kTileKeys + 32 * k + lane % kKeys, a.max_len - 1);
+          nk[k] = load_now(ksp + key);
+          nv[k] = load_now(vsp + key);
+        }
+      };
+      scales(0);
+      bool bad;
+      const int d = drafts_of(a, b, len, &bad);
+      const bool live = r < d * a.group;
+      put_aside(keep + 5 * kNext, live ? qrow : -1);
+      amul = live ? amul * base : 0.0f;
+      if (mine < a.drafts) par[mine] = up;
+      {
+        uint8_t* q = sm + CL::kQ + t * 128;
 #pragma unroll
         for (int c = 0; c < 8 / kParts; ++c)
-          *reinterpret_cast<uint4*>(q + (((c + 8 / kParts * x) ^ (t & 7)) << 4)) = v[c];
+          *reinterpret_cast<uint4*>(q + (((c + 8 / kParts * x) ^ (t & 7)) << 4)) =
+              live ? v[c] : make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();
         mbar_arrive(q_full);
       }
@@ -1016,20 +1050,6 @@ __global__ void __launch_bounds__(kCThreads, 1)
       // a warp without a live row (as its partners in the other parts) only keeps
       // the barriers going
       const bool idle = !__any_sync(0xffffffffu, live);
-      const int keys0 = at.tile * kTileKeys + kKeys * chunk;  // this part's first key
-      const float* ksp = a.k_scale + (static_cast<long long>(b) * a.heads_kv + hkv) * a.max_len;
-      const float* vsp = a.v_scale + (ksp - a.k_scale);
-      float nk[kLaneKeys], nv[kLaneKeys];
-      // loads this lane's keys of tile i (past the cache's end, where nobody looks,
-      // the last one's: without a branch, the loads run on)
-      auto scales = [&](int i) {
-#pragma unroll
-        for (int k = 0; k < kLaneKeys; ++k) {
-          const int key = min(keys0 + i * kTileKeys + 32 * k + lane % kKeys, a.max_len - 1);
-          nk[k] = load_now(ksp + key);
-          nv[k] = load_now(vsp + key);
-        }
-      };
       auto stage = [&](int n) {  // and hands them to the warp, as the n-th tile's
         float* scw = scw0 + (n & 1) * (kSoftmax / 32 * 3 * kCols);
         __syncwarp();
@@ -1099,7 +1119,6 @@ __global__ void __launch_bounds__(kCThreads, 1)
         ok = __all_sync(0xffffffffu, ok);  // reconverge before warp-collective tcgen05.ld
         tc_fence_after();
       };
-      scales(0);
       float m = -INFINITY, l = 0.0f;
       float carry = 1.0f;  // the second accumulator's scale to the new maxima
       int i = 0, flush = kFlush;  // the tile, and the one before whose product O is moved
@@ -1303,7 +1322,18 @@ __global__ void __launch_bounds__(kCThreads, 1)
         // The copies' sums are one another's rest: all stage their 16 columns, then
         // every warp adds up kRows / 4 rows.
         constexpr int kOwn = kRows / 4;
-        const uint32_t rows = smem_u32(sm + CL::kKeep) + 5 * kNext;  // `home` of row 0
+        const int row0 = (warp & 3) * kOwn + (lane >> 2), e4 = lane & 3;
+        int to[kOwn / 8];        // rows of out, or -1
+        float scale[kOwn / 8];
+#pragma unroll
+        for (int k = 0; k < kOwn / 8; ++k) {
+          to[k] = take_back(smem_u32(sm + CL::kKeep) + 5 * kNext + (row0 + 8 * k) * 4);
+          float all = 0.0f;
+#pragma unroll
+          for (int q = 0; q < kParts * kCopies; ++q)
+            all += lrow[q % kParts * 128 + q / kParts * kRows + row0 + 8 * k];
+          scale[k] = whole ? 1.0f / all : 1.0f;
+        }
 #pragma unroll 1
         for (int c = 8 / kParts * x; c < 8 / kParts * (x + 1); ++c) {
           uint32_t o[16];
@@ -1317,25 +1347,19 @@ __global__ void __launch_bounds__(kCThreads, 1)
           named_barrier(1, kSoftmax);
 #pragma unroll
           for (int k = 0; k < kOwn / 8; ++k) {
-            const int row = (warp & 3) * kOwn + 8 * k + (lane >> 2), e = lane & 3;
-            const int to = take_back(rows + row * 4);
             float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            float all = 0.0f;
 #pragma unroll
             for (int q = 0; q < kCopies; ++q) {
-              const int src = q * kRows + row;  // its lane
+              const int src = q * kRows + row0 + 8 * k;  // its lane
               const float4 p = reinterpret_cast<const float4*>(
-                  sm + CL::kQ + (4 * x + (src >> 5)) * 2048)[(src & 31) * 4 + (e ^ ((src >> 1) & 3))];
+                  sm + CL::kQ + (4 * x + (src >> 5)) * 2048)[(src & 31) * 4 + (e4 ^ ((src >> 1) & 3))];
               v = make_float4(v.x + p.x, v.y + p.y, v.z + p.z, v.w + p.w);
-#pragma unroll
-              for (int h = 0; h < kParts; ++h) all += lrow[h * 128 + src];
             }
-            if (to >= 0) {
-              const float scale = whole ? 1.0f / all : 1.0f;
-              float* dst = whole ? a.out + static_cast<long long>(to) * 128
-                                 : part + static_cast<long long>(row) * kPartRow + 4;
-              *reinterpret_cast<float4*>(dst + c * 16 + 4 * e) =
-                  make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale);
+            if (to[k] >= 0) {
+              float* dst = whole ? a.out + static_cast<long long>(to[k]) * 128
+                                 : part + static_cast<long long>(row0 + 8 * k) * kPartRow + 4;
+              *reinterpret_cast<float4*>(dst + c * 16 + 4 * e4) =
+                  make_float4(v.x * scale[k], v.y * scale[k], v.z * scale[k], v.w * scale[k]);
             }
           }
           named_barrier(1, kSoftmax);
