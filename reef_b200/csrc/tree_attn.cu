@@ -253,11 +253,15 @@ __device__ __forceinline__ void count_tiles(const TreeArgs& a, int* pre, int* sc
   __syncthreads();
 }
 
+// What a segment's beginning and end take, in units: 3 measured best at 8 to 512
+// query rows (against none: 64 x 8 drafts over up to 4k keys 38.6 -> 37.1 us, 2 x 64 over
+// 16k 177 -> 173), 2 and 4 a little behind.
+constexpr int kCost = 3;
+
 // A unit's place: sequence, (KV head, tile of query rows), tile of keys.
 struct Place {
   int b, hq, tile, tiles;
 };
-__device__ __forceinline__ Place place_of(const int* pre, int batch, int per_seq, long long u);
 
 // The first unit of CTA `cta` and how many it has.  With a segment per CTA the
 // sequence's length alone says so; otherwise every sequence's does (count_tiles:
@@ -280,28 +284,43 @@ __device__ __forceinline__ Place share_of(const TreeArgs& a, int cta, int* pre, 
     return p;
   }
   count_tiles<kThreads>(a, pre, scratch);
-  const long long units = static_cast<long long>(pre[a.batch]) * per_seq;
-  const long long u0 = units * cta / a.ctas, u1 = units * (cta + 1) / a.ctas;
-  *nunits = static_cast<int>(u1 - u0);
-  if (*nunits > 0) p = place_of(pre, a.batch, per_seq, u0);
+  // Equal shares of a line on which kCost that stand for a segment's beginning come
+  // before its units.  An even lane looks for the share's first unit, an odd one for the
+  // next share's.
+  const int batch = a.batch, lane = threadIdx.x & 31;
+  const long long all = (static_cast<long long>(pre[batch]) + batch * kCost) * per_seq;
+  const long long v = all * (cta + (lane & 1)) / a.ctas;
+  int lo = 0, hi = batch - 1;  // the last sequence that begins at v or before
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if ((static_cast<long long>(pre[mid]) + mid * kCost) * per_seq <= v) lo = mid;
+    else hi = mid - 1;
+  }
+  const long long off = v - (static_cast<long long>(pre[lo]) + lo * kCost) * per_seq;
+  p.b = lo;
+  p.tiles = pre[lo + 1] - pre[lo];
+  const unsigned each = static_cast<unsigned>(p.tiles) + kCost;
+  p.hq = off >> 32 == 0 ? static_cast<int>(static_cast<unsigned>(off) / each)
+                        : static_cast<int>(off / each);
+  p.tile = max(0, static_cast<int>(off - static_cast<long long>(p.hq) * each) - kCost);
+  const long long before =
+      static_cast<long long>(pre[lo]) * per_seq + static_cast<long long>(p.hq) * p.tiles + p.tile;
+  *nunits = static_cast<int>(__shfl_sync(0xffffffffu, before, 1) -
+                             __shfl_sync(0xffffffffu, before, 0));
+  p.b = __shfl_sync(0xffffffffu, p.b, 0);
+  p.hq = __shfl_sync(0xffffffffu, p.hq, 0);
+  p.tile = __shfl_sync(0xffffffffu, p.tile, 0);
+  p.tiles = __shfl_sync(0xffffffffu, p.tiles, 0);
+  if (*nunits > 0 && p.tiles == 0) {  // the next sequence that has any
+    p.hq = p.tile = 0;
+    do {
+      ++p.b;
+      p.tiles = pre[p.b + 1] - pre[p.b];
+    } while (p.tiles == 0);
+  }
   return p;
 }
 
-__device__ __forceinline__ Place place_of(const int* pre, int batch, int per_seq, long long u) {
-  int lo = 0, hi = batch - 1;  // the last b with pre[b] * per_seq <= u and tiles
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (static_cast<long long>(pre[mid]) * per_seq <= u) lo = mid;
-    else hi = mid - 1;
-  }
-  Place p;
-  p.b = lo;
-  p.tiles = pre[lo + 1] - pre[lo];
-  const long long rem = u - static_cast<long long>(pre[lo]) * per_seq;
-  p.hq = static_cast<int>(rem / p.tiles);
-  p.tile = static_cast<int>(rem % p.tiles);
-  return p;
-}
 __device__ __forceinline__ void next_unit(const int* pre, int batch, int per_seq, Place& p) {
   if (++p.tile < p.tiles) return;
   p.tile = 0;
@@ -1536,9 +1555,11 @@ int tree_attn_i8(const TreeProblem& p, cudaStream_t st) {
     return rc;
   if (!opt_in()) return kErrCuda;
   if (a.rows <= 8)
-    return launch_tree(tree_mma_kernel<1, 3, 2>, kTThreads, TLayout<3>::kBytes, 2, 8, 4, km, vm, a, st);
+    return launch_tree(tree_mma_kernel<1, 3, 2>, kTThreads, TLayout<3>::kBytes, 2, 8, 4, km, vm, a,
+                       st);
   if (a.rows <= 16)
-    return launch_tree(tree_mma_kernel<2, 6, 1>, kTThreads, TLayout<6>::kBytes, 1, 16, 4, km, vm, a, st);
+    return launch_tree(tree_mma_kernel<2, 6, 1>, kTThreads, TLayout<6>::kBytes, 1, 16, 4, km, vm, a,
+                       st);
   if (a.rows <= 32)
     return launch_tree(tree_tc_kernel<4>, kCThreads, CL::kBytes, 1, kTcRows, 2, km, vm, a, st);
   if (a.rows <= 64)
