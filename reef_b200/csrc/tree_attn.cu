@@ -41,19 +41,25 @@
 // product takes B with the dims contiguous.  The tensor pipe truncates when it adds
 // to O (1.4e-5 of the result over 16k keys), so every six tiles O is added to a
 // second accumulator by the softmax threads, with rounding, and begins anew (5 of
-// 180 us over 16k keys).
+// 175 us over 16k keys).
 //
-// Measured (one call, cold cache): 4 drafts over 499 keys, 32 heads of their own, 8.9
-// us, which is the launch, one round trip and the join of nothing.  64 sequences of up
-// to 4096 keys, 8 heads on 1 (53.7 MB of cache): 1 draft each 29 us, 2 drafts 42, 8 drafts
-// 53; two sequences over 16301 keys, 64 drafts, 64 heads on 8 (68.5 Gflop): 177 us, 0.39
-// Pflop/s of products or 0.78 with the rests.  Both kernels are bound by the issue of
-// the softmax warps, two to a scheduler: about 17 instructions a score, 2 of which
-// the second f16 term costs (without it, 1.4e-4 of the result would be lost).  The
-// tensor pipe is busy 23 % of the time, MUFU 21 %, HBM 6 %.  Quarter rows in four
-// warpgroups do not fit the registers (they spill and are slower); scores taken a
-// tile ahead, a barrier per pair of warps and packed arithmetic throughout changed
-// nothing.
+// Up to 64 query rows (of a KV head), the tile of 128 holds them two or four times:
+// each copy takes its own keys of every tile of 128 and zeros for the others' P', so
+// that all warps have work (64 x 8 drafts, 8 heads on one: 53 -> 41 us); the copies share
+// the maxima and add up at the end.
+//
+// Measured (one call, cold cache): 4 drafts over 499 keys, 32 heads of their own, 8.7
+// us, which is the launch and three round trips (lengths, queries, keys).  64 sequences
+// over up to 4096 keys, 8 heads on one: 1 draft each (70 MB of cache) 26 us, 2 drafts 35, 8
+// drafts (ragged, 54 MB) 36, of which 12 are the shares, the first loads, the epilogues
+// and the join.  Two sequences over 16301 keys, 64 drafts, 64 heads on 8 (68.5 Gflop): 175
+// us, 0.39 Pflop/s of products or 0.78 with the rests; a tile takes 5000 cycles, of which
+// the tensor pipe is busy for 1550.  That is the issue of the softmax warps, two to a
+// scheduler, 17 instructions a score at one in 4.8 cycles each.  Up to 32 rows the
+// products bound (2500 cycles a tile).  Measured and dropped: quarter rows in four warpgroups
+// (they spill), scores taken a tile ahead, a barrier per pair of warps, scores in
+// fragments of 16 x 8 (a quarter of the loads of scales, and no faster), O moved by the
+// converters.
 #include "attn_mma.cuh"
 #include "common.cuh"
 #include "ops.h"
