@@ -730,8 +730,10 @@ struct CL {  // shared memory layout (bytes from a 1024-aligned base)
   static constexpr int kQ = 0;                            // int8 [128][128] SW128
   static constexpr int kK = 16384;                        // kKStages x 16 KiB
   static constexpr int kV = kK + kKStages * 16384;        // kVStages x 16 KiB
-  static constexpr int kVf = kV + kVStages * 16384;       // 2 x f16 [2 dim halves][128 keys][64] SW128
-  static constexpr int kScales = kVf + 2 * 32768;         // [2 tiles][warps][ks, log2 vs, 1 / vs][kCols]
+  // 2 x f16 [2 dim halves][128 keys][64] SW128
+  static constexpr int kVf = kV + kVStages * 16384;
+  // [2 tiles][warps][ks, log2 vs, 1 / vs][kCols]
+  static constexpr int kScales = kVf + 2 * 32768;
   static constexpr int kML = kScales + 2 * kSoftmax / 32 * 3 * kCols * 4;  // [2 tiles][parts][128]
   static constexpr int kPar = kML + 2 * kSoftmax * 4;         // int[64]
   static constexpr int kPre = kPar + kMaxDrafts * 4;      // int[batch + 1]
