@@ -634,32 +634,42 @@ __device__ __noinline__ bool select_near(const Ctx& ctx, const Row& row, Cut* cu
   __syncthreads();
   if (c.tid < c.ranks && c.tid != c.rank) c.of(c.tid)->near_n[c.rank] = s->near_n[c.rank];
   c.sync();
-  // thread t: the t-th of them
+  // side by side: the parts of several CTAs in `all` (which only a row that one CTA
+  // took over uses)
   bool fits = true;
-  int total = 0, e = -1;
+  int total = 0, mine = -1;
   for (int k = 0; k < c.ranks; ++k) {
     const int n = s->near_n[k];
     fits = fits && n <= room;
-    if (c.tid >= total && c.tid < total + n) e = k * room + c.tid - total;
+    if (c.tid >= total && c.tid < total + n) mine = k * room + c.tid - total;
     total += n;
   }
   if (!fits) return false;
-  float x = 0.0f;
-  int index = 0;
-  u64 w = 0;
-  if (e >= 0) {
-    x = s->near.x[e];
-    index = s->near.index[e];
-    w = kMass ? r.fixed(x) : 1ull;
-    s->near.w[e] = w;
+  const float* xs = c.ranks > 1 ? s->all.x : s->near.x;
+  const int* at = c.ranks > 1 ? s->all.index : s->near.index;
+  if (mine >= 0) {
+    const float x = s->near.x[mine];
+    s->near.w[c.tid] = kMass ? r.fixed(x) : 1ull;
+    if (c.ranks > 1) {
+      s->all.x[c.tid] = x;
+      s->all.index[c.tid] = s->near.index[mine];
+    }
   }
   __syncthreads();
-  if (e >= 0) {
-    u64 run = 0;  // what comes before it in the order
-    for (int k = 0; k < c.ranks; ++k)
-      for (int j = k * room; j < k * room + s->near_n[k]; ++j)
-        if (s->near.x[j] > x || (s->near.x[j] == x && s->near.index[j] < index)) run += s->near.w[j];
-    if (run < target && target <= run + w)
+  // what comes before each in the order, by as many neighbouring threads as there are
+  int each = 1;
+  while (each < 32 && 2 * each * total <= kThreads) each *= 2;
+  const int e = c.tid / each;
+  if (e - c.lane / each < total) {  // (whole warps)
+    const float x = e < total ? xs[e] : 0.0f;
+    const int index = e < total ? at[e] : 0;
+    u64 run = 0;
+    for (int j = c.tid % each; j < total; j += each) {
+      const float y = xs[j];
+      if (y > x || (y == x && at[j] < index)) run += s->near.w[j];
+    }
+    for (int o = 1; o < each; o *= 2) run += __shfl_xor_sync(0xffffffffu, run, o);
+    if (e < total && c.tid % each == 0 && run < target && target <= run + s->near.w[e])
       s->found = (static_cast<u64>(__float_as_uint(x)) << 32) | static_cast<uint32_t>(index);
   }
   __syncthreads();
