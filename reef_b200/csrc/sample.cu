@@ -43,14 +43,14 @@
 // takes its place.
 //
 // What bounds it: 131 MB of logits (256 rows of 128000) would take 20 us to read; no
-// filter takes 146 us, top-p 260.  Two CTAs of 512 threads fill an SM's
+// filter takes 141 us, top-p 246.  Two CTAs of 512 threads fill an SM's
 // shared memory and registers, and each row's chain is 15 to 35 us long: the copy and
 // the maximum 4, the weights 10 (50 instructions each where every second one is
 // heavy; with the histogram 15), then half a dozen steps of 1 to 4 us that end in a
 // cluster barrier.  A single row of 50257 with top-k: 14 us, all of it that chain.
-// Measured and dropped: four weights at a time before their adds (268 us),
-// two elements to an instruction (no change), the list weighed in a pass of its own
-// and the histogram in another (341).
+// Measured and dropped: two elements to an instruction (no change), the four adds of
+// a thread into the histogram in flight at once (3 % slower), the list weighed in a
+// pass of its own and the histogram in another (341).
 #include "common.cuh"
 #include "ops.h"
 
@@ -568,8 +568,8 @@ __device__ __forceinline__ bool histogram(const Ctx& c, const Row& r, BinOf bin_
 
 // The mass of a row that is plain: s->warp holds this CTA's per warp, slot the
 // cluster's per CTA, as after row_sum; with kHist also this CTA's histogram of the
-// elements from steps.least up.  A warp that has no heavy (no light) one among 32
-// neighbours leaves out what is for those.
+// elements from steps.least up.  A warp that has no heavy (no light) one among
+// 128 neighbours leaves out what is for those.
 template <bool kHist>
 __device__ __noinline__ u64 weigh(Ctx& ctx, const Row& row, const Steps& st, const u64** slot) {
   const Ctx c = ctx;
@@ -586,18 +586,25 @@ __device__ __noinline__ u64 weigh(Ctx& ctx, const Row& row, const Steps& st, con
   for (int i = i0; i < i1; i += 128) {
     const float4 v4 = c.four(r, i + 4 * c.lane, i1);
     const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+    const float hi = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+    const bool all4 = v[0] >= r.heavy && v[1] >= r.heavy && v[2] >= r.heavy && v[3] >= r.heavy;
+    u64 w[4] = {0, 0, 0, 0};
+    if (__any_sync(0xffffffffu, hi >= r.heavy)) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const bool heavy = v[e] >= r.heavy;
-      const unsigned ballot = __ballot_sync(0xffffffffu, heavy);
-      u64 w = 0;
-      if (ballot != 0) w = r.full(fmaxf(v[e], r.least));
-      if (ballot != 0xffffffffu) {
+      for (int e = 0; e < 4; ++e) w[e] = r.full(fmaxf(v[e], r.least));
+    }
+    if (!__all_sync(0xffffffffu, all4)) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
         const uint32_t l = r.light(v[e]);
-        w = heavy ? w : l;
+        w[e] = v[e] >= r.heavy ? w[e] : l;
       }
-      sum += w;
-      if (kHist && v[e] >= steps.least) add_mass(steps.bin(v[e]), w);
+    }
+    sum += (w[0] + w[1]) + (w[2] + w[3]);
+    if (kHist) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (v[e] >= steps.least) add_mass(steps.bin(v[e]), w[e]);
     }
   }
   *slot = ctx.exchange(block_sum(c, sum))[0];
