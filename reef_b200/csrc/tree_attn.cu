@@ -57,7 +57,8 @@
 // the tensor pipe is busy for 1550.  That is the issue of the softmax warps, two to a
 // scheduler, 17 instructions a score at one in 4.8 cycles each.  Up to 32 rows the
 // products bound (2500 cycles a tile).  Measured and dropped: quarter rows in four warpgroups
-// (they spill), scores taken a tile ahead, a barrier per pair of warps, scores in
+// (they spill; with two copies they do not, and 64 x 8 takes 42 us: what a warp does
+// once a tile counts twice as often), scores taken a tile ahead, a barrier per pair of warps, scores in
 // fragments of 16 x 8 (a quarter of the loads of scales, and no faster), O moved by the
 // converters.
 #include "attn_mma.cuh"

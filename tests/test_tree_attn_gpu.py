@@ -155,7 +155,7 @@ def test_long_rows_lose_nothing(t, hq):
     assert math.sqrt(far / norm) < 64 * 2.0**-24 + 2.0**-20
 
 
-@pytest.mark.parametrize("t", [1, 16])
+@pytest.mark.parametrize("t", [1, 2, 4, 8, 16])
 @pytest.mark.parametrize("grows", [False, True])
 def test_every_count_of_tiles(t, grows):
     """One to sixteen tiles of 128 keys in one CTA's hands (a sequence each), the scores
