@@ -112,13 +112,7 @@ struct alignas(16) Shared {
       int index[kGather];
     } all;
   };
-  union {
-    uint16_t list[kWarps][kList];  // elements of a warp's run, in index order
-    struct {                       // or the odd half of a count
-      u64 ahead[kFew];
-      int rank[kFew];
-    } sub;
-  };
+  uint16_t list[kWarps][kList];  // elements of a warp's run, in index order
   int listed[kWarps];
   int near_n[kMaxCluster];
   u64 slot[2][2][kMaxCluster];   // two values of every CTA
@@ -745,6 +739,13 @@ __device__ __noinline__ void select_radix(Ctx& c, const Row& r, Cut* cut_io, flo
   *cut_io = Cut{value, static_cast<int>(shared()->found)};
 }
 
+// A token's share of the kept mass: from the integer where it has 30 bits, else anew
+// (exp in double takes one thread a microsecond).
+__device__ __forceinline__ float share(const Row& r, float x, u64 w, u64 all) {
+  const double mine = w >> 30 != 0 ? static_cast<double>(w) : r.weight(x) * kOne;
+  return static_cast<float>(mine / static_cast<double>(all));
+}
+
 // u times the total, below it
 __device__ __forceinline__ u64 drawn(float u, u64 all) {
   const u64 at = u > 0.0f ? static_cast<u64>(fmin(static_cast<double>(u), 1.0) *
@@ -762,36 +763,47 @@ __device__ __forceinline__ void finish_few(const Ctx& c, const Row& r, int k, fl
                                            KeepsMin keeps_min, float u, uint32_t* index,
                                            float* prob) {
   Shared* s = shared();
-  // two threads to an element, for the even and the odd ones of the others
-  const int e = c.tid % kFew, half = c.tid / kFew;
+  // as many neighbouring threads to an element as there are, two at least, for a part
+  // of the others each
+  int each = 2;
+  while (each < 32 && 2 * each * c.gathered <= kThreads) each *= 2;
+  const int e = c.tid / each, part = c.tid % each;
   const bool have = e < c.gathered;
   const float x = have ? s->all.x[e] : 0.0f;
-  const int at = have ? s->all.index[e] : 0;
-  u64 w = have ? r.fixed(x) : 0ull;
-  if (half == 0) s->near.w[e] = w;
+  u64 w = have && part == 0 ? r.fixed(x) : 0ull;
+  if (have && part == 0) s->near.w[e] = w;
+  if (c.tid < 3) {  // (behind them, ahead of none)
+    s->all.x[c.gathered + c.tid] = -INFINITY;
+    s->near.w[c.gathered + c.tid] = 0;
+  }
   __syncthreads();
-  // the elements ahead in the order: how many, and their mass (they come before
-  // this one, so top-k keeps them if it keeps this one)
+  // the elements ahead in the order: how many, and for top-p their mass (they come
+  // before this one, so top-k keeps them if it keeps this one)
   int rank = 0;
   u64 ahead = 0;
-  if (have) {
-#pragma unroll 4
-    for (int j = half; j < c.gathered; j += kThreads / kFew) {
-      const float y = s->all.x[j];
-      const bool before = y > x || (y == x && j < e);
-      rank += before;
-      ahead += before ? s->near.w[j] : 0ull;
+  if (have && p < 1.0f) {
+    for (int j = 4 * part; j < c.gathered; j += 4 * each) {
+      const float4 y4 = *reinterpret_cast<const float4*>(&s->all.x[j]);
+      const float y[4] = {y4.x, y4.y, y4.z, y4.w};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const bool before = y[q] > x || (y[q] == x && j + q < e);
+        rank += before;
+        ahead += before ? s->near.w[j + q] : 0ull;
+      }
+    }
+  } else if (have && k > 0) {
+#pragma unroll 2
+    for (int j = 4 * part; j < c.gathered; j += 4 * each) {
+      const float4 y4 = *reinterpret_cast<const float4*>(&s->all.x[j]);
+      const float y[4] = {y4.x, y4.y, y4.z, y4.w};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) rank += y[q] > x || (y[q] == x && j + q < e);
     }
   }
-  if (half != 0) {
-    s->sub.ahead[e] = ahead;
-    s->sub.rank[e] = rank;
-    w = 0;
-  }
-  __syncthreads();
-  if (half == 0) {
-    ahead += s->sub.ahead[e];
-    rank += s->sub.rank[e];
+  for (int o = 1; o < each; o *= 2) {
+    rank += __shfl_xor_sync(0xffffffffu, rank, o);
+    if (p < 1.0f) ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
   }
   if (k > 0 && rank >= k) w = 0;
   const u64 mass = block_sum(c, w);
@@ -805,10 +817,10 @@ __device__ __forceinline__ void finish_few(const Ctx& c, const Row& r, int k, fl
   const u64 target = drawn(u, all);
   u64 run = warp_prefix(w, c.lane) - w;
   for (int i = 0; i < c.warp; ++i) run += s->warp[i];
-  if (run <= target && target < run + w) {  // (w is 0 in the second halves)
-    *index = static_cast<uint32_t>(at);
+  if (run <= target && target < run + w) {  // (w is 0 but in an element's first thread)
+    *index = static_cast<uint32_t>(s->all.index[e]);
     if (prob != nullptr)
-      *prob = static_cast<float>(r.weight(x) * kOne / static_cast<double>(all));
+      *prob = share(r, x, w, all);
   }
 }
 
@@ -875,7 +887,7 @@ __device__ __forceinline__ bool finish_steps(const Ctx& c, const Row& r, const S
     const int e = at < run + w[0] ? 0 : 1;
     *index = static_cast<uint32_t>(s->all.index[2 * c.tid + e]);
     if (prob != nullptr)
-      *prob = static_cast<float>(r.weight(x[e]) * kOne / static_cast<double>(all));
+      *prob = share(r, x[e], w[e], all);
   }
   return true;
 }
@@ -1106,7 +1118,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
   if (locate(c, r, kept, slot, target, &at, &at_x)) {
     *index = static_cast<uint32_t>(at);
     if (prob != nullptr)
-      *prob = static_cast<float>(r.weight(at_x) * kOne / static_cast<double>(all));
+      *prob = share(r, at_x, r.fixed(at_x), all);
   }
 }
 
