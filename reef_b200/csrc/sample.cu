@@ -47,7 +47,7 @@
 // shared memory and registers, and each row's chain is 15 to 35 us long: the copy and
 // the maximum 4, the weights 10 (50 instructions each where every second one is
 // heavy; with the histogram 15), then half a dozen steps of 1 to 4 us that end in a
-// cluster barrier.  A single row of 50257 with top-k: 14 us, all of it that chain.
+// cluster barrier.  A single row of 50257 with top-k: 13 us, all of it that chain.
 // Measured and dropped: two elements to an instruction (no change), the four adds of
 // a thread into the histogram in flight at once (3 % slower), the list weighed in a
 // pass of its own and the histogram in another (341).
