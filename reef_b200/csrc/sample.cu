@@ -1,6 +1,6 @@
 // sample.cu -- token sampling with temperature, top-k, top-p and min-p from
 // given random numbers, next to lm_head.cu's greedy argmax (reef chooses
-// greedily only; this build's own definition).
+// greedily only; the definition is this file's).
 //
 // Per row of n logits x, with temperature T and a uniform number u in [0, 1):
 //   w_i = exp((x_i - max x) / T)

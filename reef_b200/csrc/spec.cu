@@ -1,7 +1,7 @@
 // spec.cu -- what follows a pass over drafted tokens: the walk that accepts a
 // path of each sequence's tree, and the compaction of the int8 KV cache to
-// that path.  reef decodes one token at a time and has neither (this build's
-// own definitions).
+// that path.  reef decodes one token at a time and has neither (the
+// definitions are this file's).
 //
 // A tree is parents[t] (t < drafts <= 64): the drafted token that t follows,
 // an earlier one (parents[t] < t), or -1.  Node 0 is the root: the last

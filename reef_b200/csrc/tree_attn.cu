@@ -1,6 +1,6 @@
 // tree_attn.cu -- int8 attention of drafted tokens over the int8 KV cache
 // (the pass that checks a tree of drafts; reef decodes one token at a time,
-// so this is this build's own definition).
+// so the definition is this file's).
 //
 // Sequence b has len committed keys and d drafted tokens, whose keys and
 // values stand in the cache right behind them, at rows len + t.  Query (t,
