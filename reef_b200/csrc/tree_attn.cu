@@ -51,7 +51,7 @@
 // Measured (one call, cold cache): 4 drafts over 499 keys, 32 heads of their own, 8.7
 // us, which is the launch and three round trips (lengths, queries, keys).  64 sequences
 // over up to 4096 keys, 8 heads on one: 1 draft each (70 MB of cache) 26 us, 2 drafts 35, 8
-// drafts (ragged, 54 MB) 36, of which 12 are the shares, the first loads, the epilogues
+// drafts (ragged, 54 MB) 34, of which 11 are the shares, the first loads, the epilogues
 // and the join.  Two sequences over 16301 keys, 64 drafts, 64 heads on 8 (68.5 Gflop): 175
 // us, 0.39 Pflop/s of products or 0.78 with the rests; a tile takes 5000 cycles, of which
 // the tensor pipe is busy for 1550.  That is the issue of the softmax warps, two to a
@@ -108,8 +108,8 @@ struct TreeArgs {
 };
 
 // meta[c]: x first segment, y 1 when it began in an earlier CTA, z last
-// segment, w 1 when it goes on in the next CTA; x = -1 for a CTA without
-// units.
+// segment, w not 0 when it goes on in the next CTA: its query rows (of the KV head,
+// live). x = -1 for a CTA without units.
 template <int kStages>
 struct TLayout {  // shared memory layout (bytes from a 1024-aligned base)
   static constexpr int kKV = 2 * kTileKeys * 128;  // K then V, int8 [128][128] SW128
@@ -635,7 +635,7 @@ __global__ void __launch_bounds__(kTThreads, kPerSm)
       float* slot = a.part + (static_cast<long long>(cta) * 2 + (cut_before ? 0 : 1)) * kRows *
                                  kPartRow;
       if (j + 1 == nunits && tid == 0 && !a.per_cta)
-        a.meta[cta] = make_int4(first_seg, first_cut ? 1 : 0, seg, ends ? 0 : 1);
+        a.meta[cta] = make_int4(first_seg, first_cut ? 1 : 0, seg, ends ? 0 : d * a.group);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -738,8 +738,8 @@ struct CL {  // shared memory layout (bytes from a 1024-aligned base)
   static constexpr int kML = kScales + 2 * kSoftmax / 32 * 3 * kCols * 4;  // [2 tiles][parts][128]
   static constexpr int kPar = kML + 2 * kSoftmax * 4;         // int[64]
   static constexpr int kPre = kPar + kMaxDrafts * 4;      // int[batch + 1]
-  static constexpr int kKeep = kPre + (kMaxBatch + 4) * 4;  // int[7][softmax threads]
-  static constexpr int kBars = kKeep + 7 * kSoftmax * 4;
+  static constexpr int kKeep = kPre + (kMaxBatch + 4) * 4;  // int[8][softmax threads]
+  static constexpr int kBars = kKeep + 8 * kSoftmax * 4;
   static constexpr int kNumBars = 9 + 2 * kKStages + 2 * kVStages + 4;
   static constexpr int kTmemSlot = kBars + kNumBars * 8;
   static constexpr int kBytes = kTmemSlot + 16 + 1024;
@@ -1051,6 +1051,7 @@ __global__ void __launch_bounds__(kCThreads, 1)
       const int d = drafts_of(a, b, len, &bad);
       const bool live = r < d * a.group;
       put_aside(keep + 5 * kNext, live ? qrow : -1);
+      put_aside(keep + 7 * kNext, d * a.group);
       amul = live ? amul * base : 0.0f;
       if (mine < a.drafts) par[mine] = up;
       {
@@ -1400,7 +1401,8 @@ __global__ void __launch_bounds__(kCThreads, 1)
       tc_fence_before();
       mbar_arrive(o_free);
       if (left == w.n && tid == 256 && !a.per_cta)
-        a.meta[cta] = make_int4(cut < 0 ? -1 - cut : cut, cut < 0 ? 1 : 0, seg, ends ? 0 : 1);
+        a.meta[cta] = make_int4(cut < 0 ? -1 - cut : cut, cut < 0 ? 1 : 0, seg,
+                                ends ? 0 : take_back(keep + 7 * kNext));
       next_piece(pre, a.batch, per_seq, at, w.n, left);
       named_barrier(1, kSoftmax);  // Q's buffer is free again
     }
@@ -1421,6 +1423,17 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a, int tile_row
   const int c = blockIdx.x, rr = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int4 none = make_int4(-1, 0, -1, 0);
   int4 mk = c + lane < a.ctas ? a.meta[c + lane] : none;
+  // c's own part is its slot 1, the others' their slot 0.  What two or three CTAs share
+  // is on its way before it is known to be needed (all of it lies in the workspace).
+  const long long step = static_cast<long long>(2) * tile_rows * kPartRow;  // one CTA
+  const float* row = a.part + static_cast<long long>(rr) * kPartRow;
+  const float* own = row + c * step + static_cast<long long>(tile_rows) * kPartRow;
+  const float* one = lane == 0 ? own : row + min(c + lane, a.ctas - 1) * step;
+  float2 ml = make_float2(0.0f, 0.0f);
+  if (lane < 4) ml = *reinterpret_cast<const float2*>(one);
+  const float4 v_own = reinterpret_cast<const float4*>(own + 4)[lane];
+  const float4 v_next =
+      reinterpret_cast<const float4*>(row + min(c + 1, a.ctas - 1) * step + 4)[lane];
   const int4 first = make_int4(__shfl_sync(0xffffffffu, mk.x, 0), __shfl_sync(0xffffffffu, mk.y, 0),
                                __shfl_sync(0xffffffffu, mk.z, 0), __shfl_sync(0xffffffffu, mk.w, 0));
   // unfinished at the end of c, and begun in c
@@ -1428,13 +1441,8 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a, int tile_row
   const int seg = first.z;
   const int per_seq = a.heads_kv * a.qtiles;
   const int b = seg / per_seq, hq = seg % per_seq;
-  bool bad;
-  const int d = drafts_of(a, b, a.lens[b], &bad);
   const int r = (hq % a.qtiles) * tile_rows + rr;
-  if (r >= d * a.group) return;
-  const long long step = static_cast<long long>(2) * tile_rows * kPartRow;  // one CTA
-  // c's own part is its slot 1, the others' their slot 0
-  const float* row = a.part + static_cast<long long>(rr) * kPartRow;
+  if (r >= first.w) return;
   float m = -INFINITY, l = 0.0f;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   for (int k0 = c; k0 < a.ctas; k0 += 32) {
@@ -1449,8 +1457,9 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a, int tile_row
                      (self ? static_cast<long long>(tile_rows) * kPartRow : 0);
     float pm = -INFINITY, pl = 0.0f;
     if (in >> lane & 1u) {
-      pm = p[0];
-      pl = p[1];
+      if (k0 > c || lane >= 4) ml = *reinterpret_cast<const float2*>(p);
+      pm = ml.x;
+      pl = ml.y;
     }
     float mx = fmaxf(m, pm);
 #pragma unroll
@@ -1470,7 +1479,9 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a, int tile_row
       const float wk = __shfl_sync(0xffffffffu, w, k);
       const float* q = row + (k0 + k) * step +
                        (k0 + k == c ? static_cast<long long>(tile_rows) * kPartRow : 0);
-      const float4 v = reinterpret_cast<const float4*>(q + 4)[lane];
+      const float4 v = k0 + k == c       ? v_own
+                       : k0 + k == c + 1 ? v_next
+                                         : reinterpret_cast<const float4*>(q + 4)[lane];
       o = make_float4(fmaf(v.x, wk, o.x), fmaf(v.y, wk, o.y), fmaf(v.z, wk, o.z),
                       fmaf(v.w, wk, o.w));
     }
