@@ -9,6 +9,8 @@ memory and the current stream.  Weights are K-major [out][kpad(in)] int8 (see
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -295,6 +297,12 @@ def add_rmsnorm_quant(x: torch.Tensor, residual: torch.Tensor, gain: torch.Tenso
 # ---- drafted tokens over the int8 KV cache ---------------------------------------
 
 
+@functools.lru_cache(maxsize=256)
+def _tree_attn_workspace(b: int, t: int, hq: int, hkv: int, max_len: int, device: int) -> int:
+    with torch.cuda.device(device):
+        return max(16, _lib.lib().reef_b200_tree_attn_workspace_bytes(b, t, hq, hkv, max_len))
+
+
 def tree_attn_i8(q8: torch.Tensor, q_scale: torch.Tensor, k_cache: torch.Tensor,
                  k_scale: torch.Tensor, v_cache: torch.Tensor, v_scale: torch.Tensor,
                  lens: torch.Tensor, parents: torch.Tensor | None = None,
@@ -311,8 +319,8 @@ def tree_attn_i8(q8: torch.Tensor, q_scale: torch.Tensor, k_cache: torch.Tensor,
     _, hkv, max_len, _ = k_cache.shape
     dev, f32, i8, i32 = q8.device, torch.float32, torch.int8, torch.int32
     if out is None:
-        make = torch.empty if draft_lens is None else torch.zeros
-        out = make((b, t, hq, d), dtype=f32, device=dev)
+        make = q_scale.new_empty if draft_lens is None else q_scale.new_zeros
+        out = make((b, t, hq, d))
     cache, rows = (b, hkv, max_len, d), (b, hkv, max_len)
     before = (_take(lens, "lens", i32, (b,), dev),
               _take(draft_lens, "draft_lens", i32, (b,), dev),
@@ -322,8 +330,7 @@ def tree_attn_i8(q8: torch.Tensor, q_scale: torch.Tensor, k_cache: torch.Tensor,
              _take(k_cache, "k_cache", i8, cache, dev), _take(k_scale, "k_scale", f32, rows, dev),
              _take(v_cache, "v_cache", i8, cache, dev), _take(v_scale, "v_scale", f32, rows, dev))
     o = _take(out, "out", f32, (b, t, hq, d), dev)
-    nbytes = _lib.lib().reef_b200_tree_attn_workspace_bytes(b, t, hq, hkv, max_len)
-    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+    ws = q8.new_empty(_tree_attn_workspace(b, t, hq, hkv, max_len, dev.index))
     _call_on(dev, "reef_b200_tree_attn_i8", b, t, hq, hkv, d, max_len, *before,
              d ** -0.5 if sm_scale is None else sm_scale, *after, ws.data_ptr(), ws.numel(), o)
     return out
@@ -342,7 +349,7 @@ def tree_accept(tokens: torch.Tensor, chosen: torch.Tensor, parents: torch.Tenso
             _take(parents, "parents", i32, (b, t), dev),
             _take(tokens, "tokens", i32, (b, t), dev, torch.uint32),
             _take(chosen, "chosen", i32, (b, t), dev, torch.uint32))
-    path = torch.empty_like(tokens, dtype=i32)
+    path = torch.empty_like(tokens if tokens.dtype is i32 else tokens.view(i32))
     accepted = path.new_empty(b)
     following = chosen.new_empty(b)
     _call_on(dev, "reef_b200_tree_accept", b, t, *args, path.data_ptr(), accepted.data_ptr(),
