@@ -349,7 +349,7 @@ def tree_accept(tokens: torch.Tensor, chosen: torch.Tensor, parents: torch.Tenso
             _take(parents, "parents", i32, (b, t), dev),
             _take(tokens, "tokens", i32, (b, t), dev, torch.uint32),
             _take(chosen, "chosen", i32, (b, t), dev, torch.uint32))
-    path = torch.empty_like(tokens if tokens.dtype is i32 else tokens.view(i32))
+    path = torch.empty_like(tokens, dtype=i32)
     accepted = path.new_empty(b)
     following = chosen.new_empty(b)
     _call_on(dev, "reef_b200_tree_accept", b, t, *args, path.data_ptr(), accepted.data_ptr(),
