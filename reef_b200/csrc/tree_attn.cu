@@ -55,12 +55,13 @@
 // and the join.  Two sequences over 16301 keys, 64 drafts, 64 heads on 8 (68.5 Gflop): 175
 // us, 0.39 Pflop/s of products or 0.78 with the rests; a tile takes 5000 cycles, of which
 // the tensor pipe is busy for 1550.  That is the issue of the softmax warps, two to a
-// scheduler, 17 instructions a score at one in 4.8 cycles each.  Up to 32 rows the
-// products bound (2500 cycles a tile).  Measured and dropped: quarter rows in four warpgroups
+// scheduler, 17 instructions a score at one in 4.8 cycles each (left out for a
+// measurement, the loads of the scales save 27 us, the rests 11, the exponentials 4).  Up
+// to 32 rows the products bound (2500 cycles a tile).  Measured and dropped: quarter rows in four warpgroups
 // (they spill; with two copies they do not, and 64 x 8 takes 42 us: what a warp does
-// once a tile counts twice as often), scores taken a tile ahead, a barrier per pair of warps, scores in
-// fragments of 16 x 8 (a quarter of the loads of scales, and no faster), O moved by the
-// converters.
+// once a tile counts twice as often), scores taken a tile ahead, a barrier per pair of
+// warps, scores in fragments of 16 x 8 (a quarter of the loads of scales, but 184 us), O
+// moved by the converters.
 #include "attn_mma.cuh"
 #include "common.cuh"
 #include "ops.h"
