@@ -858,7 +858,10 @@ __device__ __forceinline__ bool finish_steps(const Ctx& c, const Row& r, const S
   }
   __syncthreads();
   const int n = s->near_n[0];
-  if (n > kNear) return false;
+  if (n > kNear) {
+    __syncthreads();  // everyone has read the count, which select_near begins by clearing
+    return false;
+  }
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     if (near[e]) {

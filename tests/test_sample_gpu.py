@@ -134,6 +134,28 @@ def test_borders_among_equal_values(n, equal):
     check(x, u, k=np.full(rows, equal // 2 + 5), p=r.uniform(0.2, 0.999, rows))
 
 
+@pytest.mark.parametrize("n", [1000, 20000])
+def test_steps_with_more_elements_than_are_sorted(n):
+    """A list that one CTA takes over (at most 1024) with more than 512 equal logits in
+    top-p's step: the count of them is read by every warp before the selection that
+    follows clears it, whatever the warps' pace, in many rows at once and again and again."""
+    rows = 600
+    r = np.random.RandomState(n)
+    x = np.full((rows, n), -80.0, np.float32)
+    equal = 513 + np.arange(rows) % 488
+    for i in range(rows):
+        at = r.permutation(n)[: equal[i]]
+        x[i, at] = 1.5
+        x[i, at[: i % 7]] = 1.5 + np.arange(i % 7, dtype=np.float32) / 8
+    u, p = r.rand(rows).astype(np.float32), r.uniform(0.3, 0.95, rows).astype(np.float32)
+    check(x, u, p=p)
+    dev = [torch.from_numpy(a).cuda() for a in (x, u, p)]
+    want = K.sample_f32(dev[0], dev[1], top_p=dev[2])
+    for _ in range(20):
+        got = K.sample_f32(dev[0], dev[1], top_p=dev[2])
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 @pytest.mark.parametrize("p", [0.99, 0.999999])
 def test_nearly_everything_kept(p):
     """Flat rows of which top-p leaves out little: what is kept does not fit a list."""
