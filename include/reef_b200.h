@@ -318,8 +318,11 @@ int reef_b200_argmax_f32(size_t n, const float* x, uint32_t* index, reef_b200_st
  * kept.  T not above 0 (NaN among it): the first largest logit, prob 1.  A NaN
  * logit counts as -inf, and -inf is never chosen; with +inf in a row only its
  * +infs weigh.  A row without any logit above -inf gives REEF_B200_NO_TOKEN
- * and prob 0.  Sums are exact (weights rounded once to 2^-43), so the same
- * call always gives the same token.  n <= 2^20, rows <= 2^24
+ * and prob 0.  Sums are exact, so the same call always gives the same token;
+ * the weights are rounded to 2^-43 of the largest (each off by 0.55 of that at
+ * most).  Against weights that are not rounded a border between two tokens
+ * moves by about 2^-44 sqrt(n) of the largest weight, by 0.55 n 2^-43 at most (a
+ * tail of n equal logits shares its rounding).  n <= 2^20, rows <= 2^24
  * (REEF_B200_ERR_TOO_LARGE). */
 #define REEF_B200_NO_TOKEN 0xffffffffu
 int reef_b200_sample_f32(size_t rows, size_t n, const float* logits, const float* temperature,

@@ -17,10 +17,12 @@
 // (a vocabulary has 1e5 borders) that sums in float would choose wrongly for
 // one row in a few dozen.  So w is held as a 64-bit integer, w * 2^43 rounded:
 // sums of up to 2^20 of them are exact, hence the same in any order, and nothing
-// depends on the schedule.  Weights from 2^-20 up ("heavy") are computed in
-// double; of the others 23 bits are all that is left, and float with the
-// constants in two terms gives those.  Together a border moves by about 2^-44 *
-// sqrt(n), 2e-11 of the largest weight.
+// depends on the schedule.  Weights from 2^-27 up ("heavy") are computed in
+// double; the others are below 2^16 units, and float with the constants in two
+// terms is off by 0.05 of one there (the exponent's one rounding, 2^-21, and 2 ulp of
+// ex2; at 2^-20 it would be 6 units).  So an integer is off by 0.55 at most.  Logits that
+// differ make a border move by about 2^-44 * sqrt(n) of the largest weight; equal ones
+// share their rounding, and n of them move it by 0.55 n units at most.
 //
 // Passes.  A cluster of C CTAs owns a row: each keeps its slice of the logits in
 // shared memory (one bulk copy), so the row is read from HBM once however many passes
@@ -50,7 +52,9 @@
 // cluster barrier.  A single row of 50257 with top-k: 13 us, all of it that chain.
 // Measured and dropped: two elements to an instruction (no change), the four adds of
 // a thread into the histogram in flight at once (3 % slower), the list weighed in a
-// pass of its own and the histogram in another (341).
+// pass of its own and the histogram in another (341).  Heavy from 2^-27 up instead of
+// from 2^-20, where float is not enough, costs nothing but where most of a vocabulary
+// weighs between the two (256 x 128000, no filter: 117 -> 140).
 #include "common.cuh"
 #include "ops.h"
 
@@ -169,7 +173,7 @@ struct Row {
   int first;        // index of its first element in the row (below 0: not of the row, -inf)
   float top;        // the row's maximum
   bool plain;       // magnitudes at which light() holds
-  float heavy;      // values from here up weigh 2^-20 or (barely) less
+  float heavy;      // values from here up weigh 2^-27 or (barely) less
   float least;      // values below weigh nothing
   double c, rcp_t, per_bit;  // log2(e) / T, 1 / T, T ln 2
   float c_hi, c_lo, k_hi, k_lo;  // c, and top * c - 43, in two terms
@@ -180,9 +184,9 @@ struct Row {
     if (!(v > -INFINITY) || top == INFINITY) return 0.0;
     return exp((static_cast<double>(v) - static_cast<double>(top)) * rcp_t);
   }
-  // weight * 2^43 of a value below `heavy`: under 2^23.  log2 of it is v * c -
-  // (top * c - 43), one fma that rounds once, plus what the second terms add
-  // (2^-10 at most), taken to first order.
+  // weight * 2^43 of a value below `heavy`: under 2^16.  log2 of it is v * c -
+  // (top * c - 43), one fma that rounds once (2^-21 below 16), plus what the second
+  // terms add (2^-10 at most), taken to first order.
   __device__ __forceinline__ uint32_t light(float v) const {
     v = fmaxf(v, least);  // (-inf and NaN too)
     const float e = __fmaf_rn(v, c_lo, -k_lo);
@@ -1016,7 +1020,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
   r.k_hi = static_cast<float>(k2);
   r.k_lo = static_cast<float>(k2 - static_cast<double>(r.k_hi));
   r.plain = fabs(k2) < 8192.0 && fabsf(top) < 1e30f && t < 1e30f && t > 1e-30f;
-  r.heavy = r.below_top(-20.0);
+  r.heavy = r.below_top(-27.0);
   r.least = r.below_top(-60.0);
 
   // min-p in float but next to the border, in double there

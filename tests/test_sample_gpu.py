@@ -156,6 +156,77 @@ def test_steps_with_more_elements_than_are_sorted(n):
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+def tail_value(bits, t):
+    """A float near -bits ln 2 t whose weight against 0, in units of 2^-43, is a quarter
+    or less off a whole number: a weight off by less than a quarter rounds to it."""
+    x = np.float32(-bits * math.log(2.0) * t)
+    while True:
+        w = math.exp(float(x) / float(t)) * 2.0**43
+        if abs(w - round(w)) <= 0.25:
+            return x, round(w)
+        x = np.nextafter(x, np.float32(-math.inf))
+
+
+@pytest.mark.parametrize("n", [5000, 128000, 1 << 20])
+@pytest.mark.parametrize("t", [0.7, 1.3])
+@pytest.mark.parametrize("bits", [(20.3,), (21.4,), (22.6,), (23.5,), (25.2,), (26.7,), (28.1,),
+                                  (20.1, 20.9, 21.8, 22.4, 24.3, 26.9, 29.5)])
+def test_equal_logits_that_weigh_little(n, t, bits):
+    """One logit ahead of a tail of equal ones that weigh 2^-20 to 2^-30 of it.  Equal
+    weights share their rounding, so it adds up over the tail: with every weight the
+    whole number of 2^-43 next to it, sums and draws are exact (u times the total is
+    rounded to 53 bits, 2 units here).  Against weights that are not rounded a border, or
+    u times the total, moves by 0.625 units for each of n at most."""
+    t, rows = np.float32(t), 32
+    r = np.random.RandomState(n % 1000 + int(10 * bits[0]))
+    values = [tail_value(b, t) for b in bits]
+    pick = r.randint(0, len(values), n)
+    at = n // 3
+    x = np.array([v for v, _ in values], np.float32)[pick]
+    w = np.array([q for _, q in values], np.int64)[pick]
+    x[at], w[at] = 0.0, 1 << 43
+    run = np.cumsum(w)
+    total = int(run[-1])
+    exact = np.exp(x.astype(np.float64) / np.float64(t))
+    run64 = np.cumsum(exact.astype(np.longdouble))
+    # most draws into the tail, before and behind the first
+    tail = (total - (1 << 43)) / total
+    u = np.concatenate([r.rand(rows // 2) * tail / 3, 1 - r.rand(rows // 2) * tail * 2 / 3])
+    u = np.minimum(u.astype(np.float32), np.nextafter(np.float32(1), np.float32(0)))
+    xs = torch.from_numpy(x).cuda().expand(rows, n).contiguous()
+    us, ts = torch.from_numpy(u).cuda(), torch.full((rows,), float(t), device="cuda")
+    index, prob = K.sample_f32(xs, us, temperature=ts)
+    index, prob = index.cpu().numpy(), prob.cpu().numpy()
+    slack = np.longdouble(n * 0.625 * 2.0**-43)
+    checked = 0
+    for i in range(rows):
+        goal = int(np.float64(u[i]) * np.float64(total))
+        lo, hi = (int(np.searchsorted(run, goal + e, side="right")) for e in (-2, 2))
+        if lo == hi:
+            checked += 1
+            assert index[i] == lo, (i, index[i], lo)
+        j, goal = index[i], np.longdouble(u[i]) * run64[-1]
+        assert (run64[j - 1] if j else 0.0) <= goal + 2 * slack and run64[j] >= goal - 2 * slack
+        assert abs(prob[i] - exact[j] / (total * 2.0**-43)) <= 2.0**-23 * prob[i]
+    assert checked >= rows // 2
+    # top-p with its border in the tail: the largest values first, then by index
+    order = np.argsort(-x, kind="stable")
+    before = np.cumsum(w[order]) - w[order]
+    for p in (np.float32(0.9), np.float32(1.0 - tail / 2)):
+        want = float(p) * total
+        kept = order[before < want]
+        if abs(before[kept.size - 1] - want) < 4 or abs(before[min(kept.size, n - 1)] - want) < 4:
+            continue
+        kept = np.sort(kept)
+        run = np.cumsum(w[kept])
+        index, _ = K.sample_f32(xs, us, temperature=ts, top_p=torch.full((rows,), float(p), device="cuda"))
+        for i, got in enumerate(index.cpu().numpy()):
+            goal = int(np.float64(u[i]) * np.float64(run[-1]))
+            lo, hi = (int(np.searchsorted(run, goal + e, side="right")) for e in (-2, 2))
+            if lo == hi:
+                assert got == kept[lo], (p, i, got, kept[lo])
+
+
 @pytest.mark.parametrize("p", [0.99, 0.999999])
 def test_nearly_everything_kept(p):
     """Flat rows of which top-p leaves out little: what is kept does not fit a list."""
