@@ -507,8 +507,8 @@ int reef_b200_decode_attn_i8(size_t batch, size_t heads_q, size_t heads_kv, size
  * sequence with lens[b] + draft_lens[b] > max_len, or a negative length,
  * records 0x201 in the device error word and is left out.  Keys that a query
  * does not see add nothing, whatever their scales hold.  V scales are not
- * negative (a row's largest magnitude over 127 never is); one below 2^-100
- * counts as 0.  batch <= 2048 (REEF_B200_ERR_TOO_LARGE).  q8, out and the
+ * negative (a row's largest magnitude over 127 never is) and at most 2^48; one
+ * below 2^-64 counts as 0 (its key keeps its share of the softmax).  batch <= 2048 (REEF_B200_ERR_TOO_LARGE).  q8, out and the
  * workspace are 16-byte aligned; the workspace holds at least
  * reef_b200_tree_attn_workspace_bytes(); calls that may run at once need one
  * each. */

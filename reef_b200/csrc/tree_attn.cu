@@ -85,7 +85,10 @@ constexpr int kMaxCtasPerSm = 2;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 4.0f;   // the maximum is raised when a score passes it by more (log2)
 constexpr float kLift = 11.0f;  // log2 of P' at the maximum
-constexpr float kNoScale = 0x1p-100f;  // a V scale below counts as 0
+// A V scale below counts as 0, and stands for its key in P' and the softmax sum.  P' <=
+// 2^15 over it, 2^24 times, must stay below 2^128; and the P' of such a key, beside scales
+// of up to 2^48, above 2^-126 down to 2^-25 of their weight (11 - 64 - 48 - 25).
+constexpr float kNoScale = 0x1p-64f;
 
 struct TreeArgs {
   int batch, drafts, heads_q, heads_kv, max_len;

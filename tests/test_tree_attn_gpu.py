@@ -202,6 +202,47 @@ def test_v_scales_of_zero(hq):
     assert bool(((out[0, 3].double() - p @ v).abs() <= 1e-5 * (p @ v.abs())).all())
 
 
+def zeros_lifted(x):
+    """The same product with V scales of 0 as codes of 0 (what `check` takes log2 of)."""
+    none = x["v_scale"] == 0
+    return x | dict(v_cache=torch.where(none[..., None], 0, x["v_cache"]),
+                    v_scale=torch.where(none, 2.0**-64, x["v_scale"]))
+
+
+@pytest.mark.parametrize("t,hq", [(1, 8), (2, 8), (4, 8), (8, 8), (16, 8)])
+def test_a_long_stretch_of_v_scales_of_zero(t, hq):
+    """24576 keys whose V scale is 0 before 8192 with values: their part of the softmax
+    sum stays finite wherever the keys are cut, also where their scores pass the first
+    ones' by just less than what raises the running maximum."""
+    b, max_len, zeros = 150, 32768, 24576
+    x = make(b, t, hq, 1, 4, seed=70 + t)
+    g = torch.Generator(device="cuda").manual_seed(71)
+    v8, vs = rows8(g, (1, 1, max_len), 1.0)
+    vs[:, :, :zeros] = 0.0
+    x |= dict(q8=torch.ones_like(x["q8"]), q_scale=torch.ones_like(x["q_scale"]),
+              k_cache=torch.ones((b, 1, max_len, 128), dtype=torch.int8, device="cuda"),
+              k_scale=torch.full((b, 1, max_len), 2.6, device="cuda"),
+              v_cache=v8.expand(b, -1, -1, -1).contiguous(),
+              v_scale=vs.expand(b, -1, -1).contiguous())
+    x["k_scale"][:, :, :128] = 0.0
+    out = run(x, [max_len - t] * b, sm=1.0 / 128)
+    for i in range(0, b, 13):
+        check(zeros_lifted({k: v[i:i + 1] for k, v in x.items()}), [max_len - t], None, None,
+              out[i:i + 1], 1.0 / 128)
+
+
+@pytest.mark.parametrize("t,hq", [(4, 2), (4, 4), (8, 4), (8, 8), (8, 16)])
+def test_v_scales_of_zero_beside_large_ones(t, hq):
+    """Keys with V scales of 0 keep their share beside scales of 2^48."""
+    x = make(2, t, hq, 1, 1024, seed=14)
+    x["v_scale"][0, 0, ::2] = 0.0
+    x["v_scale"][0, 0, 1::2] = 2.0**48
+    x["v_scale"][1] = 2.0**48
+    x["v_scale"][1, 0, :700] = 0.0
+    out = run(x, [1000, 900], sm=0.02)
+    check(zeros_lifted(x), [1000, 900], None, None, out, 0.02)
+
+
 @pytest.mark.parametrize("junk", [math.nan, math.inf, -math.inf, 3.4e38])
 @pytest.mark.parametrize("hq", [2, 8])  # 8 and 32 query rows: both kernels
 def test_rows_nobody_sees_add_nothing(junk, hq):
