@@ -196,14 +196,25 @@ class LlamaLayer:
         `cache` behind the lens [batch] committed rows; trees as in
         kernels.tree_attn_i8.  kernels.kv_compact_i8 then keeps a path.  The layer's
         calls share its workspace, captured ones too: one at a time."""
-        dev, f32 = self.w_qkv.device, torch.float32
+        dev, f32, i8, i32 = self.w_qkv.device, torch.float32, torch.int8, torch.int32
+        if x.shape[0] % self.batch != 0:
+            raise ValueError("x must hold the same number of rows for every sequence")
+        drafts, max_len = x.shape[0] // self.batch, cache["max_len"]
+        rows, tree = (x.shape[0], self.attn_norm.numel()), (self.batch, drafts)
+        kept_rows = (self.batch, self.heads_kv, max_len)
+        y = torch.empty_like(x) if out is None else out
+        args = (K._take(x, "x", f32, rows, dev), K._take(y, "out", f32, rows, dev),
+                K._take(lens, "lens", i32, tree[:1], dev),
+                K._take(draft_lens, "draft_lens", i32, tree[:1], dev),
+                K._take(parents, "parents", i32, tree, dev),
+                K._take(cache["k"], "the cache's k", i8, kept_rows + (128,), dev),
+                K._take(cache["ks"], "the cache's ks", f32, kept_rows, dev),
+                K._take(cache["v"], "the cache's v", i8, kept_rows + (128,), dev),
+                K._take(cache["vs"], "the cache's vs", f32, kept_rows, dev))
         if getattr(self, "_tiles", None) is None and not torch.cuda.is_current_stream_capturing():
             # (a capture would only record the packing, and other streams may call next)
             self._decode_tiles()
             torch.cuda.current_stream(dev).synchronize()
-        if x.shape[0] % self.batch != 0:
-            raise ValueError("x must hold the same number of rows for every sequence")
-        drafts, max_len = x.shape[0] // self.batch, cache["max_len"]
         # (kept for good: a captured call goes on using its own)
         kept = self.__dict__.setdefault("_verify_ws", {})
         ws = kept.get((drafts, max_len))
@@ -213,15 +224,8 @@ class LlamaLayer:
             if n == 0:
                 raise ValueError("invalid description of a pass over drafted tokens")
             ws = kept[drafts, max_len] = torch.empty(n, dtype=torch.uint8, device=dev)
-        rows, tree = (x.shape[0], self.attn_norm.numel()), (self.batch, drafts)
-        y = torch.empty_like(x) if out is None else out
-        K._call_on(dev, "reef_b200_llama_verify_forward", C.byref(self.desc), drafts,
-                   K._take(x, "x", f32, rows, dev), K._take(y, "out", f32, rows, dev),
-                   K._take(lens, "lens", torch.int32, tree[:1], dev),
-                   K._take(draft_lens, "draft_lens", torch.int32, tree[:1], dev),
-                   K._take(parents, "parents", torch.int32, tree, dev), cache["k"].data_ptr(),
-                   cache["ks"].data_ptr(), cache["v"].data_ptr(), cache["vs"].data_ptr(), max_len,
-                   ws.data_ptr(), ws.numel())
+        K._call_on(dev, "reef_b200_llama_verify_forward", C.byref(self.desc), drafts, *args,
+                   max_len, ws.data_ptr(), ws.numel())
         return y
 
     def host_weights(self) -> dict:

@@ -7,6 +7,7 @@ import torch
 
 from reef_b200 import _lib
 from reef_b200 import kernels as K
+from reef_b200 import layer as RL
 
 INVALID, ALIGNMENT, TOO_LARGE = 1, 2, 7
 
@@ -147,3 +148,39 @@ def test_verify_refusals(L):
         a = list(args)
         a[i] = C.c_void_p(4096 + 4)
         assert f(ref, 2, *a, 64, P, 1 << 40, None) == ALIGNMENT
+
+
+def host_layer(batch=2, heads_kv=2, hidden=64, **kw):
+    """A layer's wrapper whose tensors are on the host: its operands are refused as on
+    the GPU, and one with nothing else wrong for lying there."""
+    layer = object.__new__(RL.LlamaLayer)
+    layer.__dict__.update(dict(batch=batch, heads_kv=heads_kv, _tiles={}, world=1,
+                               tp_mode=RL.TP_ALLREDUCE, w_qkv=torch.zeros(1),
+                               attn_norm=torch.zeros(hidden)) | kw)
+    return layer
+
+
+def host_cache(batch=2, heads_kv=2, rows=64, max_len=None):
+    shape = (batch, heads_kv, rows)
+    c = {n: torch.zeros(shape + (128,), dtype=torch.int8) for n in ("k", "v")}
+    return c | {"ks": torch.zeros(shape), "vs": torch.zeros(shape),
+                "max_len": rows if max_len is None else max_len}
+
+
+def test_verify_refuses_a_cache_that_is_not_the_layers(monkeypatch):
+    layer, x, lens = host_layer(), torch.zeros((4, 64)), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA"):
+        layer.verify(x, lens, host_cache())
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True)  # (shapes are what is looked at below)
+    for bad in (dict(batch=1), dict(batch=3), dict(heads_kv=1), dict(max_len=128), dict(max_len=32)):
+        with pytest.raises(ValueError, match="cache's k must be"):
+            layer.verify(x, lens, host_cache(**bad))
+    for name in ("k", "ks", "v", "vs"):
+        c = host_cache()
+        for bad in (c[name][:1], c[name][:, :, :32].contiguous(), c[name][None]):
+            with pytest.raises(ValueError, match=f"cache's {name} must be"):
+                layer.verify(x, lens, c | {name: bad})
+        with pytest.raises(TypeError, match=f"cache's {name} must be"):
+            layer.verify(x, lens, c | {name: c[name].half()})
+    with pytest.raises(ValueError, match="contiguous"):
+        layer.verify(x, lens, host_cache() | {"vs": host_cache(rows=128)["vs"][:, :, :64]})
