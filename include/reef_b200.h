@@ -687,8 +687,11 @@ int reef_b200_llama_decode_forward(const reef_b200_llama_layer* layer, const flo
  * values go to cache rows lens[b] + t, rotated for position lens[b] + depth (a
  * root's depth is 0), and each token attends as in reef_b200_tree_attn_i8, whose
  * lens, draft_lens and parents these are; its cache and scale alignment holds too
- * (max_len a multiple of 4).  Rows of y past a sequence's drafts, and of a
- * sequence that does not fit the cache (0x201), are unspecified. */
+ * (max_len a multiple of 4).  heads_q / heads_kv is 1, 2, 4, 8 or 16, as in the
+ * decode step.  With a communicator of several ranks the plan is
+ * REEF_B200_TP_ALLREDUCE (a layer of the other plan: REEF_B200_ERR_INVALID).
+ * Rows of y past a sequence's drafts, and of a sequence that does not fit the
+ * cache (0x201), are unspecified. */
 size_t reef_b200_llama_verify_workspace_bytes(const reef_b200_llama_layer* layer, size_t drafts,
                                               size_t max_len);
 int reef_b200_llama_verify_forward(const reef_b200_llama_layer* layer, size_t drafts,

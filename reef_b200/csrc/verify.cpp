@@ -2,6 +2,7 @@
 // new tokens per sequence, each seeing the committed cache rows, itself and its
 // ancestors in the sequence's tree.  Everything but the cache append and the
 // attention is the decode step's own (layer.cpp), on batch * drafts rows.
+#include "comm.h"
 #include "layer.h"
 
 #include <algorithm>
@@ -10,10 +11,12 @@ using namespace reef;
 
 namespace {
 
-// the decode step's description of the same layer, a row per drafted token
+// the decode step's description of the same layer, a row per drafted token.  Its o and
+// down projections are row-parallel: weights, x and y of the all-gather plan are others.
 bool rows_of(const reef_b200_llama_layer* L, size_t drafts, reef_b200_llama_layer* rows) {
   if (L == nullptr || drafts == 0 || drafts > static_cast<size_t>(kMaxDrafts) || L->batch == 0 ||
-      L->batch > 128)
+      L->batch > 128 ||
+      (comm_world(reinterpret_cast<Comm*>(L->comm)) > 1 && L->tp_mode != REEF_B200_TP_ALLREDUCE))
     return false;
   *rows = *L;
   rows->batch = L->batch * drafts;  // <= 128, checked with the rest of it

@@ -194,8 +194,11 @@ class LlamaLayer:
         """The decode step on drafted tokens: x [batch * drafts][hidden], row b *
         drafts + t the drafted token t of sequence b (the root first), appended to
         `cache` behind the lens [batch] committed rows; trees as in
-        kernels.tree_attn_i8.  kernels.kv_compact_i8 then keeps a path.  The layer's
-        calls share its workspace, captured ones too: one at a time."""
+        kernels.tree_attn_i8.  kernels.kv_compact_i8 then keeps a path.  At most 128
+        rows, and no shard of a TP_ALLGATHER layer (its w_o and w_down are others).  The
+        layer's calls share its workspace, captured ones too: one at a time."""
+        if self.world > 1 and self.tp_mode == TP_ALLGATHER:
+            raise ValueError("drafted tokens run on a TP_ALLREDUCE layer")
         dev, f32, i8, i32 = self.w_qkv.device, torch.float32, torch.int8, torch.int32
         if x.shape[0] % self.batch != 0:
             raise ValueError("x must hold the same number of rows for every sequence")

@@ -184,3 +184,13 @@ def test_verify_refuses_a_cache_that_is_not_the_layers(monkeypatch):
             layer.verify(x, lens, c | {name: c[name].half()})
     with pytest.raises(ValueError, match="contiguous"):
         layer.verify(x, lens, host_cache() | {"vs": host_cache(rows=128)["vs"][:, :, :64]})
+
+
+def test_verify_refuses_a_shard_of_the_all_gather_plan():
+    """Also without a communicator, where the library cannot know."""
+    x, lens = torch.zeros((4, 64)), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="TP_ALLREDUCE"):
+        host_layer(world=2, tp_mode=RL.TP_ALLGATHER).verify(x, lens, host_cache())
+    for fine in (dict(world=2), dict(tp_mode=RL.TP_ALLGATHER)):
+        with pytest.raises(ValueError, match="CUDA"):
+            host_layer(**fine).verify(x, lens, host_cache())
