@@ -170,7 +170,10 @@ class LlamaLayer:
     def decode(self, x: torch.Tensor, positions: torch.Tensor, cache: dict,
                out: torch.Tensor | None = None) -> torch.Tensor:
         """One decode step: x [batch][hidden] (one new token per sequence) at
-        `positions` (int32 [batch], device); appends to `cache`."""
+        `positions` (int32 [batch], device); appends to `cache`.  No shard of a
+        TP_ALLGATHER layer, as in verify."""
+        if self.world > 1 and self.tp_mode == TP_ALLGATHER:
+            raise ValueError("the decode step runs on a TP_ALLREDUCE layer")
         if getattr(self, "_tiles", None) is None:
             self._decode_tiles()
         max_len = cache["max_len"]

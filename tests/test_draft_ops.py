@@ -191,6 +191,8 @@ def test_verify_refuses_a_shard_of_the_all_gather_plan():
     x, lens = torch.zeros((4, 64)), torch.zeros(2, dtype=torch.int32)
     with pytest.raises(ValueError, match="TP_ALLREDUCE"):
         host_layer(world=2, tp_mode=RL.TP_ALLGATHER).verify(x, lens, host_cache())
+    with pytest.raises(ValueError, match="TP_ALLREDUCE"):
+        host_layer(world=2, tp_mode=RL.TP_ALLGATHER).decode(x, lens, host_cache())
     for fine in (dict(world=2), dict(tp_mode=RL.TP_ALLGATHER)):
         with pytest.raises(ValueError, match="CUDA"):
             host_layer(**fine).verify(x, lens, host_cache())
