@@ -536,10 +536,10 @@ int reef_b200_tree_accept(size_t batch, size_t drafts, const int32_t* draft_lens
  * (`layers` caches [batch][heads_kv][max_len][128] and scales [batch][heads_kv]
  * [max_len] back to back); every source is read before any row is written, so
  * a path may be in any order and name a row twice.  new_lens[b] = lens[b] +
- * accepted[b] (not lens itself: REEF_B200_ERR_INVALID).  A path entry outside
- * [0, drafts), a row outside the cache or a count outside [0, drafts] records
- * 0x201 and leaves that sequence as it is (new_lens[b] = lens[b]).  Caches
- * 16-byte aligned. */
+ * accepted[b] (not in lens, path or accepted: REEF_B200_ERR_INVALID).  A path
+ * entry outside [0, drafts), a row outside the cache or a count outside [0,
+ * drafts] records 0x201 and leaves that sequence as it is (new_lens[b] =
+ * lens[b]).  Caches 16-byte aligned. */
 int reef_b200_kv_compact_i8(size_t layers, size_t batch, size_t heads_kv, size_t head_dim,
                             size_t max_len, size_t drafts, const int32_t* lens,
                             const int32_t* path, const int32_t* accepted, int8_t* k_cache,

@@ -704,6 +704,14 @@ int reef_b200_kv_compact_i8(size_t layers, size_t batch, size_t heads_kv, size_t
   if (drafts > static_cast<size_t>(kMaxDrafts) || layers > (1u << 16) || batch > (1u << 20) ||
       heads_kv > 4096 || max_len > (1u << 24) || layers * batch * heads_kv > kMaxDim)
     return REEF_B200_ERR_TOO_LARGE;
+  // one CTA of a sequence writes its new length while others read these
+  const auto under_new_lens = [&](const int32_t* p, size_t n) {
+    const auto a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(new_lens);
+    return a < b + 4 * batch && b < a + 4 * n;
+  };
+  if (under_new_lens(lens, batch) || under_new_lens(accepted, batch) ||
+      under_new_lens(path, batch * drafts))
+    return REEF_B200_ERR_INVALID;
   if ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) % 16 != 0)
     return REEF_B200_ERR_ALIGNMENT;
   if (int rc = check_device()) return rc;

@@ -104,6 +104,22 @@ def test_compact_refusals(L):
         assert compact(L, a=a) == ALIGNMENT
 
 
+def test_compact_refuses_new_lens_in_what_it_reads(L):
+    """The new length of a sequence is written by one CTA while the others read lens,
+    path and accepted: no overlap, not even of one element."""
+    far = [C.c_void_p(1 << 20), C.c_void_p(2 << 20), C.c_void_p(3 << 20)] + [P] * 4
+    base, b, t = 1 << 30, 8, 4
+    for i, n in ((0, b), (1, b * t), (2, b)):  # lens, path, accepted at `base`
+        a = list(far)
+        a[i] = C.c_void_p(base)
+        for at in (base, base + 4, base + 4 * (n - 1), base - 4 * (b - 1)):
+            assert compact(L, b=b, t=t, a=a, new=C.c_void_p(at)) == INVALID, (i, at)
+        for at in (base + 4 * n, base - 4 * b):  # next to it: refused for what comes after
+            off = list(a)
+            off[3] = C.c_void_p(4096 + 8)
+            assert compact(L, b=b, t=t, a=off, new=C.c_void_p(at)) == ALIGNMENT, (i, at)
+
+
 def test_wrappers_refuse_tensors_before_any_call():
     f, i = torch.zeros, torch.int32
     with pytest.raises(ValueError, match="CUDA"):
