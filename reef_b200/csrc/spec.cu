@@ -115,7 +115,9 @@ __global__ void __launch_bounds__(kCThreads)
     v[j] = *reinterpret_cast<const uint4*>(c + (row0 + s) * 128 + (i & 7) * 16);
   }
   float sc = 0.0f;
-  if (tid < 2 * n) sc = (tid < n ? k_scale : v_scale)[row0 + src[tid % n]];
+  const int sr = tid < 2 * n ? tid % n : 0;
+  const bool moves = tid < 2 * n && src[sr] != sr;
+  if (moves) sc = (tid < n ? k_scale : v_scale)[row0 + src[sr]];
   __syncthreads();  // every row is held before any is written
 #pragma unroll
   for (int j = 0; j < kCVecs; ++j) {
@@ -126,7 +128,7 @@ __global__ void __launch_bounds__(kCThreads)
     int8_t* c = i >> 3 < n ? k_cache : v_cache;
     *reinterpret_cast<uint4*>(c + (row0 + r) * 128 + (i & 7) * 16) = v[j];
   }
-  if (tid < 2 * n) (tid < n ? k_scale : v_scale)[row0 + tid % n] = sc;
+  if (moves) (tid < n ? k_scale : v_scale)[row0 + sr] = sc;
 }
 
 }  // namespace

@@ -146,6 +146,25 @@ def test_compact_leaves_a_bad_sequence_and_reports_it(lens, path, accepted):
         K.check_device_error()
 
 
+@pytest.mark.parametrize("first", ["k", "v"])
+def test_compact_writes_no_row_that_is_in_its_place(first):
+    """Codes and scales.  K's and V's scales lie in one array, one a step behind the
+    other, so that a scale written back where the one has it would undo the other's move."""
+    t, max_len = 4, 16
+    c = cache((1, 1, max_len), 5)
+    both = torch.rand(max_len + 1, device="cuda")
+    k, v = both[:max_len].view(1, 1, max_len), both[1:].view(1, 1, max_len)
+    if first == "v":
+        k, v = v, k
+    want = both.clone()
+    want[1], want[2] = both[2], both[3]  # row 1 := row 2; row 0 stays
+    rows = c["k_cache"].clone()
+    K.kv_compact_i8(c["k_cache"], k, c["v_cache"], v, dev([0]), dev([[0, 2, -1, -1]]), dev([2]))
+    assert torch.equal(both, want)
+    rows[:, :, 1] = rows[:, :, 2]
+    assert torch.equal(c["k_cache"], rows)
+
+
 def test_compact_past_32_bits():
     """The last layer's rows lie past 2^32 bytes."""
     layers, b, hkv, max_len = 66, 4, 8, 16384
