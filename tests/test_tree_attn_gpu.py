@@ -302,6 +302,35 @@ def test_positions_outside_the_cache_are_reported_and_left_out():
         K.check_device_error()
 
 
+@pytest.mark.parametrize("t,hq", [(4, 2), (4, 4), (8, 4), (8, 8), (16, 8)])
+def test_shares_pass_over_sequences_that_are_empty_or_do_not_fit(t, hq):
+    """8 to 128 query rows over a cache long enough that CTAs take equal shares of all
+    sequences' keys: some at the beginning, in the middle and at the end have no drafts or
+    a place outside the cache; draft_lens above the drafts count as all of them."""
+    max_len = 2048
+    rows = [(max_len - t + 1, t), (-1, t), (5, 0), (700, t), (max_len + 1, 1), (1999, -1),
+            (2000, t + 3), (0, 1), (3, -2**31), (129, 2), (max_len, 0), (1500, t), (17, 0),
+            (2**31 - 1, t), (max_len - 1, 2), (127, t - 1), (max_len - t, t), (1, 0), (-5, 1)]
+    lens, drafts = [a for a, _ in rows], [d for _, d in rows]
+    x = make(len(rows), t, hq, 1, max_len, seed=90 + t + hq)
+    parents = trees(91, len(rows), t)
+    out = run(x, lens, parents, drafts)
+    live = 0
+    for i, (n, d) in enumerate(rows):
+        d = min(d, t)
+        if d <= 0 or n < 0 or n + d > max_len:
+            assert torch.all(out[i] == -7.0), i
+            continue
+        live += 1
+        check({k: v[i:i + 1] for k, v in x.items()}, [n], parents[i:i + 1], [d], out[i:i + 1],
+              128**-0.5)
+    assert live == 7
+    with pytest.raises(_lib.ReefError, match="0x201"):
+        K.check_device_error()
+    none = run(x, [5] * len(rows), parents, [0] * len(rows))  # nobody has any
+    assert torch.all(none == -7.0)
+
+
 def test_on_another_stream_and_in_a_graph():
     x = make(2, 8, 8, 1, 700, seed=31)
     lens = torch.tensor([690, 333], dtype=torch.int32, device="cuda")
