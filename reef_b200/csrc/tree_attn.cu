@@ -494,6 +494,7 @@ __global__ void __launch_bounds__(kTThreads, kPerSm)
       __syncthreads();  // anc is in
     }
     if (ok) ok = mbar_wait(&full[s], (j / kStages) & 1, a.err, kDevTimeoutFull);
+    ok = __all_sync(0xffffffffu, ok);  // what follows is the whole warp's, also after a timeout
     if (ok && tid == 0) waited = j + 1;
     const int key0 = at.tile * kTileKeys + wk;  // this warp's first key
     if (ok && key0 < len + d) {
