@@ -217,22 +217,32 @@ class LlamaLayer:
                 K._take(cache["ks"], "the cache's ks", f32, kept_rows, dev),
                 K._take(cache["v"], "the cache's v", i8, kept_rows + (128,), dev),
                 K._take(cache["vs"], "the cache's vs", f32, kept_rows, dev))
-        if getattr(self, "_tiles", None) is None and not torch.cuda.is_current_stream_capturing():
-            # (a capture would only record the packing, and other streams may call next)
-            self._decode_tiles()
-            torch.cuda.current_stream(dev).synchronize()
         # (kept for good: a captured call goes on using its own)
         kept = self.__dict__.setdefault("_verify_ws", {})
         ws = kept.get((drafts, max_len))
+        if ws is None or getattr(self, "_tiles", None) is None:
+            with torch.cuda.device(dev):
+                ws = self._prepare_verify(drafts, max_len)
+        K._call_on(dev, "reef_b200_llama_verify_forward", C.byref(self.desc), drafts, *args,
+                   max_len, ws.data_ptr(), ws.numel())
+        return y
+
+    def _prepare_verify(self, drafts: int, max_len: int) -> torch.Tensor:
+        """What verify's first call of a size makes, on the layer's device (the current
+        one here); returns the workspace."""
+        if getattr(self, "_tiles", None) is None and not torch.cuda.is_current_stream_capturing():
+            # (a capture would only record the packing, and other streams may call next)
+            self._decode_tiles()
+            torch.cuda.current_stream().synchronize()
+        ws = self._verify_ws.get((drafts, max_len))
         if ws is None:
             n = _lib.lib().reef_b200_llama_verify_workspace_bytes(C.byref(self.desc), drafts,
                                                                   max_len)
             if n == 0:
                 raise ValueError("invalid description of a pass over drafted tokens")
-            ws = kept[drafts, max_len] = torch.empty(n, dtype=torch.uint8, device=dev)
-        K._call_on(dev, "reef_b200_llama_verify_forward", C.byref(self.desc), drafts, *args,
-                   max_len, ws.data_ptr(), ws.numel())
-        return y
+            ws = torch.empty(n, dtype=torch.uint8, device=self.w_qkv.device)
+            self._verify_ws[drafts, max_len] = ws
+        return ws
 
     def host_weights(self) -> dict:
         """This rank's weights on the host (numpy), for the reference checks."""

@@ -212,3 +212,55 @@ def test_verify_refuses_a_shard_of_the_all_gather_plan():
     for fine in (dict(world=2), dict(tp_mode=RL.TP_ALLGATHER)):
         with pytest.raises(ValueError, match="CUDA"):
             host_layer(**fine).verify(x, lens, host_cache())
+
+
+def test_verify_prepares_on_the_layers_device(monkeypatch):
+    """Tiles and workspace of a layer whose device is not the current one: every CUDA call
+    of the preparation is made with it current, and once."""
+    current, made = [], []
+
+    class Device:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            current.append(self.dev)
+
+        def __exit__(self, *_):
+            current.pop()
+
+    class Stream:
+        def synchronize(self):
+            made.append(("synchronize", list(current)))
+
+    class Lib:
+        def reef_b200_llama_verify_workspace_bytes(self, *_):
+            made.append(("workspace", list(current)))
+            return 256
+
+    layer = host_layer(desc=_lib.LlamaLayerDesc(), _tiles=None)
+
+    def tiles():
+        made.append(("tiles", list(current)))
+        layer._tiles = {}
+
+    def capturing():
+        made.append(("capturing", list(current)))
+        return False
+
+    layer._decode_tiles = tiles
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *_: Stream())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", capturing)
+    monkeypatch.setattr(_lib, "lib", Lib)
+    calls = []
+    monkeypatch.setattr(K, "_call_on", lambda dev, name, *a: calls.append((dev, name)))
+    dev = layer.w_qkv.device
+    x, lens = torch.zeros((4, 64)), torch.zeros(2, dtype=torch.int32)
+    for _ in range(2):
+        layer.verify(x, lens, host_cache())
+    assert made == [(n, [dev]) for n in ("capturing", "tiles", "synchronize", "workspace")]
+    layer.verify(torch.zeros((6, 64)), lens, host_cache())
+    assert made[4:] == [("workspace", [dev])]
+    assert calls == [(dev, "reef_b200_llama_verify_forward")] * 3
