@@ -155,6 +155,29 @@ def test_a_capture_as_the_first_call_and_other_drafts_between_replays():
     assert torch.equal(y, want) and all(int(j[0]) == 0xff for j in junk)
 
 
+def test_the_layers_caches_in_one_stack():
+    """Each layer's cache a part of one tensor, which one call compacts."""
+    lens, t, max_len, n = [21, 4], 5, 64, 2
+    layers = [RL.LlamaLayer(SHAPE, 2, 8, seed=20 + i) for i in range(n)]
+    apart = [history(layer, lens, max_len, 30 + i) for i, layer in enumerate(layers)]
+    stack = {c: torch.stack([a[c] for a in apart]) for c in ("k", "ks", "v", "vs")}
+    parts = [{c: v[i] for c, v in stack.items()} | {"max_len": max_len} for i in range(n)]
+    x = torch.randn((2 * t, 512), device="cuda", generator=torch.Generator(device="cuda").manual_seed(3))
+    parents = i32([[-1, 0, 0, 2, 1], [-1, 0, 1, 1, 3]])
+    path, accepted = i32([[0, 2, 3, -1, -1], [0, 1, 3, 4, -1]]), i32([3, 4])
+    a = b = x
+    for layer, one, part in zip(layers, apart, parts):
+        a, b = layer.verify(a, i32(lens), one, parents), layer.verify(b, i32(lens), part, parents)
+    assert torch.equal(a, b)
+    new = K.kv_compact_i8(*stack.values(), i32(lens), path, accepted)
+    for one in apart:
+        K.kv_compact_i8(one["k"], one["ks"], one["v"], one["vs"], i32(lens), path, accepted)
+    assert new.tolist() == [24, 8]
+    for i, one in enumerate(apart):
+        for c in stack:
+            assert torch.equal(stack[c][i], one[c]), (i, c)
+
+
 def test_refusals():
     layer = RL.LlamaLayer(SHAPE, 2, 8, seed=8)
     cache = layer.alloc_cache(64)
