@@ -11,6 +11,9 @@ GEMM sweep.  The recipe behind the summaries in profiles/.
     python profile_cases.py sweep [--out sweep.json] [--tp 1]
     torchrun --nproc-per-node N profile_cases.py tp [--chunks 1,2,4 --steps 20]
     python profile_cases.py stream [--sizes 35,69,138,276]
+    python profile_cases.py operator --name tree_2x64_16k
+    python profile_cases.py operator_timing [--name tree]
+    python profile_cases.py verify_timing
 
 Each single-kernel case allocates its seeded inputs once, launches the kernel
 twice (a warm-up launch, then the one to capture: ``ncu -k regex:<name> -s 1
@@ -30,6 +33,14 @@ one JSON line per point with its roofline fraction (tensor-bound against twice
 the measured burst bf16 rate for M >= 1024, HBM-bound against the measured
 copy bandwidth below).  Operands rotate through enough copies that every call
 reads them from DRAM, not L2.
+
+``operator`` launches one of perf/operators.py's listed cases twice, for a
+capture; ``operator_timing`` times the kernels of every listed case whose name
+holds --name, from a CUDA graph: its inputs in L2 where they fit (three sets in
+turn), and cold, each call behind a read of 512 MiB whose own time is taken off
+(the two graphs in turn, the median of the differences).  ``verify_timing`` times
+the Llama layer on drafted tokens next to the decode step (Llama-70B's TP=8
+shard, 4096-row caches, four layers in turn).
 """
 from __future__ import annotations
 
@@ -308,6 +319,104 @@ SWEEP_NK = ((4096, 4096), (11008, 4096), (4096, 11008), (28672, 8192), (8192, 28
 L2_BYTES = 126 << 20
 
 
+def _operators():
+    import importlib.util
+    here = os.path.dirname(os.path.abspath(__file__))
+    spec = importlib.util.spec_from_file_location("operators", os.path.join(here, "perf", "operators.py"))
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    mod.own = True
+
+    def call(s):  # (the case's own output takes the int8 rows back to float with torch)
+        if s["case"]["op"] == "add_rms":
+            return K.add_rmsnorm_quant(s["x"], s["residual"], s["gain"], s["eps"])
+        return mod.run(s)
+
+    return mod, call
+
+
+def operator(name: str) -> None:
+    mod, call = _operators()
+    s = mod.prepare(next(c for c in mod.listed() if c["name"] == name), 1)
+    for _ in range(2):
+        call(s)
+    torch.cuda.synchronize()
+
+
+def _graph(f, calls: int):
+    f(0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for i in range(calls):
+            f(i)
+    return graph
+
+
+def _replay_us(graph) -> float:
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    a.record()
+    graph.replay()
+    b.record()
+    torch.cuda.synchronize()
+    return a.elapsed_time(b) * 1e3
+
+
+def operator_timing(part: str, calls: int = 24, reps: int = 15) -> None:
+    mod, call = _operators()
+    big = torch.zeros(1 << 27, device="cuda")
+    into = torch.zeros((), device="cuda")
+    for case in mod.listed():
+        if part not in case["name"]:
+            continue
+        sets = [mod.prepare(case, i) for i in range(3)]
+
+        def cold(i):
+            torch.sum(big, 0, out=into)
+            call(sets[i % 3])
+
+        warm = _graph(lambda i: call(sets[i % 3]), calls)
+        both, read = _graph(cold, calls), _graph(lambda i: torch.sum(big, 0, out=into), calls)
+        near, far = [], []
+        for _ in range(reps):
+            near.append(_replay_us(warm) / calls)
+            far.append((_replay_us(both) - _replay_us(read)) / calls)
+        near.sort()
+        far.sort()
+        print(f"{case['name']:26s} in L2 {near[reps // 2]:8.2f} us   cold {far[reps // 2]:8.2f} us "
+              f"({far[2]:.2f} to {far[-3]:.2f})", flush=True)
+
+
+def verify_timing(copies: int = 4, calls: int = 8, reps: int = 20) -> None:
+    from reef_b200.layer import LLAMA_70B, LlamaLayer
+    max_len = 4096
+    for batch, drafts in ((64, 1), (64, 2), (32, 4), (16, 8), (2, 64), (1, 8)):
+        g = torch.Generator(device="cuda").manual_seed(7)
+        layers = [LlamaLayer(LLAMA_70B, batch, 8, seed=11 + c, world=8, rank=0)
+                  for c in range(copies)]
+        caches = [one.alloc_cache(max_len) for one in layers]
+        for c in caches:
+            for n in ("k", "v"):
+                c[n].random_(-127, 128, generator=g)
+                c[n + "s"].uniform_(0.005, 0.02, generator=g)
+        x = torch.randn((batch * drafts, 8192), generator=g, device="cuda")
+        y = torch.empty_like(x)
+        lens = torch.full((batch,), max_len - drafts, dtype=torch.int32, device="cuda")
+        tree = torch.tensor([[(t - 1) // 2 if t else -1 for t in range(drafts)]] * batch,
+                            dtype=torch.int32, device="cuda")
+        steps = {"verify": lambda i: layers[i % copies].verify(x, lens, caches[i % copies], tree,
+                                                               out=y)}
+        if drafts == 1:
+            steps["decode"] = lambda i: layers[i % copies].decode(x, lens, caches[i % copies], out=y)
+        for name, f in steps.items():
+            for i in range(copies):
+                f(i)
+            graph = _graph(f, calls)
+            us = sorted(_replay_us(graph) / calls for _ in range(reps))[reps // 2]
+            print(f"{name} {batch} x {drafts} over {max_len - drafts} rows: {us:.1f} us", flush=True)
+        del layers, caches
+
+
 def _peaks() -> dict:
     root = os.path.dirname(os.path.abspath(__file__))
     try:
@@ -407,7 +516,9 @@ def sweep(out: str | None, tps=(1,), iters: int = 20, reps: int = 3) -> None:
 def main() -> None:
     ap = argparse.ArgumentParser()
     ap.add_argument("case", choices=["gemm", "flash", "qkv", "decode", "decode_step", "layer",
-                                     "layer_timing", "sweep", "tp", "stream"])
+                                     "layer_timing", "sweep", "tp", "stream", "operator",
+                                     "operator_timing", "verify_timing"])
+    ap.add_argument("--name", default="", help="operator, operator_timing: a case, or part of names")
     ap.add_argument("--sizes", default="35,69,138,276", help="stream: working sets in MB")
     ap.add_argument("--chunks", default="1,2,4", help="tp: chunk counts of the all-gather plan")
     ap.add_argument("--steps", type=int, default=3)
@@ -439,6 +550,12 @@ def main() -> None:
         decode_step(a.steps)
     elif a.case == "layer":
         layer(a.batch, a.steps)
+    elif a.case == "operator":
+        operator(a.name)
+    elif a.case == "operator_timing":
+        operator_timing(a.name)
+    elif a.case == "verify_timing":
+        verify_timing()
     elif a.case == "layer_timing":
         layer_timing(a.batch, max(a.steps, 5))
     else:
