@@ -45,6 +45,16 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// A word of an ldmatrix .trans over int8 pairs: bytes (k, d), (k, d+1),
+// (k+1, d), (k+1, d+1).  Out: the f16 pairs {(k, d), (k+1, d)} and
+// {(k, d+1), (k+1, d+1)}, each value v + 1152 exactly (byte v ^ 0x80 = v +
+// 128 as the mantissa under the exponent byte 0x64, i.e. 1024 + v + 128).
+__device__ __forceinline__ void split_biased(uint32_t w, uint32_t& even, uint32_t& odd) {
+  const uint32_t u = w ^ 0x80808080u;
+  even = __byte_perm(u, 0x64646464u, 0x4240);
+  odd = __byte_perm(u, 0x64646464u, 0x4341);
+}
+
 // 2^x (ex2.approx.ftz: 2 ulp; -inf -> 0, results below 2^-126 flush to 0)
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;

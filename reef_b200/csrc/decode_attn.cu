@@ -96,16 +96,6 @@ static_assert(DL::merge_bytes(8) <= DL::kKV, "G <= 8 merges inside a stage");
 static_assert(DL::bytes(8) <= 232448 / 2 - 1024, "two CTAs per SM up to G = 8");
 static_assert(DL::bytes(16) <= 232448 - 1024, "one CTA per SM at G = 16");
 
-// A word of an ldmatrix .trans over int8 pairs: bytes (k, d), (k, d+1),
-// (k+1, d), (k+1, d+1).  Out: the f16 pairs {(k, d), (k+1, d)} and
-// {(k, d+1), (k+1, d+1)}, each value v + 1152 exactly (byte v ^ 0x80 = v +
-// 128 as the mantissa under the exponent byte 0x64, i.e. 1024 + v + 128).
-__device__ __forceinline__ void split_biased(uint32_t w, uint32_t& even, uint32_t& odd) {
-  const uint32_t u = w ^ 0x80808080u;
-  even = __byte_perm(u, 0x64646464u, 0x4240);
-  odd = __byte_perm(u, 0x64646464u, 0x4341);
-}
-
 __device__ __forceinline__ int seq_len(const DecodeArgs& a, int b) {
   return a.lens != nullptr ? a.lens[b] : a.len;
 }

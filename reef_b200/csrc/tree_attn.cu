@@ -179,16 +179,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-// D (16x8 f32) += A (16x16 f16, row) x B (16x8 f16, col)
-__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                        uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
-      "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
 // Two int8 codes with their sign bits flipped, each under the exponent byte
 // 0x64, i.e. the f16 values code + 1152 -> the codes, exactly
 __device__ __forceinline__ uint32_t unbias(uint32_t x) {
@@ -197,13 +187,11 @@ __device__ __forceinline__ uint32_t unbias(uint32_t x) {
                             *reinterpret_cast<const __half2*>(&bias));
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// A word of an ldmatrix .trans over int8 pairs: bytes (k, d), (k, d + 1),
-// (k + 1, d), (k + 1, d + 1).  Out: the f16 pairs {(k, d), (k + 1, d)} and
-// {(k, d + 1), (k + 1, d + 1)}.
+// split_biased's pairs without the bias: the codes themselves
 __device__ __forceinline__ void split_codes(uint32_t w, uint32_t& even, uint32_t& odd) {
-  const uint32_t u = w ^ 0x80808080u;
-  even = unbias(__byte_perm(u, 0x64646464u, 0x4240));
-  odd = unbias(__byte_perm(u, 0x64646464u, 0x4341));
+  split_biased(w, even, odd);
+  even = unbias(even);
+  odd = unbias(odd);
 }
 
 // log2 and reciprocal of a V scale (2^-22 off at most); of one that counts as
@@ -605,10 +593,10 @@ __global__ void __launch_bounds__(kTThreads, kPerSm)
           // the tile's own sum, then one rounded add: the tensor cores' adds
           // truncate, and a long row of them would show
           float t0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, t1[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          mma_f16(t0, va, pl[nt][0], pl[nt][1]);
-          mma_f16(t1, vc, pl[nt][0], pl[nt][1]);
-          mma_f16(t0, va, ph[nt][0], ph[nt][1]);
-          mma_f16(t1, vc, ph[nt][0], ph[nt][1]);
+          mma_f16_16816(t0, va, pl[nt][0], pl[nt][1]);
+          mma_f16_16816(t1, vc, pl[nt][0], pl[nt][1]);
+          mma_f16_16816(t0, va, ph[nt][0], ph[nt][1]);
+          mma_f16_16816(t1, vc, ph[nt][0], ph[nt][1]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             o[2 * cc][nt][e] += t0[e];
