@@ -306,9 +306,9 @@ __global__ void __launch_bounds__(kChunks * 32)
 // hold the bits rmsnorm_quant gives on h.  The row stays in registers, so x and
 // residual are read once and h is never read back; h may be x or residual:
 // a thread reads its elements before it writes them, and nobody else reads
-// them.  13 bytes an element: bound by HBM, 127.6 us for 16384 rows of 4096 (6.8 TB/s,
-// what a plain copy reaches), 4.9 us for 64 rows of 8192, where the launch and one
-// round trip are what there is.
+// them.  13 bytes an element: bound by HBM, 128 us for 16384 rows of 4096 (6.8 TB/s,
+// what a plain copy reaches; 133 with nothing of it in L2), 5.1 us for 64 rows of 8192
+// (cold 6.9), where the launch and one round trip are what there is.
 template <int P>
 __global__ void __launch_bounds__(kChunks * 32)
     add_rmsnorm_quant_kernel(int width, float eps, const float* x, const float* residual,

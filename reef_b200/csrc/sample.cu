@@ -45,11 +45,14 @@
 // takes its place.
 //
 // What bounds it: 131 MB of logits (256 rows of 128000) would take 20 us to read; no
-// filter takes 141 us, top-p 246.  Two CTAs of 512 threads fill an SM's
+// filter takes 141 us, top-p 248 (cold 260).  Two CTAs of 512 threads fill an SM's
 // shared memory and registers, and each row's chain is 15 to 35 us long: the copy and
 // the maximum 4, the weights 10 (50 instructions each where every second one is
 // heavy; with the histogram 15), then half a dozen steps of 1 to 4 us that end in a
-// cluster barrier.  A single row of 50257 with top-k: 13 us, all of it that chain.
+// cluster barrier; per instruction issued (0.51 a cycle and scheduler, seven warps) a warp
+// stands 4 cycles at barriers and for the memory order they give, 2.5 at fixed latencies,
+// 2.5 at loads and the tables.  A single row of 50257 with top-k: 14 us (cold 19), all of
+// it that chain.
 // Measured and dropped: two elements to an instruction (no change), the four adds of
 // a thread into the histogram in flight at once (3 % slower), the list weighed in a
 // pass of its own and the histogram in another (341).  Heavy from 2^-27 up instead of

@@ -11,8 +11,8 @@
 // tree_accept: from cur = 0, next cur = the lowest c > cur with parents[c] =
 // cur and tokens[c] = chosen[cur], until there is none; the nodes passed are
 // the path, chosen[cur] of its last node the token that follows.  At most 64
-// steps of two compares and two votes by one warp: bound by the launch (1.4 us for one
-// tree of 8, 2.0 us for 512 of 64).
+// steps of two compares and two votes by one warp: bound by the launch (1.6 us for one
+// tree of 8, 2.3 us for 512 of 64; cold 2.0 and 3.2).
 //
 // kv_compact_i8: row len + i := row len + path[i], i < accepted, for K, V and
 // their scales, in every layer and KV head.  One CTA owns the rows of one
@@ -20,8 +20,8 @@
 // 128 bytes at most: 4 KiB per warp) before it writes any, so a path may be in
 // any order and name a row twice.  Rows already in their place are neither
 // read nor written.  264 bytes a row, read and written once; a CTA has few of them,
-// so one round trip to HBM bounds it: 2.2 us for 32 heads of one sequence, 8.2 us for
-// 16 layers x 32 sequences x 8 heads (18.4 MB of rows, 2.2 TB/s of 6.5).
+// so one round trip to HBM bounds it: 2.5 us for 32 heads of one sequence (cold 2.8), 8.6
+// us for 16 layers x 32 sequences x 8 heads (18.4 MB of rows, 2.1 TB/s of 6.5; cold 11.4).
 #include "common.cuh"
 #include "ops.h"
 

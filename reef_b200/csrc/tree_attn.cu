@@ -32,8 +32,8 @@
 // P^T by f16 mma.sync (the rows are the n = 8 side, so few are padding).
 //
 // More rows, tree_tc_kernel: tcgen05 with a tile of 128 query rows, bound by
-// the exponentials and conversions of the softmax warps and the tensor pipe (S in
-// int8, P'.V twice in f16).  Scores go into two TMEM tiles in turn, so that the
+// the latency of the softmax warps, which go through their steps together (S in
+// int8, P'.V twice in f16 leave the tensor pipe busy for a fifth).  Scores go into two TMEM tiles in turn, so that the
 // next are there before the softmax of one ends; two warpgroups share a tile, a
 // thread holding half of a query row's 128 scores; P' overwrites the scores (its
 // heads in the first 64 columns, the rests in the last) and the product reads it
@@ -48,16 +48,21 @@
 // that all warps have work (64 x 8 drafts, 8 heads on one: 53 -> 41 us); the copies share
 // the maxima and add up at the end.
 //
-// Measured (one call, cold cache): 4 drafts over 499 keys, 32 heads of their own, 8.7
-// us, which is the launch and three round trips (lengths, queries, keys).  64 sequences
-// over up to 4096 keys, 8 heads on one: 1 draft each (70 MB of cache) 26 us, 2 drafts 35, 8
-// drafts (ragged, 54 MB) 34, of which 11 are the shares, the first loads, the epilogues
-// and the join.  Two sequences over 16301 keys, 64 drafts, 64 heads on 8 (68.5 Gflop): 175
-// us, 0.39 Pflop/s of products or 0.78 with the rests; a tile takes 5000 cycles, of which
-// the tensor pipe is busy for 1550.  That is the issue of the softmax warps, two to a
-// scheduler, 17 instructions a score at one in 4.8 cycles each (left out for a
-// measurement, the loads of the scales save 27 us, the rests 11, the exponentials 4).  Up
-// to 32 rows the products bound (2500 cycles a tile).  Measured and dropped: quarter rows in four warpgroups
+// Measured (a call in a graph of them, inputs in L2 where they fit; with everything cold
+// in brackets): 4 drafts over 499 keys, 32 heads of their own, 8.7 us (8.7), which is the
+// launch and three round trips (lengths, queries, keys).  64 sequences over up to 4096
+// keys, 8 heads on one: 1 draft each (70 MB of cache) 26 us, 2 drafts 35, 8 drafts (ragged,
+// 54 MB) 35 (39), of which 11 are the shares, the first loads, the epilogues and the join.
+// Two sequences over 16301 keys, 64 drafts, 64 heads on 8 (68.5 Gflop): 178 us (188), 0.38
+// Pflop/s of products or 0.77 with the rests; a tile takes 5000 cycles, of which the
+// tensor pipe is busy for 1100.  What holds it is latency: a scheduler has two softmax
+// warps, a converter and one that mostly waits, and issues in 0.48 of its cycles (0.42 for
+// 64 x 8).  Per instruction issued, warps stand 2.0 cycles at loads from TMEM and waits
+// for barriers in memory, 1.6 at the fixed latencies of arithmetic, 1.4 at the barrier on
+// which all eight softmax warps meet once a tile: they read scales, take exponentials and
+// wait for scores at the same time.  Left out for a measurement, the loads of the scales
+// save 27 us, the rests 11, the exponentials 4.  Up to 32 rows a tile takes 2500 cycles.
+// Measured and dropped: quarter rows in four warpgroups
 // (they spill; with two copies they do not, and 64 x 8 takes 42 us: what a warp does
 // once a tile counts twice as often), scores taken a tile ahead, a barrier per pair of
 // warps, scores in fragments of 16 x 8 (a quarter of the loads of scales, but 184 us), O

@@ -1,7 +1,9 @@
 // verify.cpp -- the Llama layer on drafted tokens: the decode step with `drafts`
 // new tokens per sequence, each seeing the committed cache rows, itself and its
 // ancestors in the sequence's tree.  Everything but the cache append and the
-// attention is the decode step's own (layer.cpp), on batch * drafts rows.
+// attention is the decode step's own (layer.cpp), on batch * drafts rows.  Llama-70B's
+// TP = 8 shard over 4096 cached rows: 64 x 1 94 us (the decode step: 86, whose attention
+// rounds P to f16 and begins its loads before the append ends), 16 x 8 102, 64 x 2 114.
 #include "comm.h"
 #include "layer.h"
 
