@@ -672,7 +672,9 @@ int reef_b200_llama_layer_forward_events(const reef_b200_llama_layer* layer, con
  * [128] int8 (16-byte aligned), k_scale / v_scale [batch][heads_kv][max_len]
  * fp32 (one scale per token and head).  Every projection uses the skinny
  * W8A8 GEMM; the row-parallel ones all-reduce exactly as in the prefill
- * layer, so every rank's y is bit-identical to TP=1. */
+ * layer, so every rank's y is bit-identical to TP=1.  x, w_o, s_o, w_down and
+ * s_down are laid out as for REEF_B200_TP_ALLREDUCE whatever tp_mode says: a
+ * layer whose weights are REEF_B200_TP_ALLGATHER's must not be given. */
 size_t reef_b200_llama_decode_workspace_bytes(const reef_b200_llama_layer* layer,
                                               size_t max_len);
 int reef_b200_llama_decode_forward(const reef_b200_llama_layer* layer, const float* x, float* y,
